@@ -63,6 +63,20 @@ struct Lib {
   CXG_FN(cxg_relation_pairs_workspace_size);
   CXG_FN(cxg_relation_pairs_count);
   CXG_FN(cxg_relation_pairs_fill);
+  CXG_FN(cxg_rows8_pitch);
+  CXG_FN(cxg_rows8_write);
+  CXG_FN(cxg_rows8_write_at_workspace_size);
+  CXG_FN(cxg_rows8_write_at);
+  CXG_FN(cxg_rows8_read);
+  CXG_FN(cxg_rows8_aggregate_workspace_size);
+  CXG_FN(cxg_rows8_aggregate);
+  CXG_FN(cxg_rows8_wgrad_workspace_size);
+  CXG_FN(cxg_rows8_wgrad);
+  CXG_FN(cxg_residual_norm_max_width);
+  CXG_FN(cxg_residual_norm_keeps);
+  CXG_FN(cxg_residual_norm_forward);
+  CXG_FN(cxg_residual_norm_backward_workspace_size);
+  CXG_FN(cxg_residual_norm_backward);
 #undef CXG_FN
 } lib;
 
@@ -102,6 +116,20 @@ void init(const std::string &path) {
   CXG_FN(cxg_relation_pairs_workspace_size);
   CXG_FN(cxg_relation_pairs_count);
   CXG_FN(cxg_relation_pairs_fill);
+  CXG_FN(cxg_rows8_pitch);
+  CXG_FN(cxg_rows8_write);
+  CXG_FN(cxg_rows8_write_at_workspace_size);
+  CXG_FN(cxg_rows8_write_at);
+  CXG_FN(cxg_rows8_read);
+  CXG_FN(cxg_rows8_aggregate_workspace_size);
+  CXG_FN(cxg_rows8_aggregate);
+  CXG_FN(cxg_rows8_wgrad_workspace_size);
+  CXG_FN(cxg_rows8_wgrad);
+  CXG_FN(cxg_residual_norm_max_width);
+  CXG_FN(cxg_residual_norm_keeps);
+  CXG_FN(cxg_residual_norm_forward);
+  CXG_FN(cxg_residual_norm_backward_workspace_size);
+  CXG_FN(cxg_residual_norm_backward);
 #undef CXG_FN
 }
 
@@ -685,6 +713,432 @@ Tensor linear(const Tensor &x, const Tensor &w, const optional<Tensor> &bias, co
   return linear_product(x, w, false, bias, add);
 }
 
+// ---- rows held in 8 bits ---------------------------------------------------------------------------------------------
+const char *const kTransform = " does not take tensors of a transform (vmap, forward-mode differentiation, tracing)";
+
+int code_of(const Tensor &t) { return t.scalar_type() == at::kFloat ? CXG_F32 : CXG_BF16; }
+
+// A matrix of rows that lie any distance apart, each in one piece; a copy of any other.
+Tensor row_matrix(const Tensor &t, const char *name) {
+  if (!t.is_cuda()) fail(std::string(name) + " must be a CUDA tensor (this backend has no CPU path)");
+  if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16)
+    fail(std::string(name) + " has dtype " + c10::toString(t.scalar_type()) + ", which this operator does not take");
+  if (t.dim() != 2 || t.size(1) == 0) fail(std::string(name) + " must be a matrix with at least one column");
+  if (t.size(1) > (1 << 20)) fail(std::string(name) + " has more than 2^20 columns");
+  const bool rows = t.stride(1) == 1 || t.size(1) == 1;
+  return rows && (t.stride(0) >= t.size(1) || t.size(0) <= 1) ? t : t.contiguous();
+}
+int64_t row_step(const Tensor &t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+void same_device(const Tensor &a, const Tensor &b, const char *name) {
+  if (a.device() != b.device()) fail(std::string(name) + " is on another device");
+}
+
+// codes [rows + 1, pitch], scales [rows + 1, pitch / 32]: the last row of zeros
+struct Held {
+  Tensor codes, scales;
+  int64_t rows() const { return codes.size(0) - 1; }
+};
+
+Held held_like(int64_t rows, int64_t width, at::Device device) {
+  const int64_t pitch = lib.cxg_rows8_pitch(static_cast<int>(width));
+  const auto opt = at::TensorOptions().dtype(at::kByte).device(device);
+  return {at::empty({rows + 1, pitch}, opt), at::empty({rows + 1, pitch / 32}, opt)};
+}
+
+Held quantize(const Tensor &x_in) {
+  if (for_torch(x_in)) fail(std::string("quantize_rows") + kTransform);
+  const Tensor x = row_matrix(x_in, "x");
+  c10::cuda::CUDAGuard guard(x.device());
+  Held h = held_like(x.size(0), x.size(1), x.device());
+  check(lib.cxg_rows8_write(x.data_ptr(), code_of(x), row_step(x), x.size(0), static_cast<int>(x.size(1)), h.codes.data_ptr(),
+                            h.scales.data_ptr(), 1, stream_of(x)),
+        "cxg_rows8_write");
+  return h;
+}
+
+// Rows of zeros.
+Held held_zeros(int64_t rows, int64_t width, at::Device device) {
+  if (rows < 0 || width <= 0 || width > (1 << 20)) fail("Rows8: bad sizes");
+  if (!device.is_cuda()) fail("Rows8: the device must be a CUDA device (this backend has no CPU path)");
+  c10::cuda::CUDAGuard guard(device);
+  Held h = held_like(rows, width, device);
+  h.codes.zero_();
+  h.scales.zero_();
+  return h;
+}
+
+// Rows of x over rows [0, n) of what is held, or over the rows that index names (owner: the words of cxg_rows8_write_at).
+void quantize_into(const Tensor &x_in, const Tensor &codes, const Tensor &scales, int64_t width, const optional<Tensor> &index,
+                   const optional<Tensor> &owner) {
+  if (for_torch(x_in)) fail(std::string("quantize_rows") + kTransform);
+  const Tensor x = row_matrix(x_in, "x");
+  const int64_t rows = codes.size(0) - 1, n = x.size(0);
+  same_device(codes, x, "x");
+  if (x.size(1) != width) fail("quantize_rows: x has " + std::to_string(x.size(1)) + " columns, the rows have " + std::to_string(width));
+  c10::cuda::CUDAGuard guard(x.device());
+  void *st = stream_of(x);
+  if (!index) {
+    if (n > rows) fail("quantize_rows: x has " + std::to_string(n) + " rows, there are " + std::to_string(rows));
+    check(lib.cxg_rows8_write(x.data_ptr(), code_of(x), row_step(x), n, static_cast<int>(width), codes.data_ptr(), scales.data_ptr(),
+                              0, st),
+          "cxg_rows8_write");
+  } else {
+    of_type(*index, "index", {at::kLong});
+    same_device(codes, *index, "index");
+    if (index->dim() != 1 || index->size(0) != n) fail("quantize_rows: index must name a row for every row of x");
+    size_t need = 0;
+    check(lib.cxg_rows8_write_at_workspace_size(n, &need), "cxg_rows8_write_at_workspace_size");
+    const Workspace ws = workspace_on(x.device().index(), st, static_cast<int64_t>(need), "");
+    check(lib.cxg_rows8_write_at(x.data_ptr(), code_of(x), row_step(x), n, static_cast<int>(width), index->data_ptr<int64_t>(),
+                                 codes.data_ptr(), scales.data_ptr(), rows, owner->data_ptr<int32_t>(), ws.data(), ws.bytes(), st),
+          "cxg_rows8_write_at");
+  }
+  // a backward pass that was to read these rows hears of it
+  codes.unsafeGetTensorImpl()->bump_version();
+  scales.unsafeGetTensorImpl()->bump_version();
+}
+
+at::ScalarType row_type(const std::string &who, at::ScalarType t) {
+  if (t != at::kFloat && t != at::kBFloat16) fail(who + ": dtype must be float32 or bfloat16");
+  return t;
+}
+
+Tensor dequantize(const Tensor &codes, const Tensor &scales, int64_t width, const optional<Tensor> &index, at::ScalarType type) {
+  row_type("dequantize_rows", type);
+  c10::cuda::CUDAGuard guard(codes.device());
+  const int64_t rows = codes.size(0) - 1;
+  if (index) {
+    of_type(*index, "index", {at::kLong});
+    same_device(codes, *index, "index");
+    if (index->dim() != 1) fail("dequantize_rows: index must be a vector");
+  }
+  Tensor out = at::empty({index ? index->size(0) : rows, width}, codes.options().dtype(type));
+  check(lib.cxg_rows8_read(codes.data_ptr(), scales.data_ptr(), rows, static_cast<int>(width),
+                           index ? index->data_ptr<int64_t>() : nullptr, out.size(0), out.data_ptr(), code_of(out), width,
+                           stream_of(codes)),
+        "cxg_rows8_read");
+  return out;
+}
+
+Tensor rows8_aggregate(const Tensor &codes, const Tensor &scales, int64_t width, const Tensor &ptr, const Tensor &idx,
+                       int64_t num_node, bool mean, const optional<Tensor> &edge_value, at::ScalarType type, int64_t split) {
+  row_type("rows8_aggregate", type);
+  index_of(ptr, "ptr");
+  index_of(idx, "idx");
+  same_device(codes, ptr, "ptr");
+  same_device(codes, idx, "idx");
+  if (ptr.dim() != 1 || ptr.size(0) < 1 || idx.dim() != 1) fail("rows8_aggregate: ptr and idx must be vectors, ptr of at least one entry");
+  const int64_t n = rows_of(ptr, num_node);
+  if (edge_value) {
+    if (mean) fail("rows8_aggregate: a mean takes no edge values");
+    if (for_torch(*edge_value)) fail(std::string("rows8_aggregate") + kTransform);
+    if (recorded(*edge_value)) fail("rows8_aggregate: there is no gradient for edge values");
+    f32(*edge_value, "edge_value");
+    same_device(codes, *edge_value, "edge_value");
+    if (edge_value->numel() != idx.size(0)) fail("rows8_aggregate: one edge value per edge");
+  }
+  c10::cuda::CUDAGuard guard(codes.device());
+  Tensor y = at::empty({n, width}, codes.options().dtype(type));
+  size_t need = 0;
+  check(lib.cxg_rows8_aggregate_workspace_size(idx.size(0), static_cast<int>(width), static_cast<int>(split), &need),
+        "cxg_rows8_aggregate_workspace_size");
+  void *st = stream_of(codes);
+  const Workspace ws = workspace_on(codes.device().index(), st, static_cast<int64_t>(need), "spmm");
+  check(lib.cxg_rows8_aggregate(codes.data_ptr(), scales.data_ptr(), codes.size(0) - 1, static_cast<int>(width), ptr.data_ptr(),
+                                static_cast<int>(ptr.element_size()), idx.data_ptr(), static_cast<int>(idx.element_size()),
+                                edge_value ? edge_value->data_ptr<float>() : nullptr, n, idx.size(0), mean ? CXG_MEAN : CXG_SUM,
+                                static_cast<int>(split), y.data_ptr(), code_of(y), ws.data(), ws.bytes(), st),
+        "cxg_rows8_aggregate");
+  return y;
+}
+
+// (dy^T . rows [n, width], column sums of dy [n] or none), fp32
+std::pair<Tensor, Tensor> rows8_weight_grad(const Tensor &codes, const Tensor &scales, int64_t width, const Tensor &dy_in, bool bias) {
+  if (for_torch(dy_in)) fail(std::string("rows8_weight_grad") + kTransform);
+  const Tensor dy = row_matrix(dy_in, "grad");
+  same_device(codes, dy, "grad");
+  const int64_t m = dy.size(0), n = dy.size(1);
+  if (m > codes.size(0) - 1) fail("rows8_weight_grad: grad has " + std::to_string(m) + " rows, there are " + std::to_string(codes.size(0) - 1));
+  c10::cuda::CUDAGuard guard(dy.device());
+  const auto opt = dy.options().dtype(at::kFloat);
+  Tensor dw = at::empty({n, width}, opt), db = bias ? at::empty({n}, opt) : Tensor();
+  size_t need = 0;
+  check(lib.cxg_rows8_wgrad_workspace_size(m, static_cast<int>(width), static_cast<int>(n), &need), "cxg_rows8_wgrad_workspace_size");
+  void *st = stream_of(dy);
+  const Workspace ws = workspace_on(dy.device().index(), st, static_cast<int64_t>(need), "");
+  check(lib.cxg_rows8_wgrad(codes.data_ptr(), scales.data_ptr(), m, static_cast<int>(width), dy.data_ptr(), code_of(dy), row_step(dy),
+                            static_cast<int>(n), 0, dw.data_ptr<float>(), bias ? db.data_ptr<float>() : nullptr, ws.data(),
+                            ws.bytes(), st),
+        "cxg_rows8_wgrad");
+  return {dw, db};
+}
+
+// The result of a linear transform in the input's type: the tensor-core kernel for the fp32 matrices it takes, else torch's.
+Tensor plain_linear(const Tensor &x, const Tensor &w, const optional<Tensor> &bias, const optional<Tensor> &add) {
+  const bool add_fits = !add || (dense_rows(*add) && add->sizes() == at::IntArrayRef({x.size(0), w.size(0)}));
+  if (linear_fits(x, w) && add_fits && (!bias || bias->is_contiguous())) return linear_product(x, w, false, bias, add);
+  const Tensor y = at::linear(x, w, bias);
+  return add ? *add + y : y;
+}
+
+// A linear transform whose backward pass reads its input in 8 bits.
+class LinearKept8Function : public torch::autograd::Function<LinearKept8Function> {
+ public:
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const optional<Tensor> &bias,
+                        const optional<Tensor> &add, const optional<Tensor> &codes, const optional<Tensor> &scales) {
+    Held held;
+    if (codes)
+      held = {*codes, *scales};
+    else if (w.requires_grad())  // nobody reads the rows otherwise
+      held = quantize(x);
+    ctx->save_for_backward({w, held.codes, held.scales});
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["bias_bf16"] = bias && bias->scalar_type() == at::kBFloat16;
+    ctx->saved_data["add"] = add.has_value();
+    return plain_linear(x, w, bias, add);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    if (at::GradMode::is_enabled()) fail("linear_kept8: the rows it keeps in 8 bits have no second derivative");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &w = saved[0];
+    const Tensor g = grads[0].contiguous();
+    c10::cuda::CUDAGuard guard(g.device());
+    Tensor dx, dw, db;
+    const bool bias = ctx->saved_data["bias"].toBool(), need_db = bias && ctx->needs_input_grad(2);
+    const bool need_add = ctx->saved_data["add"].toBool() && ctx->needs_input_grad(bias ? 3 : 2);
+    if (ctx->needs_input_grad(0))
+      dx = dense_rows(g) && dense_rows(w) &&
+                   lib.cxg_linear_f32_supported(g.size(0), static_cast<int>(g.size(1)), static_cast<int>(w.size(1)))
+               ? linear_product(g, w, true, c10::nullopt, c10::nullopt)
+               : at::mm(g, w);
+    if (ctx->needs_input_grad(1)) {
+      const auto grad = rows8_weight_grad(saved[1], saved[2], w.size(1), g, need_db);
+      dw = grad.first.to(w.scalar_type());
+      db = grad.second;
+    } else if (need_db) {
+      db = g.sum(0, false, at::kFloat);
+    }
+    if (need_db) db = db.to(ctx->saved_data["bias_bf16"].toBool() ? at::kBFloat16 : at::kFloat);
+    return {dx, dw, db, need_add ? grads[0] : Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor linear_kept8(Tensor x, Tensor w, optional<Tensor> bias, optional<Tensor> add, const optional<Tensor> &codes,
+                    const optional<Tensor> &scales) {
+  if (for_torch(x, w, bias, add)) fail(std::string("linear_kept8") + kTransform);
+  if (at::autocast::is_autocast_enabled(at::kCUDA)) {
+    const auto type = row_type("linear_kept8 under autocast", at::autocast::get_autocast_dtype(at::kCUDA));
+    x = x.to(type), w = w.to(type);
+    if (bias) bias = bias->to(type);
+    if (add) add = add->to(type);
+  }
+  for (const Tensor *t : {&x, &w}) {
+    if (!t->is_cuda()) fail("linear_kept8: x and weight must be CUDA tensors (this backend has no CPU path)");
+    if (t->dim() != 2 || t->size(1) == 0) fail("linear_kept8: x and weight must be matrices");
+  }
+  row_type("linear_kept8", x.scalar_type());
+  if (w.scalar_type() != x.scalar_type() || (bias && bias->scalar_type() != x.scalar_type()) || (add && add->scalar_type() != x.scalar_type()))
+    fail("linear_kept8: x, weight, bias and add must be of one type");
+  if (w.size(1) != x.size(1) || w.size(0) == 0) fail("linear_kept8: weight must be [out, " + std::to_string(x.size(1)) + "]");
+  if (bias && (bias->dim() != 1 || bias->size(0) != w.size(0))) fail("linear_kept8: bias must be [" + std::to_string(w.size(0)) + "]");
+  if (add && (add->dim() != 2 || add->size(0) != x.size(0) || add->size(1) != w.size(0))) fail("linear_kept8: add must have the shape of the result");
+  same_device(x, w, "weight");
+  if (bias) same_device(x, *bias, "bias");
+  if (add) same_device(x, *add, "add");
+  if (codes) {
+    same_device(x, *codes, "kept");
+    if (codes->size(0) - 1 != x.size(0) || codes->size(1) != lib.cxg_rows8_pitch(static_cast<int>(x.size(1))))
+      fail("linear_kept8: kept must hold the rows of x");
+  }
+  c10::cuda::CUDAGuard guard(x.device());
+  c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);
+  if (recorded(x, w, bias, add))
+    return LinearKept8Function::apply(x, w, bias, add, codes, scales);
+  return plain_linear(x, w, bias, add);
+}
+
+// ---- the step between two blocks of a residual network -----------------------------------------------------------------
+struct ResidualOptions {
+  bool post, next, layer, keep;
+  double eps;
+};
+
+const float *param(const optional<Tensor> &t) { return t ? t->data_ptr<float>() : nullptr; }
+
+cxg_residual_desc describe_residual(const Tensor &x, const optional<Tensor> &f, const optional<Tensor> &gate, const optional<Tensor> &scale,
+                                    const optional<Tensor> &w2, const optional<Tensor> &b2, const optional<Tensor> &w1,
+                                    const optional<Tensor> &b1, const ResidualOptions &o) {
+  cxg_residual_desc d = {};
+  d.x = x.data_ptr();
+  if (f) d.f = f->data_ptr();
+  if (gate) {
+    d.gate = gate->data_ptr();
+    d.gate_mode = gate->dim() == 2 && gate->size(1) == x.size(1) && x.size(1) > 1 ? CXG_GATE_VALUE : CXG_GATE_ROW;
+  }
+  d.scale = param(scale), d.post_weight = param(w2), d.post_bias = param(b2), d.next_weight = param(w1), d.next_bias = param(b1);
+  d.n = x.size(0);
+  d.width = static_cast<int32_t>(x.size(1));
+  d.dtype = code_of(x);
+  d.layer = o.layer, d.post = o.post, d.next = o.next;
+  d.eps = static_cast<float>(o.eps);
+  return d;
+}
+
+// {y (with f), h (with next), codes and scales of h (with keep)}
+variable_list residual_forward(const Tensor &x, const optional<Tensor> &f, const optional<Tensor> &gate, const optional<Tensor> &scale,
+                               const optional<Tensor> &w2, const optional<Tensor> &b2, const optional<Tensor> &w1,
+                               const optional<Tensor> &b1, const ResidualOptions &o) {
+  cxg_residual_desc d = describe_residual(x, f, gate, scale, w2, b2, w1, b1, o);
+  variable_list out;
+  if (f) {
+    out.push_back(at::empty_like(x));
+    d.y = out.back().data_ptr();
+  }
+  Tensor h;
+  if (o.next) {
+    h = at::empty_like(x);
+    out.push_back(h);
+    d.h = h.data_ptr();
+  }
+  Held held;
+  bool with_h = false;
+  if (o.keep) {
+    held = held_like(x.size(0), x.size(1), x.device());
+    d.codes = held.codes.data_ptr();
+    with_h = d.n > 0 && lib.cxg_residual_norm_keeps(&d) == 1;
+    d.codes = with_h ? held.codes.data_ptr() : nullptr;
+    d.scales = with_h ? held.scales.data_ptr() : nullptr;
+  }
+  check(lib.cxg_residual_norm_forward(&d, stream_of(x)), "cxg_residual_norm_forward");
+  if (o.keep) {
+    if (!with_h)
+      check(lib.cxg_rows8_write(h.data_ptr(), code_of(h), h.size(1), h.size(0), static_cast<int>(h.size(1)), held.codes.data_ptr(),
+                                held.scales.data_ptr(), 1, stream_of(h)),
+            "cxg_rows8_write");
+    out.push_back(held.codes);
+    out.push_back(held.scales);
+  }
+  return out;
+}
+
+class ResidualNormFunction : public torch::autograd::Function<ResidualNormFunction> {
+ public:
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const optional<Tensor> &f, const optional<Tensor> &gate,
+                               const optional<Tensor> &scale, const optional<Tensor> &w2, const optional<Tensor> &b2,
+                               const optional<Tensor> &w1, const optional<Tensor> &b1, bool post, bool next, bool layer, double eps,
+                               bool keep) {
+    const ResidualOptions o{post, next, layer, keep, eps};
+    variable_list out = residual_forward(x, f, gate, scale, w2, b2, w1, b1, o);
+    auto or_none = [](const optional<Tensor> &t) { return t ? *t : Tensor(); };
+    ctx->save_for_backward({x, or_none(f), or_none(gate), or_none(scale), or_none(w2), or_none(b2), or_none(w1), or_none(b1)});
+    ctx->saved_data["options"] = std::vector<bool>{post, next, layer};
+    ctx->saved_data["eps"] = eps;
+    if (keep) ctx->mark_non_differentiable({out[out.size() - 2], out[out.size() - 1]});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    if (at::GradMode::is_enabled()) fail("residual_norm: its backward pass has no derivative");
+    const auto saved = ctx->get_saved_variables();
+    auto given = [&](int i) { return saved[i].defined() ? optional<Tensor>(saved[i]) : c10::nullopt; };
+    const auto flags = ctx->saved_data["options"].toBoolList();
+    const ResidualOptions o{flags[0], flags[1], flags[2], false, ctx->saved_data["eps"].toDouble()};
+    const Tensor &x = saved[0];
+    const optional<Tensor> f = given(1);
+    c10::cuda::CUDAGuard guard(x.device());
+    cxg_residual_desc d = describe_residual(x, f, given(2), given(3), given(4), given(5), given(6), given(7), o);
+    const int h_at = f ? 1 : 0;
+    Tensor dy, dh;
+    if (f && grads[0].defined()) dy = grads[0].contiguous();
+    if (o.next && grads[h_at].defined()) dh = grads[h_at].contiguous();
+    variable_list out(13);
+    if (!dy.defined() && !dh.defined()) return out;
+    d.dy = dy.defined() ? dy.data_ptr() : nullptr;
+    d.dh = dh.defined() ? dh.data_ptr() : nullptr;
+    // the edges of the node are those of the tensors that were given
+    bool need[8];
+    for (int i = 0, edge = 0; i < 8; ++i) need[i] = saved[i].defined() && ctx->needs_input_grad(edge++);
+    void **into[3] = {&d.dx, &d.df, &d.dgate};
+    for (int i = 0; i < 3; ++i)
+      if (need[i]) {
+        out[i] = at::empty_like(saved[i]);
+        *into[i] = out[i].data_ptr();
+      }
+    Tensor sums = at::empty({5, x.size(1)}, x.options().dtype(at::kFloat));
+    size_t bytes = 0;
+    check(lib.cxg_residual_norm_backward_workspace_size(d.n, d.width, &bytes), "cxg_residual_norm_backward_workspace_size");
+    void *st = stream_of(x);
+    {
+      const Workspace ws = workspace_on(x.device().index(), st, static_cast<int64_t>(bytes), "");
+      check(lib.cxg_residual_norm_backward(&d, sums.data_ptr<float>(), ws.data(), ws.bytes(), st), "cxg_residual_norm_backward");
+    }
+    for (int i = 3; i < 8; ++i)
+      if (need[i]) out[i] = sums.select(0, i - 3);
+    return out;
+  }
+};
+
+// A parameter as fp32 [width] (or one value for all columns), differentiably.
+optional<Tensor> row_parameter(const optional<Tensor> &t, const Tensor &x, const char *name) {
+  if (!t) return t;
+  same_device(x, *t, name);
+  if (!t->is_floating_point()) fail(std::string("residual_norm: ") + name + " must be of a floating-point type");
+  Tensor v = t->to(at::kFloat);
+  if (std::string(name) == "scale" && v.numel() == 1) v = v.reshape({1}).expand({x.size(1)});
+  if (v.dim() != 1 || v.size(0) != x.size(1)) fail(std::string("residual_norm: ") + name + " must be [" + std::to_string(x.size(1)) + "]");
+  return v.contiguous();
+}
+
+std::vector<optional<Tensor>> residual_norm(const Tensor &x_in, const optional<Tensor> &f_in, const optional<Tensor> &gate_in,
+                                            const optional<Tensor> &scale_in, bool post, const optional<Tensor> &post_weight,
+                                            const optional<Tensor> &post_bias, bool next, const optional<Tensor> &next_weight,
+                                            const optional<Tensor> &next_bias, bool layer, double eps, bool keep) {
+  if (for_torch(x_in, f_in, gate_in, scale_in, post_weight, post_bias, next_weight, next_bias))
+    fail(std::string("residual_norm") + kTransform);
+  auto rows = [&](const Tensor &t, const char *name) {
+    if (!t.is_cuda()) fail(std::string(name) + " must be a CUDA tensor (this backend has no CPU path)");
+    if (t.scalar_type() != x_in.scalar_type()) fail(std::string("residual_norm: ") + name + " must be of x's type");
+    same_device(x_in, t, name);
+    return t.contiguous();
+  };
+  row_type("residual_norm", x_in.scalar_type());
+  if (x_in.dim() != 2 || x_in.size(1) == 0) fail("residual_norm: x must be a matrix with at least one column");
+  if (x_in.size(1) > lib.cxg_residual_norm_max_width())
+    fail("residual_norm: rows of " + std::to_string(x_in.size(1)) + " values, at most " + std::to_string(lib.cxg_residual_norm_max_width()));
+  if (!(eps >= 0)) fail("residual_norm: eps must not be negative");
+  const Tensor x = rows(x_in, "x");
+  optional<Tensor> f, gate;
+  if (f_in) {
+    f = rows(*f_in, "f");
+    if (f->sizes() != x.sizes()) fail("residual_norm: f must have the shape of x");
+  } else if (gate_in || scale_in || post_weight || post_bias || !next) {
+    fail("residual_norm: without f there is the norm of x alone (no gate, scale or norm of f)");
+  }
+  if (!next && (next_weight || next_bias || keep)) fail("residual_norm: parameters or kept rows of a norm that is not asked for");
+  if (!post && (post_weight || post_bias)) fail("residual_norm: parameters of a norm that is not asked for");
+  if (gate_in) {
+    gate = rows(*gate_in, "gate");
+    const bool per_row = (gate->dim() == 1 || (gate->dim() == 2 && gate->size(1) == 1)) && gate->size(0) == x.size(0);
+    if (!per_row && gate->sizes() != x.sizes()) fail("residual_norm: gate must have the shape of x, or one value per row");
+  }
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto scale = row_parameter(scale_in, x, "scale"), w2 = row_parameter(post_weight, x, "post_weight"),
+             b2 = row_parameter(post_bias, x, "post_bias"), w1 = row_parameter(next_weight, x, "next_weight"),
+             b1 = row_parameter(next_bias, x, "next_bias");
+  const bool norm_f = f && post;
+  const variable_list out =
+      recorded(x, f, gate, scale, w2, b2, w1, b1)
+          ? ResidualNormFunction::apply(x, f, gate, scale, w2, b2, w1, b1, norm_f, next, layer, eps, keep)
+          : residual_forward(x, f, gate, scale, w2, b2, w1, b1, ResidualOptions{norm_f, next, layer, keep, eps});
+  std::vector<optional<Tensor>> all(4);
+  size_t at = 0;
+  all[0] = f ? out[at++] : x_in;
+  if (next) all[1] = out[at++];
+  if (keep) all[2] = out[at], all[3] = out[at + 1];
+  return all;
+}
+
 // ---- SAGE layer ------------------------------------------------------------------------------------------------------
 // into += g . w, or g . w into a new matrix
 Tensor linear_input_grad(const Tensor &g, const Tensor &w, const Tensor &into) {
@@ -1048,6 +1502,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return head_mean_bias(x, bias, heads, c);
   });
   m.def("relation_pairs", &relation_pairs);
+  m.def("rows8_pitch", [](int64_t width) { return lib.cxg_rows8_pitch(static_cast<int>(width)); });
+  m.def("rows8_zeros", [](int64_t rows, int64_t width, at::Device device) {
+    const Held h = held_zeros(rows, width, device);
+    return std::make_pair(h.codes, h.scales);
+  });
+  m.def("rows8_quantize", [](const Tensor &x) {
+    const Held h = quantize(x);
+    return std::make_pair(h.codes, h.scales);
+  });
+  m.def("rows8_quantize_into", &quantize_into);
+  m.def("rows8_dequantize", &dequantize);
+  m.def("rows8_aggregate", &rows8_aggregate);
+  m.def("rows8_weight_grad", [](const Tensor &codes, const Tensor &scales, int64_t width, const Tensor &dy, bool bias) {
+    const auto g = rows8_weight_grad(codes, scales, width, dy, bias);
+    return std::make_pair(g.first, bias ? optional<Tensor>(g.second) : c10::nullopt);
+  });
+  m.def("linear_kept8", &linear_kept8);
+  m.def("residual_norm", &residual_norm);
   m.def("sample_batch_fits", &sample_batch_fits);
   m.def("sample_batch", &sample_batch);
 }

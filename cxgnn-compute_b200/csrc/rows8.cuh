@@ -1,0 +1,64 @@
+// Rows held in 8 bits: the values of a row in groups of 32, a group as one power of two s = 2^(e - 127), held as the byte e,
+// and a whole number c of -127 .. 127 per value; the value is c * s. e is the smallest with max|x| / s < 127.5, kept within
+// 1 .. 248, so that s and 1 / s are normal numbers; c = x / s rounded to nearest, ties to even: off by at most s / 2, at most
+// 2^-7 of the group's largest value. Seven bits and a power of two are exact in fp32 and in bf16. A group with a value that
+// is not finite has e = 255 and c = 0: 2^128 is read as infinity, and zero times it is NaN, with no test where rows are read.
+//
+// In memory: codes [rows + 1][pitch] bytes, pitch = width in whole groups of 32, zeros behind the width; scales
+// [rows + 1][pitch / 32] bytes. The last row is of zeros: what ids outside the rows stand for. (One scale per group and not per
+// row: activations behind a ReLU differ by orders of magnitude along a row. Scales in an array of their own: rows of codes
+// then start on whole sectors, and the scales of a million rows of 128 stay in L2.)
+#pragma once
+#include "common.cuh"
+
+namespace cxg {
+namespace rows8 {
+
+constexpr int kGroup = 32;
+constexpr uint32_t kNotFinite = 255;
+
+inline int groups_of(int width) { return (width + kGroup - 1) / kGroup; }
+
+// The byte of the scale, from the largest absolute value's bit pattern. A mantissa of 127.5 / 64 and more would round to 128
+// and carries into the exponent instead.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top_bits) {
+  if (top_bits >= 0x7f800000u) return kNotFinite;
+  const int e = static_cast<int>((top_bits + 0x10000u) >> 23) - 6;
+  return static_cast<uint32_t>(min(max(e, 1), 248));
+}
+
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// x / s of finite groups: the product with 2^(254 - e - 127) is exact, or so small that it rounds to zero either way
+__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+
+// The code as the low byte of the result: adding 1.5 * 2^23 rounds to whole numbers, ties to even, and leaves their two's
+// complement in the low bits. The limit matters at the top of the range of fp32 alone, where e is kept at 248.
+__device__ __forceinline__ uint32_t code_bits(float x, float inv) {
+  return __float_as_uint(fminf(fmaxf(x * inv, -127.f), 127.f) + 12582912.f);
+}
+
+__device__ __forceinline__ uint32_t pack_codes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// Code i of a word as fp32: the code with its sign bit flipped is code + 128; as the low byte of 2^23 it is 2^23 + 128 + code.
+template <int I>
+__device__ __forceinline__ float code_value(uint32_t flipped) {
+  return __uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7440 | I)) - 8388736.f;
+}
+__device__ __forceinline__ void code_values(float *f, uint32_t word) {
+  const uint32_t w = word ^ 0x80808080u;
+  f[0] = code_value<0>(w), f[1] = code_value<1>(w), f[2] = code_value<2>(w), f[3] = code_value<3>(w);
+}
+
+// Row of item i where every row has `per` items: i / per by a multiplication with ceil(2^64 / per), exact for i * per < 2^64.
+struct Rows {
+  uint64_t magic;
+  uint32_t per;
+  __host__ __device__ explicit Rows(uint32_t p = 1) : magic(p > 1 ? ~0ull / p + 1 : 0), per(p) {}
+  __device__ __forceinline__ int64_t row(uint64_t i) const { return static_cast<int64_t>(magic ? __umul64hi(i, magic) : i); }
+};
+
+}  // namespace rows8
+}  // namespace cxg

@@ -1,0 +1,382 @@
+// Aggregation over rows in 8 bits: y[d, :] = red over the edges e of row d of v[e] * codes[s(e), :] * scale[s(e), group].
+//
+// The walk of spmm_walk_impl.cuh with rows of a quarter of the bytes: tiles of edges from the same plan, a group of G lanes per
+// tile, 32 / G tiles side by side in a warp, U edges in flight per lane, sums in edge order in one fp32 accumulator per
+// column, partials of rows that cross tiles added by the same fix-up. Same bits on every run.
+//
+// A lane holds VB codes of a row, which lie in one group of 32 and share a scale. A code becomes fp32 by a byte permutation
+// and an addition (rows8.cuh); code * scale is exact, and so is scale * v (a power of two) but where that leaves the range of
+// normal numbers, so each edge rounds once, in the addition. (Two codes cost 2 permutations, a packed addition and a packed
+// multiplication-addition; converting with the conversion instruction would cost a quarter-rate instruction per code.)
+#include "rows8.cuh"
+#include "spmm_walk_impl.cuh"
+
+namespace cxg {
+namespace {
+
+using namespace rows8;
+using walk::kFar;
+using walk::kThreads;
+
+struct Rows8Args {
+  WalkArgs w;  // ptr, idx, y, edge_val, plan and partials; width: columns, row_bytes: pitch of the codes
+  const uint8_t *codes, *scales;
+  int64_t n_src;  // rows; ids outside stand for the row of zeros behind the last
+  int groups;
+  int whole;  // rows of y are whole 16-byte vectors
+};
+
+template <int VB>
+struct Codes {
+  static constexpr int W = VB / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const uint8_t *p) {
+    if constexpr (VB == 16) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (VB == 8) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+      w[0] = v.x, w[1] = v.y;
+    } else {
+      w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+    }
+  }
+};
+
+// acc[2i], acc[2i + 1] += codes * s
+template <int VB>
+__device__ __forceinline__ void add_codes(unsigned long long *acc, const Codes<VB> &c, float s) {
+  unsigned long long ss, bias;
+  asm("mov.b64 %0, {%1,%1};" : "=l"(ss) : "f"(s));
+  asm("mov.b64 %0, {%1,%1};" : "=l"(bias) : "f"(-8388736.f));
+#pragma unroll
+  for (int i = 0; i < VB / 4; ++i) {
+    const uint32_t w = c.w[i] ^ 0x80808080u;
+    const uint32_t a = __byte_perm(w, 0x4b000000u, 0x7440), b = __byte_perm(w, 0x4b000000u, 0x7441),
+                   d = __byte_perm(w, 0x4b000000u, 0x7442), e = __byte_perm(w, 0x4b000000u, 0x7443);
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1,%2};\n\tadd.rn.f32x2 t, t, %3;\n\tfma.rn.f32x2 %0, t, %4, %0;\n\t}"
+        : "+l"(acc[2 * i])
+        : "r"(a), "r"(b), "l"(bias), "l"(ss));
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1,%2};\n\tadd.rn.f32x2 t, t, %3;\n\tfma.rn.f32x2 %0, t, %4, %0;\n\t}"
+        : "+l"(acc[2 * i + 1])
+        : "r"(d), "r"(e), "l"(bias), "l"(ss));
+  }
+}
+
+// VALMODE: 0 sum, 1 a value per edge, 3 mean.
+template <typename T, int VB, int G, int NV, int U, int VALMODE, int MINB>
+__global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_constant__ Rows8Args r) {
+  const WalkArgs &a = r.w;
+  constexpr int NG = 32 / G;
+  const int lane = threadIdx.x & 31;
+  const int lg = lane & (G - 1);
+  dependency_wait();
+  const uint32_t e_total = static_cast<uint32_t>(edge_total(a));
+  const int n_dst = static_cast<int>(a.n_dst);
+  const int n_tiles = static_cast<int>((e_total + static_cast<int64_t>(a.tile) - 1) / a.tile);
+  const int step = static_cast<int>(gridDim.x) * (kThreads / 32) * NG;  // tiles that are walked at the same time
+  const uint32_t pitch = static_cast<uint32_t>(a.row_bytes), groups = static_cast<uint32_t>(r.groups);
+  // codes [(lg + q * G) * VB, +VB) of a row; a lane behind the row reads its neighbours' line again and stores nothing
+  const uint8_t *cq[NV], *sq[NV];
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    const int c = (lg + q * G) * VB, at = c < static_cast<int>(pitch) ? c : static_cast<int>(pitch) - VB;
+    cq[q] = r.codes + at, sq[q] = r.scales + at / kGroup;
+  }
+  auto col = [&](int q) { return (lg + q * G) * VB; };
+
+  auto store = [&](int row, float (&f)[NV][VB]) {
+    T *y = static_cast<T *>(a.y) + static_cast<int64_t>(row) * a.width;
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      if (r.whole) {
+        constexpr int N = 16 / static_cast<int>(sizeof(T));
+        if constexpr (VB >= N) {
+#pragma unroll
+          for (int i = 0; i < VB; i += N)
+            if (col(q) + i < a.width) Vec<T>::store_stream(y + col(q) + i, Vec<T>::from_float(f[q] + i));
+        } else {  // 4 bf16
+          if (col(q) < a.width) walk::store_row_bytes<T, VB * static_cast<int>(sizeof(T))>(reinterpret_cast<uint8_t *>(y + col(q)), f[q]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VB; ++i)
+          if (col(q) + i < a.width) y[col(q) + i] = from_f32<T>(f[q][i]);
+      }
+    }
+  };
+  auto zero_row = [&](int row) {
+    float z[NV][VB];
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+      for (int i = 0; i < VB; ++i) z[q][i] = 0.f;
+    store(row, z);
+  };
+  const int t_first = static_cast<int>((blockIdx.x * static_cast<unsigned>(kThreads) + threadIdx.x) / G);
+  if (e_total == 0) {  // no edge at all: every row is empty
+    for (int row = t_first; row < n_dst; row += step) zero_row(row);
+    return;
+  }
+
+  // ids and edge values of a batch of 32 edges per group (as in spmm_walk)
+  constexpr int kBatch = 36;
+  __shared__ __align__(16) uint32_t id_stage[kThreads / 32][NG * kBatch];
+  __shared__ __align__(16) float val_stage[VALMODE == 1 ? kThreads / 32 : 1][VALMODE == 1 ? NG * kBatch : 4];
+  uint32_t *my_ids = id_stage[threadIdx.x >> 5] + lane / G * kBatch;
+  float *my_vals = VALMODE == 1 ? val_stage[threadIdx.x >> 5] + lane / G * kBatch : nullptr;
+  int t_next = 0;
+  for (int t = t_first; t - lane / G < n_tiles; t = t_next) {
+    t_next = n_tiles;
+    if (step < n_tiles) {
+      if (lane == 0) t_next = step + atomicAdd(a.hdr + kWalkHdrNext, NG);
+    }
+    uint32_t begin = 0, row_begin = 0, row_end = 0;
+    int row = 0, len = 0;
+    if (t < n_tiles) {
+      const WalkTile here = load_tile(a, t);
+      begin = here.begin, row_begin = here.row_begin, row_end = here.row_end;
+      row = static_cast<int>(here.row);
+      len = static_cast<int>(load_tile(a, t + 1).begin - begin);
+    }
+
+    constexpr int IB = 32 / G;
+    uint32_t id_nxt[IB];
+    float val_nxt[IB];
+    auto load_batch = [&](int first) {
+#pragma unroll
+      for (int j = 0; j < IB; ++j) {
+        const int pos = first + j * G + lg;
+        id_nxt[j] = static_cast<uint32_t>(r.n_src);
+        val_nxt[j] = 0.f;
+        if (pos < len) {
+          const uint32_t e = begin + pos;
+          const uint64_t id = a.idx_bytes == 8
+                                  ? static_cast<uint64_t>(walk::load_id_stream(static_cast<const int64_t *>(a.idx) + e))
+                                  : static_cast<uint64_t>(static_cast<int64_t>(walk::load_id_stream(static_cast<const int32_t *>(a.idx) + e)));
+          if (id < static_cast<uint64_t>(r.n_src)) id_nxt[j] = static_cast<uint32_t>(id);
+          if (VALMODE == 1) val_nxt[j] = __ldg(a.edge_val + e);
+        }
+      }
+    };
+
+    auto end_raw = [&](int i) { return walk::load_ptr_low(a.ptr, min(i + 1, n_dst), a.ptr_bytes); };
+    auto end_rel = [&](int i, uint32_t raw) -> int {
+      const uint32_t v = raw - begin;
+      return i >= n_dst || v > static_cast<uint32_t>(kFar) ? kFar : static_cast<int>(v);
+    };
+    int rend = kFar, rstart = 0, stop = kFar;
+    uint32_t next_raw = 0;
+    if (len > 0) {
+      if (t == 0)
+        for (int i = 0; i < row; ++i) zero_row(i);  // leading rows without edges
+      rstart = row_begin < begin ? -1 : 0;
+      next_raw = end_raw(row + 1);
+      rend = end_rel(row, row_end);
+      while (rend == 0) {  // empty rows that the previous tile's walk wrote
+        ++row;
+        rend = end_rel(row, next_raw);
+        next_raw = end_raw(row + 1);
+      }
+      stop = min(rend, len);
+    }
+    unsigned long long acc[NV][VB / 2];
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+      for (int i = 0; i < VB / 2; ++i) acc[q][i] = 0ull;
+
+    // the walk stands at a row end, at the end of the tile, or at both
+    auto event = [&](int pos) {
+      const bool row_done = pos == rend;
+      float f[NV][VB];
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+#pragma unroll
+        for (int i = 0; i < VB / 2; ++i) {
+          asm("mov.b64 {%0,%1}, %2;" : "=f"(f[q][2 * i]), "=f"(f[q][2 * i + 1]) : "l"(acc[q][i]));
+          acc[q][i] = 0ull;
+        }
+      if (row_done && rstart >= 0) {
+        if (VALMODE == 3) {
+#pragma unroll
+          for (int q = 0; q < NV; ++q) walk::divide_by_count<VB>(f[q], static_cast<float>(rend - rstart));
+        }
+        store(row, f);
+      } else if (row < n_dst) {
+        // the row began in an earlier tile, or goes on in the next one
+        float *p = a.partials + (static_cast<int64_t>(t) * 2 + (rstart < 0 ? 0 : 1)) * a.part_stride;
+#pragma unroll
+        for (int q = 0; q < NV; ++q)
+#pragma unroll
+          for (int i = 0; i < VB; i += 4)
+            if (col(q) + i < a.part_stride)
+              *reinterpret_cast<float4 *>(p + col(q) + i) = make_float4(f[q][i], f[q][i + 1], f[q][i + 2], f[q][i + 3]);
+      }
+      if (row_done) {
+        rstart = pos;
+        for (;;) {
+          ++row;
+          rend = end_rel(row, next_raw);
+          next_raw = end_raw(row + 1);
+          if (rend != pos) break;
+          zero_row(row);  // a row without edges
+        }
+      }
+      stop = pos == len ? kFar : min(rend, len);
+    };
+
+    const int longest = G == 32 ? len : __reduce_max_sync(0xffffffffu, len);
+    load_batch(0);
+    for (int p = 0; p < longest; p += U) {
+      const int in_batch = p & 31;
+      if (in_batch == 0) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < IB; ++j) {
+          my_ids[j * G + lg] = id_nxt[j];
+          if (VALMODE == 1) my_vals[j * G + lg] = val_nxt[j];
+        }
+        __syncwarp();
+        load_batch(p + 32);
+      }
+      Codes<VB> c[U][NV];
+      uint32_t s[U][NV];
+      constexpr int W4 = U < 4 ? U : 4;
+      uint32_t ids[W4];
+      float vals[W4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u % W4 == 0) walk::load_ids(ids, my_ids + in_batch + u);
+        const uint64_t id = ids[u % W4];
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+          c[u][q].load(cq[q] + id * pitch);
+          s[u][q] = __ldg(sq[q] + id * groups);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (VALMODE == 1 && u % W4 == 0) walk::load_ids(vals, my_vals + in_batch + u);
+#pragma unroll
+        for (int q = 0; q < NV; ++q)
+          add_codes<VB>(acc[q], c[u][q], VALMODE == 1 ? scale_of(s[u][q]) * vals[u % W4] : scale_of(s[u][q]));
+        if (p + u + 1 == stop) event(p + u + 1);
+      }
+    }
+    t_next = __shfl_sync(0xffffffffu, t_next, 0) + lane / G;
+  }
+}
+
+// Lane layouts by the pitch of the codes. With resident set nothing is launched: it receives the tiles walked at the same time.
+template <typename T, int VALMODE>
+bool launch_pitch(const Rows8Args &r, cudaStream_t st, int *resident) {
+  auto go = [&](auto kernel, int g, int ctas) {
+    const int per_cta = kThreads / g;
+    if (resident != nullptr) {
+      *resident = kNumSM * ctas * per_cta;
+      return true;
+    }
+    int64_t grid = (r.w.max_tiles + per_cta - 1) / per_cta;
+    const int64_t most = kNumSM * ctas;
+    if (grid > most) grid = most;
+    return launch_dependent(kernel, static_cast<unsigned>(grid < 1 ? 1 : grid), kThreads, 0, st, r) == cudaSuccess;
+  };
+#define CXG_ROWS8_WALK(VB, G, NV, U, CTAS) \
+  if (r.w.row_bytes <= VB * G * NV)        \
+  return go(rows8_walk<T, VB, G, NV, U, VALMODE, CTAS>, G, CTAS)
+  CXG_ROWS8_WALK(4, 8, 1, 8, 8);
+  CXG_ROWS8_WALK(8, 8, 1, 8, 8);
+  CXG_ROWS8_WALK(16, 8, 1, 4, 8);
+  CXG_ROWS8_WALK(16, 16, 1, 4, 8);
+  CXG_ROWS8_WALK(16, 32, 1, 4, 8);
+  CXG_ROWS8_WALK(16, 32, 2, 2, 5);
+  CXG_ROWS8_WALK(16, 32, 4, 2, 3);
+#undef CXG_ROWS8_WALK
+  return false;
+}
+
+bool dispatch(const Rows8Args &r, int out_dtype, cudaStream_t st, int *resident) {
+  const int valmode = r.w.edge_val != nullptr ? 1 : r.w.reduce == CXG_MEAN ? 3 : 0;
+  if (out_dtype == CXG_F32)
+    return valmode == 0   ? launch_pitch<float, 0>(r, st, resident)
+           : valmode == 1 ? launch_pitch<float, 1>(r, st, resident)
+                          : launch_pitch<float, 3>(r, st, resident);
+  return valmode == 0   ? launch_pitch<__nv_bfloat16, 0>(r, st, resident)
+         : valmode == 1 ? launch_pitch<__nv_bfloat16, 1>(r, st, resident)
+                        : launch_pitch<__nv_bfloat16, 3>(r, st, resident);
+}
+
+constexpr int kMostWidth = 2048;
+
+int tile_edges(const Rows8Args &r, int64_t nnz, int split_edges) {
+  if (split_edges > 0) return split_edges;
+  int resident = kNumSM * 32;
+  dispatch(r, CXG_F32, nullptr, &resident);
+  return walk_tile_of_waves(nnz, resident);
+}
+
+}  // namespace
+}  // namespace cxg
+
+using namespace cxg;
+
+extern "C" int cxg_rows8_aggregate_workspace_size(int64_t nnz, int width, int split_edges, size_t *bytes) {
+  CXG_REQUIRE(bytes != nullptr, CXG_ENULL, "cxg_rows8_aggregate_workspace_size: bytes is NULL");
+  CXG_REQUIRE(nnz >= 0 && width > 0 && split_edges >= 0, CXG_EINVAL, "cxg_rows8_aggregate_workspace_size: bad sizes");
+  CXG_REQUIRE(width <= kMostWidth, CXG_EUNSUPPORTED, "cxg_rows8_aggregate: rows of %d values, at most %d", width, kMostWidth);
+  Rows8Args r = {};
+  r.w.row_bytes = rows8::groups_of(width) * rows8::kGroup;
+  WalkLayout L;
+  const int rc = walk_layout(nnz, walk_part_stride(width), tile_edges(r, nnz, split_edges), &L);
+  if (rc != CXG_OK) return set_error(rc, "cxg_rows8_aggregate: graph too large for 32-bit tile ids");
+  *bytes = L.total;
+  return CXG_OK;
+}
+
+extern "C" int cxg_rows8_aggregate(const void *codes, const void *scales, int64_t n_src, int width, const void *ptr, int ptr_bytes,
+                                   const void *idx, int idx_bytes, const float *edge_val, int64_t n_dst, int64_t nnz, int reduce,
+                                   int split_edges, void *y, int y_dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  CXG_REQUIRE(n_src >= 0 && width > 0 && n_dst >= 0 && nnz >= 0 && split_edges >= 0, CXG_EINVAL, "cxg_rows8_aggregate: bad sizes");
+  CXG_REQUIRE((ptr_bytes == 4 || ptr_bytes == 8) && (idx_bytes == 4 || idx_bytes == 8), CXG_EINVAL,
+              "cxg_rows8_aggregate: ptr and idx are of 4 or 8 bytes");
+  CXG_REQUIRE(y_dtype == CXG_F32 || y_dtype == CXG_BF16, CXG_EINVAL, "cxg_rows8_aggregate: dtype %d", y_dtype);
+  CXG_REQUIRE(reduce == CXG_SUM || (reduce == CXG_MEAN && edge_val == nullptr), CXG_EINVAL,
+              "cxg_rows8_aggregate: a sum, or a mean without edge values");
+  CXG_REQUIRE(width <= kMostWidth, CXG_EUNSUPPORTED, "cxg_rows8_aggregate: rows of %d values, at most %d", width, kMostWidth);
+  constexpr int64_t most = INT32_MAX - (1 << 20);
+  CXG_REQUIRE(n_dst <= most && nnz <= most && n_src < UINT32_MAX, CXG_ELIMIT,
+              "cxg_rows8_aggregate: rows and edges are counted in 32 bits");
+  if (n_dst == 0) return CXG_OK;
+  CXG_REQUIRE(codes && scales && ptr && y && (idx || nnz == 0), CXG_ENULL, "cxg_rows8_aggregate: NULL argument");
+  CXG_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 16 == 0, CXG_EINVAL, "cxg_rows8_aggregate: codes must be 16-byte aligned");
+  Rows8Args r = {};
+  WalkArgs &a = r.w;
+  a.ptr = ptr, a.idx = idx, a.y = y, a.edge_val = edge_val;
+  a.n_dst = n_dst, a.nnz = nnz, a.feat = a.width = width, a.heads = 1;
+  a.row_bytes = a.x_pitch = rows8::groups_of(width) * rows8::kGroup;
+  a.ptr_bytes = ptr_bytes, a.idx_bytes = idx_bytes, a.reduce = reduce;
+  r.codes = static_cast<const uint8_t *>(codes), r.scales = static_cast<const uint8_t *>(scales);
+  r.n_src = n_src, r.groups = rows8::groups_of(width);
+  r.whole = ((static_cast<uint64_t>(width) * (y_dtype == CXG_F32 ? 4 : 2)) | reinterpret_cast<uintptr_t>(y)) % 16 == 0;
+  a.tile = tile_edges(r, nnz, split_edges);
+  a.part_stride = static_cast<int>(walk_part_stride(width));
+  WalkLayout L;
+  const int rc = walk_layout(nnz, a.part_stride, a.tile, &L);
+  if (rc != CXG_OK) return set_error(rc, "cxg_rows8_aggregate: graph too large for 32-bit tile ids");
+  CXG_REQUIRE(workspace != nullptr && workspace_bytes >= L.total && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, CXG_EWORKSPACE,
+              "cxg_rows8_aggregate: workspace %zu bytes, need %zu", workspace_bytes, L.total);
+  char *ws = static_cast<char *>(workspace);
+  a.hdr = reinterpret_cast<int32_t *>(ws + L.hdr);
+  a.tiles = ws + L.tiles;
+  a.count = reinterpret_cast<int32_t *>(ws + L.count);
+  a.partials = reinterpret_cast<float *>(ws + L.partials);
+  a.max_tiles = L.max_tiles;
+  cudaStream_t st = as_stream(stream);
+  walk_plan_run(a, st);
+  if (!dispatch(r, y_dtype, st, nullptr)) return set_error(CXG_ECUDA, "cxg_rows8_aggregate: %s", cudaGetErrorString(cudaGetLastError()));
+  const cudaError_t e = walk_fix_run(a, y_dtype, st);
+  if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_aggregate: %s", cudaGetErrorString(e));
+  count_launches(3);
+  return check_launch("cxg_rows8_aggregate");
+}

@@ -1,0 +1,475 @@
+// Weight gradient from a layer's input held in 8 bits, on the 5th-generation tensor cores:
+//   dW[o][i] = sum over the rows r of dy[r][o] * codes[r][i] * scale[r][i / 32],   db[o] = sum over the rows of dy[r][o]
+//
+// codes * scale has 7 bits and is an exact bf16 operand; fp32 dy is cut into three bf16 parts of 8 bits each, which hold all 24
+// of its bits: dy = hi + mid + lo exactly. So every product is exact and a sum of m rows takes three bf16 instructions' worth
+// of tensor core time (one for bf16 dy), where compensated TF32 would take three of half the rate and lose bits.
+//
+// The contraction runs over rows, so both operands are "MN-major": a stage holds 64 rows of the input (A: 128 columns, two
+// spans of 128 bytes per row in a 128-byte swizzle) and of dy (B: hi, then mid, then lo spans). Both are made in registers:
+// producer warps load 16 bytes at a time a whole stage ahead, convert, and write the operands where the tensor core reads
+// them. One instruction multiplies A by [hi | mid], another adds A by lo to mid's accumulator. An accumulator takes
+// `chunk` stages, as the tensor core's additions cut off what an fp32 addition rounds (its error grows with the number of
+// additions); the epilogue warps, each lane a column of the input, keep the sums of the chunks in registers.
+//
+// A block owns a contiguous range of rows of one pair of 128-column blocks; its sums go to a partial of its own and a second
+// kernel adds the partials in order: the same bits on every run. Every wait is bounded (see tensor_core.cuh).
+#include "rows8.cuh"
+#include "tensor_core.cuh"
+
+namespace cxg {
+namespace {
+
+using namespace tc;
+using rows8::kGroup;
+
+constexpr int kPos = 64;           // rows per stage
+constexpr int kSpan = kPos * 128;  // bytes of a span: 64 columns of bf16, one row behind the other
+constexpr int kProdWarps = 8, kEpiWarps = 8;
+constexpr int kMmaWarp = kEpiWarps, kFirstProd = kMmaWarp + 1;
+constexpr int kThreads = 32 * (kEpiWarps + 1 + kProdWarps);
+constexpr int kMaxStages = 4;
+constexpr int kSmemBudget = 220 * 1024;
+
+struct R8Args {
+  const uint8_t *codes, *scales;
+  const void *dy;
+  int64_t m, ld;
+  int k, n, pitch, groups, k_blocks, stages, chunk, test_stall;
+  float *partial;     // [pair of column blocks][gridDim.x][128 columns of dy][128 columns of the input]
+  float *partial_db;  // [gridDim.x][n] or NULL
+  int32_t *status;
+  long long wait_cycles;
+};
+
+struct R8Barriers {
+  uint64_t full[kMaxStages];   // producers -> MMA
+  uint64_t empty[kMaxStages];  // MMA -> producers
+  uint64_t acc_full[2];        // MMA -> epilogue
+  uint64_t acc_empty[2];       // epilogue -> MMA
+};
+
+__device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Two neighbouring codes (bytes 2 * H and 2 * H + 1 of a word) times the scale, as two bf16. With c = low - 128 * sign:
+// 0x4300 | (c & 0x7f) is 128 + low and 0x4300 | (c & 0x80) is 128 + 128 * sign in bf16, and their difference is exact.
+template <int H>
+__device__ __forceinline__ uint32_t two_values(uint32_t word, __nv_bfloat162 scale) {
+  const uint32_t w = __byte_perm(word, 0x43434343u, H == 0 ? 0x4140 : 0x4342);
+  const uint32_t lo = w & 0xff7fff7fu, hi = w & 0xff80ff80u;
+  __nv_bfloat162 a, b;
+  __builtin_memcpy(&a, &lo, 4);
+  __builtin_memcpy(&b, &hi, 4);
+  a = __hmul2(__hsub2(a, b), scale);
+  uint32_t out;
+  __builtin_memcpy(&out, &a, 4);
+  return out;
+}
+
+// hi, mid and lo of 8 fp32 values, as 8 bf16 each. Cutting instead of rounding keeps the sum exact (8 bits each). Infinities and
+// NaN go into hi alone (what is left of them would be NaN).
+__device__ __forceinline__ void three_parts(const float (&v)[8], uint32_t (&hi)[4], uint32_t (&mid)[4], uint32_t (&lo)[4]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  const bool finite = top < 0x7f800000u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t h[2], m[2], l[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float f = v[2 * i + j];
+      h[j] = __float_as_uint(f) & 0xffff0000u;
+      float r = f - __uint_as_float(h[j]);
+      if (!finite) {
+        if ((h[j] & 0x7f800000u) == 0x7f800000u) r = 0.f;
+        if (f != f) h[j] = 0x7fc00000u;
+      }
+      m[j] = __float_as_uint(r) & 0xffff0000u;
+      l[j] = __float_as_uint(r - __uint_as_float(m[j]));
+    }
+    hi[i] = __byte_perm(h[0], h[1], 0x7632);
+    mid[i] = __byte_perm(m[0], m[1], 0x7632);
+    lo[i] = __byte_perm(l[0], l[1], 0x7632);
+  }
+}
+
+// SPANS: 64-column spans of a block of dy. VEC: rows of dy are whole 16-byte vectors.
+template <typename T, bool VEC, int SPANS>
+__global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant__ R8Args a) {
+  constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+  constexpr int kCols = 64 * SPANS;
+  constexpr uint32_t kStageBytes = (2 + kParts * SPANS) * kSpan;
+  constexpr int kAccCols = kParts == 3 ? 2 * kCols : kCols;  // of a buffer in tensor memory
+  constexpr int kTmem = 2 * kAccCols;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  __shared__ __align__(8) R8Barriers bars;
+  __shared__ float db_side[kProdWarps][128];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_slot;
+  volatile int *abort_flag = &abort_slot;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int x_at = static_cast<int>(blockIdx.y % a.k_blocks) * 128, g_at = static_cast<int>(blockIdx.y / a.k_blocks) * 128;
+  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_slot)), "r"(kTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    abort_slot = 0;
+    for (int s = 0; s < kMaxStages; ++s) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(&bars.full[s])), "r"(32 * kProdWarps) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(&bars.empty[s])) : "memory");
+    }
+    for (int b = 0; b < 2; ++b) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(&bars.acc_full[b])) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(&bars.acc_empty[b])), "r"(32 * kEpiWarps) : "memory");
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  dependency_wait();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_d = tmem_base_slot;
+  const int64_t n_tiles = (a.m + kPos - 1) / kPos;
+  const int64_t tile_lo = n_tiles * blockIdx.x / gridDim.x, tile_hi = n_tiles * (blockIdx.x + 1) / gridDim.x;
+
+  if (warp >= kFirstProd) {
+    // ================= producers =================
+    constexpr int kThr = 32 * kProdWarps;
+    constexpr int kXUnits = kPos * 8 / kThr;                // 16 codes each
+    constexpr int kUnitsPerRow = 8 * SPANS;                 // of dy: 8 values each
+    constexpr int kGUnits = kPos * kUnitsPerRow / kThr;
+    const int pt = tid - 32 * kFirstProd;
+    const int xu = pt & 7, gu = pt % kUnitsPerRow;
+    const int xcol = x_at + xu * 16, gcol = g_at + gu * 8;
+    const bool x_in = xcol < a.pitch;
+    struct Raw {
+      uint4 codes[kXUnits];
+      uint32_t scale[kXUnits];
+      uint32_t dy[kGUnits][sizeof(T) == 4 ? 8 : 4];
+    };
+    auto load = [&](int64_t tile, Raw &r) {
+#pragma unroll
+      for (int j = 0; j < kXUnits; ++j) {
+        const int64_t row = tile * kPos + (pt >> 3) + j * (kThr / 8);
+        r.codes[j] = make_uint4(0, 0, 0, 0);
+        r.scale[j] = 0;
+        if (x_in && tile < tile_hi && row < a.m) {
+          r.codes[j] = __ldg(reinterpret_cast<const uint4 *>(a.codes + row * a.pitch + xcol));
+          r.scale[j] = __ldg(a.scales + row * a.groups + xcol / kGroup);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kGUnits; ++j) {
+        const int64_t row = tile * kPos + pt / kUnitsPerRow + j * (kThr / kUnitsPerRow);
+        constexpr int W = sizeof(T) == 4 ? 8 : 4;
+#pragma unroll
+        for (int i = 0; i < W; ++i) r.dy[j][i] = 0;
+        if (tile >= tile_hi || row >= a.m) continue;
+        const T *p = static_cast<const T *>(a.dy) + row * a.ld + gcol;
+        if constexpr (VEC) {
+#pragma unroll
+          for (int i = 0; i < W; i += 4)
+            if (gcol + i < a.n) {
+              const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p + i));
+              r.dy[j][i] = v.x, r.dy[j][i + 1] = v.y, r.dy[j][i + 2] = v.z, r.dy[j][i + 3] = v.w;
+            }
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (gcol + i < a.n) r.dy[j][i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (gcol + i < a.n) r.dy[j][i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(p) + i)) << (16 * (i & 1));
+        }
+      }
+    };
+    float db[8] = {};
+    auto put = [&](const Raw &r, uint32_t stage) {
+#pragma unroll
+      for (int j = 0; j < kXUnits; ++j) {
+        const int row = (pt >> 3) + j * (kThr / 8);
+        const __nv_bfloat162 s = __float2bfloat162_rn(rows8::scale_of(r.scale[j]));
+        const uint32_t w[4] = {r.codes[j].x, r.codes[j].y, r.codes[j].z, r.codes[j].w};
+        uint32_t v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = two_values<0>(w[i], s), v[2 * i + 1] = two_values<1>(w[i], s);
+        const uint32_t span = stage + (xu >> 2) * kSpan;
+        const int c = (xu & 3) * 2, odd = xu >> 2;  // the second span's lanes start with their odd chunk: other banks
+        const uint32_t first = span + swizzled_offset<false>(row, c + odd), second = span + swizzled_offset<false>(row, c + 1 - odd);
+        if (odd) {
+          st_shared16(first, v[4], v[5], v[6], v[7]);
+          st_shared16(second, v[0], v[1], v[2], v[3]);
+        } else {
+          st_shared16(first, v[0], v[1], v[2], v[3]);
+          st_shared16(second, v[4], v[5], v[6], v[7]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kGUnits; ++j) {
+        const int row = pt / kUnitsPerRow + j * (kThr / kUnitsPerRow);
+        const uint32_t at = stage + (2 + (gu >> 3)) * kSpan + swizzled_offset<false>(row, gu & 7);
+        if constexpr (sizeof(T) == 4) {
+          float v[8];
+          uint32_t hi[4], mid[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.dy[j][i]), db[i] += v[i];
+          three_parts(v, hi, mid, lo);
+          st_shared16(at, hi[0], hi[1], hi[2], hi[3]);
+          st_shared16(at + SPANS * kSpan, mid[0], mid[1], mid[2], mid[3]);
+          st_shared16(at + 2 * SPANS * kSpan, lo[0], lo[1], lo[2], lo[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) db[i] += __uint_as_float(i & 1 ? r.dy[j][i / 2] & 0xffff0000u : r.dy[j][i / 2] << 16);
+          st_shared16(at, r.dy[j][0], r.dy[j][1], r.dy[j][2], r.dy[j][3]);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    };
+    Ring ring(a.stages);
+    bool alive = true;
+    auto hand_over = [&](const Raw &r) {
+      const int s = ring.stage;
+      if (ring.reused()) alive = wait_bar(&bars.empty[s], ring.emptied(), abort_flag, a.status, a.wait_cycles);
+      if (!alive) return;
+      put(r, base + static_cast<uint32_t>(s) * kStageBytes);
+      if (!(a.test_stall && ring.round == 0 && s == 0)) mbar_arrive(&bars.full[s]);
+      ring.next();
+    };
+    Raw one, two;
+    load(tile_lo, one);
+    for (int64_t tile = tile_lo; tile < tile_hi && alive; tile += 2) {
+      load(tile + 1, two);
+      hand_over(one);
+      if (!alive || tile + 1 >= tile_hi) break;
+      load(tile + 2, one);
+      hand_over(two);
+    }
+    if (a.partial_db != nullptr && x_at == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int o = kUnitsPerRow; o < 32; o <<= 1) db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+        if (lane < kUnitsPerRow) db_side[warp - kFirstProd][gu * 8 + i] = db[i];
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kProdWarps) : "memory");
+      if (pt < kCols && g_at + pt < a.n) {
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < kProdWarps; ++w) t += db_side[w][pt];
+        a.partial_db[static_cast<int64_t>(blockIdx.x) * a.n + g_at + pt] = t;
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ================= MMA issuer: the whole warp walks the tiles, one lane issues =================
+    auto wait_all = [&](uint64_t *bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, a.status, a.wait_cycles)) != 0;
+    };
+    const uint32_t idesc = make_idesc_mn(1, 128, kCols), idesc_wide = make_idesc_mn(1, 128, kParts == 3 ? 2 * kCols : kCols);
+    Ring ring(a.stages);
+    int64_t chunk = 0;
+    int in_chunk = 0;
+    bool alive = true;
+    for (int64_t tile = tile_lo; tile < tile_hi && alive; ++tile) {
+      const int buf = static_cast<int>(chunk & 1);
+      if (in_chunk == 0 && chunk >= 2) {  // the epilogue has read the chunk that used this buffer before
+        alive = wait_all(&bars.acc_empty[buf], static_cast<uint32_t>(((chunk >> 1) - 1) & 1));
+        if (!alive) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      const int s = ring.stage;
+      alive = wait_all(&bars.full[s], ring.filled());
+      if (!alive) break;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t d = tmem_d + buf * kAccCols;
+      const uint32_t x0 = base + static_cast<uint32_t>(s) * kStageBytes, g0 = x0 + 2 * kSpan;
+#pragma unroll
+      for (int j = 0; j < kPos / 16; ++j) {
+        const uint32_t go_on = (in_chunk > 0 || j > 0) ? 1u : 0u;
+        const uint64_t xa = make_desc_mn_sw128<false>(x0 + j * 2048, kSpan);
+        mma_ss<false>(d, xa, make_desc_mn_sw128<false>(g0 + j * 2048, kSpan), idesc_wide, go_on);
+        if constexpr (kParts == 3)
+          mma_ss<false>(d + kCols, xa, make_desc_mn_sw128<false>(g0 + 2 * SPANS * kSpan + j * 2048, kSpan), idesc, 1u);
+      }
+      commit_to(&bars.empty[s]);
+      if (++in_chunk == a.chunk || tile + 1 == tile_hi) {
+        commit_to(&bars.acc_full[buf]);
+        in_chunk = 0;
+        ++chunk;
+      }
+      ring.next();
+    }
+    if (!alive) {  // what was issued ends before tensor memory is given back
+      const long long t0 = clock64();
+      while (clock64() - t0 < 200000) {
+      }
+    }
+  } else {
+    // ================= epilogue: lane = column of the input, half of the columns of dy per four warps =================
+    constexpr int kHalf = kCols / 2;
+    float acc[kHalf];
+#pragma unroll
+    for (int c = 0; c < kHalf; ++c) acc[c] = 0.f;
+    const int first = (warp >> 2) * kHalf, row = (warp & 3) * 32 + lane;
+    const int64_t n_chunks = (tile_hi - tile_lo + a.chunk - 1) / a.chunk;
+    bool alive = true;
+    for (int64_t chunk = 0; chunk < n_chunks; ++chunk) {
+      const int buf = static_cast<int>(chunk & 1);
+      alive = __all_sync(0xffffffffu, wait_bar(&bars.acc_full[buf], static_cast<uint32_t>((chunk >> 1) & 1), abort_flag, a.status,
+                                               a.wait_cycles)) != 0;
+      if (!alive) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t taddr = tmem_d + (static_cast<uint32_t>((warp & 3) * 32) << 16) + buf * kAccCols + first;
+#pragma unroll
+      for (int c = 0; c < kHalf; c += 16) {
+        uint32_t v[16], w[16];
+        tmem_ld16(v, taddr + c);
+        if constexpr (kParts == 3) tmem_ld16(w, taddr + kCols + c);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          acc[c + i] += kParts == 3 ? __uint_as_float(v[i]) + __uint_as_float(w[i]) : __uint_as_float(v[i]);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      mbar_arrive(&bars.acc_empty[buf]);
+    }
+    if (alive && x_at + row < a.k) {
+      float *out = a.partial + ((static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 128 + first) * 128 + row;
+#pragma unroll
+      for (int c = 0; c < kHalf; ++c)
+        if (g_at + first + c < a.n) out[c * 128] = acc[c];
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_d), "r"(kTmem) : "memory");
+  }
+}
+
+// dw[o][i] and db[o]: the blocks' partials in order, eight loads in flight.
+__global__ void __launch_bounds__(128) rows8_wgrad_join(const float *partial, const float *partial_db, float *dw, float *db, int k, int n,
+                                                        int k_blocks, int parts) {
+  dependency_wait();
+  const int64_t i = blockIdx.x * 128ll + threadIdx.x, kn = static_cast<int64_t>(k) * n;
+  const float *p;
+  int64_t step;
+  if (i < kn) {
+    const int o = static_cast<int>(i / k), c = static_cast<int>(i % k);
+    const int64_t pair = c / 128 + static_cast<int64_t>(k_blocks) * (o / 128);
+    p = partial + (pair * parts * 128 + o % 128) * 128 + c % 128;
+    step = 128 * 128;
+  } else if (db != nullptr && i < kn + n) {
+    p = partial_db + (i - kn);
+    step = n;
+  } else {
+    return;
+  }
+  float s = 0.f;
+  int q = 0;
+  for (; q + 8 <= parts; q += 8) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = p[(q + u) * step];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += v[u];
+  }
+  for (; q < parts; ++q) s += p[q * step];
+  if (i < kn)
+    dw[i] = s;
+  else
+    db[i - kn] = s;
+}
+
+__device__ int32_t r8_status;  // set when a bounded wait ran out, cleared by cxg_rows8_wgrad_status
+
+int parts_of(int k, int n, int64_t m) {
+  const int64_t pairs = static_cast<int64_t>((k + 127) / 128) * ((n + 127) / 128);
+  const int64_t tiles = (m + kPos - 1) / kPos, parts = pairs < kNumSM ? kNumSM / pairs : 1;
+  return static_cast<int>(parts < tiles ? parts : tiles);
+}
+
+}  // namespace
+}  // namespace cxg
+
+using namespace cxg;
+
+extern "C" int cxg_rows8_wgrad_workspace_size(int64_t m, int k, int n, size_t *bytes) {
+  CXG_REQUIRE(bytes != nullptr, CXG_ENULL, "cxg_rows8_wgrad_workspace_size: bytes is NULL");
+  CXG_REQUIRE(m >= 0 && k > 0 && n > 0, CXG_EINVAL, "cxg_rows8_wgrad_workspace_size: bad sizes");
+  const size_t pairs = static_cast<size_t>((k + 127) / 128) * ((n + 127) / 128), parts = static_cast<size_t>(parts_of(k, n, m));
+  *bytes = parts * (pairs * 128 * 128 + n) * sizeof(float);
+  return CXG_OK;
+}
+
+extern "C" int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m, int k, const void *dy, int dtype, int64_t ld, int n,
+                               uint32_t flags, float *dw, float *db, void *workspace, size_t workspace_bytes, void *stream) {
+  CXG_REQUIRE(m >= 0 && k > 0 && n > 0 && ld >= n && (dtype == CXG_F32 || dtype == CXG_BF16), CXG_EINVAL,
+              "cxg_rows8_wgrad: bad sizes or type");
+  CXG_REQUIRE(dw != nullptr, CXG_ENULL, "cxg_rows8_wgrad: dw is NULL");
+  const int k_blocks = (k + 127) / 128, n_blocks = (n + 127) / 128;
+  CXG_REQUIRE(static_cast<int64_t>(k_blocks) * n_blocks <= 65535 && static_cast<int64_t>(k) * n < (1ll << 31), CXG_EUNSUPPORTED,
+              "cxg_rows8_wgrad: a weight of %d x %d", n, k);
+  cudaStream_t st = as_stream(stream);
+  if (m == 0) {
+    cudaError_t e = cudaMemsetAsync(dw, 0, sizeof(float) * static_cast<size_t>(k) * n, st);
+    if (e == cudaSuccess && db != nullptr) e = cudaMemsetAsync(db, 0, sizeof(float) * n, st);
+    return e == cudaSuccess ? CXG_OK : set_error(CXG_ECUDA, "cxg_rows8_wgrad: %s", cudaGetErrorString(e));
+  }
+  CXG_REQUIRE(codes && scales && dy, CXG_ENULL, "cxg_rows8_wgrad: NULL argument");
+  CXG_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 16 == 0, CXG_EINVAL, "cxg_rows8_wgrad: codes must be 16-byte aligned");
+  size_t need = 0;
+  cxg_rows8_wgrad_workspace_size(m, k, n, &need);
+  CXG_REQUIRE(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, CXG_EWORKSPACE,
+              "cxg_rows8_wgrad: workspace %zu bytes, need %zu", workspace_bytes, need);
+  const int parts = parts_of(k, n, m), elem = dtype == CXG_F32 ? 4 : 2;
+  R8Args a = {};
+  a.codes = static_cast<const uint8_t *>(codes), a.scales = static_cast<const uint8_t *>(scales), a.dy = dy;
+  a.m = m, a.ld = ld, a.k = k, a.n = n, a.groups = rows8::groups_of(k), a.pitch = a.groups * kGroup, a.k_blocks = k_blocks;
+  a.test_stall = (flags & CXG_WGRAD_TEST_STALL) ? 1 : 0;
+  a.partial = static_cast<float *>(workspace);
+  a.partial_db = db != nullptr ? a.partial + static_cast<size_t>(k_blocks) * n_blocks * parts * (128 * 128) : nullptr;
+  a.wait_cycles = wait_limit_cycles();
+  const int spans = n > 64 ? 2 : 1;
+  const int stage = (2 + (dtype == CXG_F32 ? 3 : 1) * spans) * kSpan;
+  a.stages = (kSmemBudget - 1024) / stage < kMaxStages ? (kSmemBudget - 1024) / stage : kMaxStages;
+  a.chunk = (dtype == CXG_F32 ? 512 : 1024) / kPos;
+  const int smem = 1024 + a.stages * stage;
+  void *word = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&word, r8_status);
+  a.status = static_cast<int32_t *>(word);
+  const bool vec = (static_cast<uint64_t>(ld) * elem | static_cast<uint64_t>(n) * elem | reinterpret_cast<uintptr_t>(dy)) % 16 == 0;
+  const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(k_blocks * n_blocks));
+  auto go = [&](auto kernel) {
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = launch_dependent(kernel, grid, kThreads, smem, st, a);
+  };
+  auto by_spans = [&](auto one, auto two) { spans == 1 ? go(one) : go(two); };
+  if (dtype == CXG_F32)
+    vec ? by_spans(rows8_wgrad<float, true, 1>, rows8_wgrad<float, true, 2>)
+        : by_spans(rows8_wgrad<float, false, 1>, rows8_wgrad<float, false, 2>);
+  else
+    vec ? by_spans(rows8_wgrad<__nv_bfloat16, true, 1>, rows8_wgrad<__nv_bfloat16, true, 2>)
+        : by_spans(rows8_wgrad<__nv_bfloat16, false, 1>, rows8_wgrad<__nv_bfloat16, false, 2>);
+  if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_wgrad: %s", cudaGetErrorString(e));
+  const int64_t outs = static_cast<int64_t>(k) * n + (db != nullptr ? n : 0);
+  launch_dependent(rows8_wgrad_join, static_cast<unsigned>((outs + 127) / 128), 128, 0, st, a.partial, a.partial_db, dw, db, k, n,
+                   k_blocks, parts);
+  count_launches(2);
+  return check_launch("cxg_rows8_wgrad");
+}
+
+extern "C" int cxg_rows8_wgrad_status(void *stream) {
+  void *word = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&word, r8_status);
+  if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_wgrad_status: %s", cudaGetErrorString(e));
+  return take_status_word(word, stream, "cxg_rows8_wgrad");
+}

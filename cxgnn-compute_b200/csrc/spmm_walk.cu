@@ -447,6 +447,22 @@ size_t walk_copy_bytes(const cxg_spmm_desc *d, int64_t n_src) {
   return static_cast<size_t>(n_src) * copy_pitch(row_bytes);
 }
 
+cudaError_t walk_fix_run(const WalkArgs &a, int dtype, cudaStream_t st) {
+  // tiles a warp looks over: one while the chip holds a warp for each, up to sixteen (two roles on 32 lanes)
+  int per = 1;
+  while (per < 16 && a.max_tiles > static_cast<int64_t>(per) * kNumSM * 24) per *= 2;
+  const int per_block = kFixThreads / 32 * per;
+  const unsigned fg = static_cast<unsigned>((a.max_tiles + per_block - 1) / per_block);
+  const bool v4 = a.part_stride % 4 == 0;
+  int lanes = 1;  // per chain
+  while (lanes < 32 && lanes * (v4 ? 4 : 1) < a.width) lanes *= 2;
+  if (dtype == CXG_F32)
+    return v4 ? launch_dependent(walk_fix<float, 4>, fg, kFixThreads, 0, st, a, per, lanes)
+              : launch_dependent(walk_fix<float, 1>, fg, kFixThreads, 0, st, a, per, lanes);
+  return v4 ? launch_dependent(walk_fix<__nv_bfloat16, 4>, fg, kFixThreads, 0, st, a, per, lanes)
+            : launch_dependent(walk_fix<__nv_bfloat16, 1>, fg, kFixThreads, 0, st, a, per, lanes);
+}
+
 int walk_launch(const cxg_spmm_desc *d, bool whole_rows, int64_t n_src, void *rows, void *workspace, size_t workspace_bytes,
                 cudaStream_t st) {
   const bool copied = rows != nullptr;
@@ -492,21 +508,7 @@ int walk_launch(const cxg_spmm_desc *d, bool whole_rows, int64_t n_src, void *ro
   }
   walk_plan_run(a, st);
   if (!dispatch(d, a, copied, st, nullptr)) return set_error(CXG_EUNSUPPORTED, "cxg_spmm_csr: rows of %d bytes", a.row_bytes);
-  // tiles a warp looks over: one while the chip holds a warp for each, up to sixteen (two roles on 32 lanes)
-  int per = 1;
-  while (per < 16 && L.max_tiles > static_cast<int64_t>(per) * kNumSM * 24) per *= 2;
-  const int per_block = kFixThreads / 32 * per;
-  const unsigned fg = static_cast<unsigned>((L.max_tiles + per_block - 1) / per_block);
-  const bool v4 = a.part_stride % 4 == 0;
-  int lanes = 1;  // per chain
-  while (lanes < 32 && lanes * (v4 ? 4 : 1) < a.width) lanes *= 2;
-  cudaError_t e;
-  if (d->dtype == CXG_F32)
-    e = v4 ? launch_dependent(walk_fix<float, 4>, fg, kFixThreads, 0, st, a, per, lanes)
-           : launch_dependent(walk_fix<float, 1>, fg, kFixThreads, 0, st, a, per, lanes);
-  else
-    e = v4 ? launch_dependent(walk_fix<__nv_bfloat16, 4>, fg, kFixThreads, 0, st, a, per, lanes)
-           : launch_dependent(walk_fix<__nv_bfloat16, 1>, fg, kFixThreads, 0, st, a, per, lanes);
+  const cudaError_t e = walk_fix_run(a, d->dtype, st);
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_spmm_csr: %s", cudaGetErrorString(e));
   count_launches(3);
   return check_launch("cxg_spmm_csr (walk)");

@@ -64,6 +64,8 @@ constexpr int64_t walk_part_stride(int64_t width) { return (width + 3) / 4 * 4; 
 bool walk_eligible(const cxg_spmm_desc *d);
 // The plan kernel for a.ptr, a.tile, a.whole_rows: fills hdr, tiles, count (and sets a.tile_magic).
 void walk_plan_run(WalkArgs &a, cudaStream_t st);
+// The fix-up of the plan's tiles and their partials; y is of type dtype (CXG_F32, CXG_BF16).
+cudaError_t walk_fix_run(const WalkArgs &a, int dtype, cudaStream_t st);
 // The walk alone over the plan and the weights per (edge, head) in `a` (fp32 rows in vectors of vb bytes, heads a power of two),
 // behind which walk_weights_slack bytes can be read. With resident_tiles set it only tells how many tiles are walked at the
 // same time. False, too, for tiles of more than kWeightedTile edges.

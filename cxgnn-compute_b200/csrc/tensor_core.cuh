@@ -60,6 +60,42 @@ __device__ __forceinline__ uint32_t make_idesc(int fmt, int m, int n) {
   return d;
 }
 
+// MN-major operand in a 128-byte swizzled layout: rows of 128 bytes (one per step of the contraction index), `lbo`
+// bytes between 128-byte spans along M / N. 16-bit elements: groups of 8 rows 1024 bytes apart, the 16-byte chunks of
+// a row permuted by row % 8 (layout type 2). 32-bit elements have their own form, the only one the tensor core takes
+// for MN-major TF32 operands: groups of 4 rows 512 bytes apart, the 32-byte chunks of a row permuted by row % 4
+// (layout type 1, "128-byte swizzle with a 32-byte base").
+template <bool W32>
+__device__ __forceinline__ uint64_t make_desc_mn_sw128(uint32_t addr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3fff);
+  d |= static_cast<uint64_t>((lbo >> 4) & 0x3fff) << 16;
+  d |= static_cast<uint64_t>((W32 ? 512 : 1024) >> 4) << 32;
+  d |= 1ull << 46;  // descriptor version of sm_100
+  d |= (W32 ? 1ull : 2ull) << 61;
+  return d;
+}
+
+// Byte offset of 16-byte chunk c16 of row p inside a span of either layout.
+template <bool W32>
+__device__ __forceinline__ uint32_t swizzled_offset(int p, int c16) {
+  if (W32) return p * 128 + ((((c16 >> 1) ^ (p & 3)) << 5) | ((c16 & 1) << 4));
+  return p * 128 + ((c16 ^ (p & 7)) << 4);
+}
+
+// fp32 accumulate, A and B of format `fmt` (1 = bf16, 2 = tf32), both MN-major.
+__device__ __forceinline__ uint32_t make_idesc_mn(int fmt, int m, int n) {
+  uint32_t d = 0;
+  d |= 1u << 4;
+  d |= static_cast<uint32_t>(fmt) << 7;
+  d |= static_cast<uint32_t>(fmt) << 10;
+  d |= 1u << 15;  // A is MN-major
+  d |= 1u << 16;  // B is MN-major
+  d |= static_cast<uint32_t>(n >> 3) << 17;
+  d |= static_cast<uint32_t>(m >> 4) << 24;
+  return d;
+}
+
 // One MMA of a warp: every lane comes here with the same operands and one of them issues it. (Behind `if (lane == 0)` the
 // compiler cannot tell that the operands are the same in all active lanes and an instruction took 134 cycles whatever its
 // size; issued this way 73, and 135 for 128 x 256, which is the tensor core's own time.)

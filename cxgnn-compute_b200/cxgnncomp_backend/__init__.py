@@ -229,6 +229,7 @@ _tmm_status = _sig("cxg_typed_matmul_status", [_vp, _vp])
 _wgrad_status = _sig("cxg_typed_wgrad_status", [_vp, _vp])
 _linear_status = _sig("cxg_linear_f32_status", [_vp])
 _dense_wgrad_status = _sig("cxg_dense_wgrad_f32_status", [_vp])
+_rows8_wgrad_status = _sig("cxg_rows8_wgrad_status", [_vp])
 
 
 def check_device_status(kind="spmm", device=None):
@@ -236,13 +237,14 @@ def check_device_status(kind="spmm", device=None):
     limit instead of spinning forever) or, for "spmm", ptr[num_node] exceeded the length of idx.
     "spmm", "typed_matmul", "typed_wgrad": asks about the LAST call on this stream, if it was of that kind (the calls of one
     stream share a scratch buffer, which holds the record; for any other last call nothing is checked).
-    "linear": asks about all fp32 linear transforms of the layers and their gradients (cxg_linear_f32, cxg_dense_wgrad_f32)
-    on this device since they were asked about last."""
+    "linear": asks about all fp32 linear transforms of the layers and their gradients (cxg_linear_f32, cxg_dense_wgrad_f32,
+    cxg_rows8_wgrad) on this device since they were asked about last."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if kind == "linear":
         with _on(device):
             failed = [(fn(_stream()), name) for fn, name in ((_linear_status, "cxg_linear_f32_status"),
-                                                             (_dense_wgrad_status, "cxg_dense_wgrad_f32_status"))]
+                                                             (_dense_wgrad_status, "cxg_dense_wgrad_f32_status"),
+                                                             (_rows8_wgrad_status, "cxg_rows8_wgrad_status"))]
         for rc, name in failed:
             _check(rc, name)
         return
@@ -1232,6 +1234,9 @@ from ._rgcn import (pad_rel, pad_rel_idx, typed_linear, typed_linear_s2e, typed_
                     aggr_rgcn_direct_func, rel_schedule, typed_matmul_raw, topo_sort, aggr_rel_direct,
                     typed_matmul_all_relations, typed_matmul_all_relations_supported, transform_all_relations,
                     dense_linear, typed_wgrad, typed_wgrad_supported)
+
+from ._rows8 import (Rows8, quantize_rows, dequantize_rows, rows8_aggregate, rows8_weight_grad,  # noqa: E402,F401
+                     linear_kept8, residual_norm)
 
 # pybind's export_values(): the enum members are module attributes too
 SUM, MAX, MIN, MEAN = REDUCEOP.SUM, REDUCEOP.MAX, REDUCEOP.MIN, REDUCEOP.MEAN

@@ -663,6 +663,78 @@ int cxg_typed_matmul(const void *a, const void *w, void *c, const int64_t *rel,
 int cxg_spmm_csr_static(const cxg_spmm_desc *desc, void *stream);
 int cxg_spmm_csr_static_status(void *stream);
 
+/*
+ * ---- rows held in 8 bits --------------------------------------------------
+ * Activations that a backward pass needs again, feature tables and caches of hidden states, at a quarter of fp32 and about
+ * half of bf16. No counterpart in the reference.
+ *
+ * A row is cut into groups of 32 values; a group is held as a byte e, which stands for s = 2^(e - 127), and a whole number c of
+ * -127 .. 127 per value, which stands for c * s. e is the smallest with max|x| / s < 127.5, kept within 1 .. 248; c = x / s
+ * rounded to nearest, ties to even. The values are exact in fp32 and bf16, and off by at most s / 2, at most 2^-7 of the
+ * group's largest. A group with a value that is not finite (e = 255) reads as NaN throughout.
+ *
+ * codes: [rows + 1][cxg_rows8_pitch(width)] bytes, 16-byte aligned, zeros behind the width; scales: [rows + 1][pitch / 32]
+ * bytes. The row behind the last is of zeros: it is what ids outside [0, rows) are read as.
+ */
+int cxg_rows8_pitch(int width);
+/* Rows [0, n) of x ([n, width], row i at x + i * ld values; CXG_F32 or CXG_BF16) to rows [0, n); zero_row: row n is written
+   with zeros too (n is then the number of rows). */
+int cxg_rows8_write(const void *x, int dtype, int64_t ld, int64_t n, int width, void *codes, void *scales, int zero_row,
+                    void *stream);
+/* Row i of x to row index[i]; ids outside [0, rows) are left out, and of positions with the same id the last one counts.
+   owner: int32 [rows], all -1, as it is again when the call has run. Calls that write the same rows have to be ordered by the
+   caller. n < 2^31. */
+int cxg_rows8_write_at_workspace_size(int64_t n, size_t *bytes);
+int cxg_rows8_write_at(const void *x, int dtype, int64_t ld, int64_t n, int width, const int64_t *index, void *codes, void *scales,
+                       int64_t rows, int32_t *owner, void *workspace, size_t workspace_bytes, void *stream);
+/* out[i] ([n, width], rows ld values apart) = row index[i], or row i where index is NULL (n <= rows). */
+int cxg_rows8_read(const void *codes, const void *scales, int64_t rows, int width, const int64_t *index, int64_t n, void *out,
+                   int dtype, int64_t ld, void *stream);
+/* y[d, :] = sum or mean over row d of the CSR graph of [edge_val[e] *] row idx[e]: cxg_spmm_csr over rows in 8 bits, sums in
+   fp32 in edge order, the same bits on every run. idx outside [0, n_src): a row of zeros. y: [n_dst, width] of y_dtype.
+   Widths up to 2048; split_edges as in cxg_spmm_desc. Rows and edges below 2^31 - 2^20. An edge count ptr[n_dst] above nnz is
+   cut to nnz and reported by cxg_spmm_csr_status(workspace). */
+int cxg_rows8_aggregate_workspace_size(int64_t nnz, int width, int split_edges, size_t *bytes);
+int cxg_rows8_aggregate(const void *codes, const void *scales, int64_t n_src, int width, const void *ptr, int ptr_bytes,
+                        const void *idx, int idx_bytes, const float *edge_val, int64_t n_dst, int64_t nnz, int reduce,
+                        int split_edges, void *y, int y_dtype, void *workspace, size_t workspace_bytes, void *stream);
+/* dw [n, k] = dy^T . rows, db [n] = column sums of dy (NULL: not wanted), both fp32: the gradients of a linear transform whose
+   input (m rows of width k) was kept in 8 bits. dy: [m, n], rows ld values apart. The rows are exact bf16 operands of the
+   tensor core; fp32 dy is cut into three bf16 parts, which hold all of its bits. flags: 0 or CXG_WGRAD_TEST_STALL. The status of its bounded waits:
+   cxg_rows8_wgrad_status. */
+int cxg_rows8_wgrad_workspace_size(int64_t m, int k, int n, size_t *bytes);
+int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m, int k, const void *dy, int dtype, int64_t ld, int n, uint32_t flags, float *dw,
+                    float *db, void *workspace, size_t workspace_bytes, void *stream);
+int cxg_rows8_wgrad_status(void *stream);
+
+/*
+ * ---- the step between two blocks of a residual network --------------------
+ * n = post ? norm(f) * post_weight + post_bias : f;  y = x + scale * sigmoid(gate) * n;  h = norm(y) * next_weight + next_bias
+ * row by row. norm: (v - mean) / sqrt(var + eps) with layer, v / sqrt(mean v^2 + eps) without. Matrices [n, width] of `dtype`,
+ * contiguous; parameters fp32 [width], NULL: ones (weights, scale) or zeros (biases). f == NULL: h = norm(x) alone (next, no
+ * gate, no post). h is computed from y before y is rounded to `dtype`. Widths up to cxg_residual_norm_max_width().
+ */
+#define CXG_GATE_NONE 0
+#define CXG_GATE_VALUE 1 /* gate [n, width] */
+#define CXG_GATE_ROW 2   /* gate [n] */
+typedef struct cxg_residual_desc {
+  const void *x, *f, *gate;
+  const float *scale, *post_weight, *post_bias, *next_weight, *next_bias;
+  void *y, *h;          /* forward: outputs; y may be NULL */
+  void *codes, *scales; /* forward: h in 8 bits too (n > 0), NULL: not wanted; only where cxg_residual_norm_keeps says 1 */
+  const void *dy, *dh;  /* backward: gradients of y and h, NULL: zeros */
+  void *dx, *df, *dgate;/* backward: outputs, NULL: not wanted */
+  int64_t n;
+  int32_t width, dtype, gate_mode, layer, post, next;
+  float eps;
+} cxg_residual_desc;
+int cxg_residual_norm_max_width(void);
+int cxg_residual_norm_keeps(const cxg_residual_desc *desc);
+int cxg_residual_norm_forward(const cxg_residual_desc *desc, void *stream);
+/* sums: fp32 [5][width], the gradients of scale, post_weight, post_bias, next_weight, next_bias, added in a fixed order. */
+int cxg_residual_norm_backward_workspace_size(int64_t n, int width, size_t *bytes);
+int cxg_residual_norm_backward(const cxg_residual_desc *desc, float *sums, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
