@@ -10,20 +10,22 @@
 // y, the statistics and the normalised rows are computed again from x, f and gate: reading a row's statistics would save
 // two of its reductions, reading y instead of x nothing.
 //
-// Both are bound by memory: a row is read once, held in registers (8 values per lane; a part of a warp, a warp or up to
-// 16 warps per row), and written once. Statistics, products and sums are fp32 whatever the rows' type; y is rounded when it is
-// stored, h is computed from it before. The sums over rows are kept per lane for the whole grid's pass, added up per block,
-// and the blocks' sums are added in order by a second kernel: the same bits on every run.
+// Both are bound by memory: a row is read once, held in registers (16 bytes of every matrix per lane; a part of a warp, a warp
+// or up to 16 warps per row), and written once. A warp asks for its next row before it works on the one that it has: its
+// chains of shuffles (up to nine sums of a row, one behind the other, for the layer norms' gradients) are longer than what
+// the other warps of an SM cover. Parameters come out of L1 for every row; held in registers they cost a third of the warps.
+// Statistics, products and sums are fp32 whatever the rows' type; y is rounded when it is stored, h is computed from it before.
+// The sums over rows are kept per lane for the whole grid's pass, added up per block, and the blocks' sums are added in order
+// by a second kernel: the same bits on every run.
 #include "rows8.cuh"
 
 namespace cxg {
 namespace {
 
-constexpr int kValues = 8;     // of a row per lane
 constexpr int kSums = 5;       // dscale, dw2, db2, dw1, db1
 constexpr int kMostWarps = 16;
-constexpr int kMostWidth = kMostWarps * 32 * kValues;
-constexpr int kBlock = 256;    // threads where a row takes a warp or less
+constexpr int kMostWidth = 4096;
+constexpr int kBlock = 128;    // threads where a row takes a warp or less
 
 struct ResArgs {
   cxg_residual_desc d;
@@ -32,40 +34,56 @@ struct ResArgs {
   int keep, groups;  // forward: rows in 8 bits of h
 };
 
-// Where a lane's values lie: vectors of N values, the lanes' first vectors side by side, then their second ones.
-template <typename T, bool VEC>
+// Where a lane's values lie: Q vectors of N values, the lanes' first vectors side by side, then their second ones. Rows that are
+// not whole 16-byte vectors are read value by value, as many per lane.
+template <typename T, bool VEC, int VECTORS>
 struct Place {
   static constexpr int N = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
-  static constexpr int Q = kValues / N;
+  static constexpr int Q = VEC ? VECTORS : VECTORS * 16 / static_cast<int>(sizeof(T));
+  static constexpr int V = N * Q;  // values
+  using Element = T;
+  static constexpr bool kVec = VEC;
 };
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_row(float (&v)[kValues], const void *base, int64_t row, int width, int p, int lanes) {
-  using P = Place<T, VEC>;
-  const T *src = static_cast<const T *>(base) + row * width;
+// A lane's part of a row as it was loaded.
+template <typename P>
+struct Raw {
+  using T = typename P::Element;
+  typename Vec<T>::Raw v[P::kVec ? P::Q : 1];
+  T e[P::kVec ? 1 : P::Q];
+  __device__ __forceinline__ void load(const void *base, int64_t row, int width, int p, int lanes) {
+    const T *src = static_cast<const T *>(base) + row * width;
 #pragma unroll
-  for (int q = 0; q < P::Q; ++q) {
-    const int c = (q * lanes + p) * P::N;
-    if constexpr (VEC) {
-      if (c < width) Vec<T>::to_float(v + q * P::N, Vec<T>::load(src + c));
-      else
-#pragma unroll
-        for (int i = 0; i < P::N; ++i) v[q * P::N + i] = 0.f;
-    } else {
-      v[q] = c < width ? to_f32(__ldg(src + c)) : 0.f;
+    for (int q = 0; q < P::Q; ++q) {
+      const int c = (q * lanes + p) * P::N;
+      if constexpr (P::kVec) {
+        v[q] = {};
+        if (c < width) v[q] = Vec<T>::load(src + c);
+      } else {
+        e[q] = from_f32<T>(0.f);
+        if (c < width) e[q] = __ldg(src + c);
+      }
     }
   }
-}
+  __device__ __forceinline__ void get(float (&f)[P::V]) const {
+#pragma unroll
+    for (int q = 0; q < P::Q; ++q)
+      if constexpr (P::kVec)
+        Vec<T>::to_float(f + q * P::N, v[q]);
+      else
+        f[q] = to_f32(e[q]);
+  }
+};
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_row(void *base, int64_t row, int width, int p, int lanes, const float (&v)[kValues]) {
-  using P = Place<T, VEC>;
+template <typename P>
+__device__ __forceinline__ void store_row(void *base, int64_t row, int width, int p, int lanes, const float (&v)[P::V]) {
+  using T = typename P::Element;
   T *dst = static_cast<T *>(base) + row * width;
 #pragma unroll
   for (int q = 0; q < P::Q; ++q) {
     const int c = (q * lanes + p) * P::N;
     if (c < width) {
-      if constexpr (VEC)
+      if constexpr (P::kVec)
         Vec<T>::store_stream(dst + c, Vec<T>::from_float(v + q * P::N));
       else
         dst[c] = from_f32<T>(v[q]);
@@ -73,24 +91,24 @@ __device__ __forceinline__ void store_row(void *base, int64_t row, int width, in
   }
 }
 
-// A parameter's values at the lane's columns (`other` where there is no parameter, zeros behind the row).
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_param(float (&v)[kValues], const float *w, float other, int width, int p, int lanes) {
-  using P = Place<T, VEC>;
+// A parameter's values at the lane's columns (`other` where there is no parameter; anything behind the row).
+template <typename P>
+__device__ __forceinline__ void load_param(float (&v)[P::V], const float *w, float other, int width, int p, int lanes) {
+#pragma unroll
+  for (int i = 0; i < P::V; ++i) v[i] = other;
+  if (w == nullptr) return;
 #pragma unroll
   for (int q = 0; q < P::Q; ++q) {
     const int c = (q * lanes + p) * P::N;
+    if (c >= width) continue;
+    if constexpr (P::kVec) {
 #pragma unroll
-    for (int i = 0; i < P::N; i += VEC ? 4 : 1) {
-      if (w == nullptr || c + i >= width) {
-#pragma unroll
-        for (int k = 0; k < (VEC ? 4 : 1); ++k) v[q * P::N + i + k] = c + i < width ? other : 0.f;
-      } else if constexpr (VEC) {
+      for (int i = 0; i < P::N; i += 4) {
         const float4 t = __ldg(reinterpret_cast<const float4 *>(w + c + i));
         v[q * P::N + i] = t.x, v[q * P::N + i + 1] = t.y, v[q * P::N + i + 2] = t.z, v[q * P::N + i + 3] = t.w;
-      } else {
-        v[q] = __ldg(w + c);
       }
+    } else {
+      v[q] = __ldg(w + c);
     }
   }
 }
@@ -136,32 +154,39 @@ struct RowSum {
   }
 };
 
-// v becomes norm(v); returns the factor. Values behind the row (column >= width) become zeros.
-template <typename T, bool VEC, typename Sum>
-__device__ __forceinline__ float normalise(float (&v)[kValues], const ResArgs &a, Sum &sum, int p, int lanes) {
-  using P = Place<T, VEC>;
+// v becomes norm(v); returns the factor. Values behind the row (zeros before) stay zeros.
+template <typename P, typename Sum>
+__device__ __forceinline__ float normalise(float (&v)[P::V], const ResArgs &a, Sum &sum, int p, int lanes) {
   if (a.d.layer) {
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < kValues; ++i) t += v[i];
+    for (int i = 0; i < P::V; ++i) t += v[i];
     const float mean = sum.one(t) * a.inv_width;
 #pragma unroll
-    for (int i = 0; i < kValues; ++i) v[i] = ((i / P::N) * lanes + p) * P::N + i % P::N < a.d.width ? v[i] - mean : 0.f;
+    for (int q = 0; q < P::Q; ++q) {
+      const float off = (q * lanes + p) * P::N < a.d.width ? mean : 0.f;
+#pragma unroll
+      for (int i = 0; i < P::N; ++i) v[q * P::N + i] -= off;
+    }
   }
   float t = 0.f;
 #pragma unroll
-  for (int i = 0; i < kValues; ++i) t = fmaf(v[i], v[i], t);
+  for (int i = 0; i < P::V; ++i) t = fmaf(v[i], v[i], t);
   const float r = __frsqrt_rn(fmaf(sum.one(t), a.inv_width, a.d.eps));
 #pragma unroll
-  for (int i = 0; i < kValues; ++i) v[i] *= r;
+  for (int i = 0; i < P::V; ++i) v[i] *= r;
   return r;
 }
 
-// sigmoid and its derivative without cancellation: t = exp(-|g|), s = 1 / (1 + t) or t / (1 + t), s' = t / (1 + t)^2
+// sigmoid and its derivative without cancellation: t = exp(-|g|), s = 1 / (1 + t) or t / (1 + t), s' = t / (1 + t)^2. The
+// reciprocal of 1 .. 2 is the hardware's, off by an ulp.
 __device__ __forceinline__ void sigmoid(float g, float *s, float *ds) {
-  const float t = expf(-fabsf(g)), q = __frcp_rn(1.f + t);
-  *s = g >= 0.f ? q : t * q;
-  *ds = t * q * q;
+  const float t = expf(-fabsf(g));
+  float q;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + t));
+  const float tq = t * q;
+  *s = g >= 0.f ? q : tq;
+  *ds = tq * q;
 }
 
 // Rows of the grid: `per` per block at a time; the lanes of a warp go through the loop together.
@@ -178,107 +203,126 @@ struct Rows {
   }
 };
 
-template <typename T, int LANES, int WARPS, bool VEC>
-__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock) residual_forward(const __grid_constant__ ResArgs a) {
-  using P = Place<T, VEC>;
+// h in 8 bits as it is stored, to row `row`; zeros where `in` is false.
+template <typename P>
+__device__ __forceinline__ void keep_row(const ResArgs &a, int64_t row, bool in, const float (&h)[P::V], int p, int lanes) {
+  using T = typename P::Element;
+  constexpr int kShare = rows8::kGroup / P::N;  // lanes that hold a group
+#pragma unroll
+  for (int q = 0; q < P::Q; ++q) {
+    const int c = (q * lanes + p) * P::N;
+    float v[P::N];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < P::N; ++i) {
+      v[i] = in && c < a.d.width ? to_f32(from_f32<T>(h[q * P::N + i])) : 0.f;
+      top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int k = 1; k < kShare; k <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
+    const uint32_t e = rows8::scale_byte(top);
+    uint32_t w[P::N / 4];
+    rows8::codes_of<P::N>(w, v, e);
+    if (row <= a.d.n && c < a.groups * rows8::kGroup) {
+      uint8_t *out = static_cast<uint8_t *>(a.d.codes) + row * (static_cast<int64_t>(a.groups) * rows8::kGroup) + c;
+      if constexpr (P::N == 4)
+        *reinterpret_cast<uint32_t *>(out) = w[0];
+      else
+        *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[P::N / 4 - 1]);
+      if (c % rows8::kGroup == 0)
+        static_cast<uint8_t *>(a.d.scales)[row * a.groups + c / rows8::kGroup] = static_cast<uint8_t>(e);
+    }
+  }
+}
+
+// Warps per SM: 64 registers a thread forward, 128 backward, 168 where eight values per lane meet five sums of each (with 128
+// registers these spill 250 bytes a lane).
+constexpr int forward_warps(int values, bool gated) { return values > 4 && gated ? 24 : 32; }
+constexpr int backward_warps(int values, bool biases) { return values > 4 && biases ? 12 : 16; }
+
+// Blocks per SM of `threads` threads with that many warps.
+constexpr int blocks_of(int warps, int threads) { return warps * 32 / threads > 0 ? warps * 32 / threads : 1; }
+
+// GATED: a gate per value.
+template <typename T, int LANES, int WARPS, bool VEC, int VECTORS, bool GATED>
+__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock,
+                                  blocks_of(forward_warps(Place<T, VEC, VECTORS>::V, GATED), WARPS > 1 ? 32 * WARPS : kBlock))
+    residual_forward(const __grid_constant__ ResArgs a) {
+  using P = Place<T, VEC, VECTORS>;
   constexpr int kLanes = LANES * WARPS;
   __shared__ float2 place[2][WARPS];
   RowSum<LANES, WARPS> sum(place);
   const cxg_residual_desc &d = a.d;
   const int p = threadIdx.x & (kLanes - 1), width = d.width;
+  const bool with_f = d.f != nullptr, row_gate = d.gate_mode == CXG_GATE_ROW;
   dependency_wait();
-  float scale[kValues], w2[kValues], b2[kValues], w1[kValues], b1[kValues];
-  load_param<T, VEC>(scale, d.scale, 1.f, width, p, kLanes);
-  load_param<T, VEC>(w2, d.post_weight, 1.f, width, p, kLanes);
-  load_param<T, VEC>(b2, d.post_bias, 0.f, width, p, kLanes);
-  load_param<T, VEC>(w1, d.next_weight, 1.f, width, p, kLanes);
-  load_param<T, VEC>(b1, d.next_bias, 0.f, width, p, kLanes);
   const Rows<LANES, WARPS> rows;
-  for (int64_t row0 = rows.first; row0 < d.n + a.keep; row0 += rows.step) {
-    const int64_t row = row0 + rows.sub, at = row < d.n ? row : 0;
+  Raw<P> rx, rf, rg;
+  T rr = from_f32<T>(0.f);
+  auto load = [&](int64_t row) {
+    const int64_t at = row < d.n ? row : d.n - 1;
+    rx.load(d.x, at, width, p, kLanes);
+    if (with_f) rf.load(d.f, at, width, p, kLanes);
+    if (GATED) rg.load(d.gate, at, width, p, kLanes);
+    if (row_gate) rr = __ldg(static_cast<const T *>(d.gate) + at);
+  };
+  const int64_t n_end = d.n + a.keep;
+  if (rows.first < n_end) load(rows.first + rows.sub);
+  for (int64_t row0 = rows.first; row0 < n_end; row0 += rows.step) {
+    const int64_t row = row0 + rows.sub;
     const bool in = row < d.n;
-    float y[kValues];
-    if (in || WARPS == 1)
-      load_row<T, VEC>(y, d.x, at, width, p, kLanes);
-    else
-#pragma unroll
-      for (int i = 0; i < kValues; ++i) y[i] = 0.f;
-    if (d.f != nullptr) {
-      float n[kValues], g[kValues];
-      float g_row = 0.f;
-      if (in || WARPS == 1) {
-        load_row<T, VEC>(n, d.f, at, width, p, kLanes);
-        if (d.gate_mode == CXG_GATE_VALUE) load_row<T, VEC>(g, d.gate, at, width, p, kLanes);
-        if (d.gate_mode == CXG_GATE_ROW) g_row = to_f32(__ldg(static_cast<const T *>(d.gate) + at));
-      } else {
-#pragma unroll
-        for (int i = 0; i < kValues; ++i) n[i] = 0.f, g[i] = 0.f;
-      }
+    float y[P::V], n[P::V], s[P::V], one = 1.f, ds;
+    rx.get(y);
+    if (with_f) rf.get(n);
+    if (GATED) rg.get(s);
+    const float g_row = to_f32(rr);
+    if (row0 + rows.step < n_end) load(row + rows.step);
+    if (with_f) {
       if (d.post) {
-        normalise<T, VEC>(n, a, sum, p, kLanes);
+        normalise<P>(n, a, sum, p, kLanes);
+        float w[P::V], b[P::V];
+        load_param<P>(w, d.post_weight, 1.f, width, p, kLanes);
+        if (d.post_bias != nullptr) {
+          load_param<P>(b, d.post_bias, 0.f, width, p, kLanes);
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) n[i] = fmaf(n[i], w2[i], b2[i]);
-      }
-      float s = 1.f, ds;
-      if (d.gate_mode == CXG_GATE_ROW) sigmoid(g_row, &s, &ds);
+          for (int i = 0; i < P::V; ++i) n[i] = fmaf(n[i], w[i], b[i]);
+        } else {
 #pragma unroll
-      for (int i = 0; i < kValues; ++i) {
-        if (d.gate_mode == CXG_GATE_VALUE) sigmoid(g[i], &s, &ds);
-        y[i] = fmaf(scale[i] * s, n[i], y[i]);
+          for (int i = 0; i < P::V; ++i) n[i] *= w[i];
+        }
       }
-      if (d.y != nullptr && in) store_row<T, VEC>(d.y, row, width, p, kLanes, y);
+      if (row_gate) sigmoid(g_row, &one, &ds);
+      if (GATED) {
+#pragma unroll
+        for (int i = 0; i < P::V; ++i) sigmoid(s[i], &s[i], &ds);
+      }
+      float scale[P::V];
+      load_param<P>(scale, d.scale, 1.f, width, p, kLanes);
+#pragma unroll
+      for (int i = 0; i < P::V; ++i) y[i] = fmaf(scale[i] * (GATED ? s[i] : one), n[i], y[i]);
+      if (d.y != nullptr && in) store_row<P>(d.y, row, width, p, kLanes, y);
     }
     if (d.next) {
-      normalise<T, VEC>(y, a, sum, p, kLanes);
+      normalise<P>(y, a, sum, p, kLanes);
+      float w[P::V], b[P::V];
+      load_param<P>(w, d.next_weight, 1.f, width, p, kLanes);
+      load_param<P>(b, d.next_bias, 0.f, width, p, kLanes);
 #pragma unroll
-      for (int i = 0; i < kValues; ++i) y[i] = fmaf(y[i], w1[i], b1[i]);
-      if (in) store_row<T, VEC>(d.h, row, width, p, kLanes, y);
+      for (int i = 0; i < P::V; ++i) y[i] = fmaf(y[i], w[i], b[i]);
+      if (in) store_row<P>(d.h, row, width, p, kLanes, y);
       if constexpr (VEC) {
-        if (a.keep) {  // the rows in 8 bits of h as it is stored, and the row of zeros behind them
-          constexpr int kShare = rows8::kGroup / P::N;  // lanes that hold a group
-#pragma unroll
-          for (int q = 0; q < P::Q; ++q) {
-            const int c = (q * kLanes + p) * P::N;
-            float v[P::N];
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < P::N; ++i) {
-              v[i] = in ? to_f32(from_f32<T>(y[q * P::N + i])) : 0.f;
-              top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-            }
-#pragma unroll
-            for (int k = 1; k < kShare; k <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
-            const uint32_t e = rows8::scale_byte(top);
-            const float inv = e == rows8::kNotFinite ? 0.f : rows8::inverse_scale(e);
-            uint32_t w[P::N / 4];
-#pragma unroll
-            for (int i = 0; i < P::N / 4; ++i)
-              w[i] = e == rows8::kNotFinite
-                         ? 0u
-                         : rows8::pack_codes(rows8::code_bits(v[4 * i], inv), rows8::code_bits(v[4 * i + 1], inv),
-                                             rows8::code_bits(v[4 * i + 2], inv), rows8::code_bits(v[4 * i + 3], inv));
-            if (row <= d.n && c < a.groups * rows8::kGroup) {
-              uint8_t *out = static_cast<uint8_t *>(d.codes) + row * (static_cast<int64_t>(a.groups) * rows8::kGroup) + c;
-              if constexpr (P::N == 4)
-                *reinterpret_cast<uint32_t *>(out) = w[0];
-              else
-                *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[P::N / 4 - 1]);
-              if (c % rows8::kGroup == 0)
-                static_cast<uint8_t *>(d.scales)[row * a.groups + c / rows8::kGroup] = static_cast<uint8_t>(e);
-            }
-          }
-        }
+        if (a.keep) keep_row<P>(a, row, in, y, p, kLanes);
       }
     }
   }
 }
 
 // g becomes r (g - <g> - u <g u>) (without <g> where no mean was taken off)
-template <typename Sum>
-__device__ __forceinline__ void back_through_norm(float (&g)[kValues], const float (&u)[kValues], float r, const ResArgs &a, Sum &sum) {
+template <int V, typename Sum>
+__device__ __forceinline__ void back_through_norm(float (&g)[V], const float (&u)[V], float r, const ResArgs &a, Sum &sum) {
   float t0 = 0.f, t1 = 0.f;
 #pragma unroll
-  for (int i = 0; i < kValues; ++i) t0 += g[i], t1 = fmaf(g[i], u[i], t1);
+  for (int i = 0; i < V; ++i) t0 += g[i], t1 = fmaf(g[i], u[i], t1);
   float mean = 0.f, dot;
   if (a.d.layer) {
     const float2 t = sum.both(t0, t1);
@@ -287,135 +331,152 @@ __device__ __forceinline__ void back_through_norm(float (&g)[kValues], const flo
     dot = sum.one(t1) * a.inv_width;
   }
 #pragma unroll
-  for (int i = 0; i < kValues; ++i) g[i] = r * (fmaf(-u[i], dot, g[i]) - mean);
+  for (int i = 0; i < V; ++i) g[i] = r * (fmaf(-u[i], dot, g[i]) - mean);
 }
 
-template <typename T, int LANES, int WARPS, bool VEC>
-__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, WARPS > 1 ? kMostWarps / WARPS : 2)
+// BIASES: sums for them too.
+template <typename T, int LANES, int WARPS, bool VEC, int VECTORS, bool GATED, bool BIASES>
+__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock,
+                                  blocks_of(backward_warps(Place<T, VEC, VECTORS>::V, BIASES), WARPS > 1 ? 32 * WARPS : kBlock))
     residual_backward(const __grid_constant__ ResArgs a) {
-  using P = Place<T, VEC>;
+  using P = Place<T, VEC, VECTORS>;
   constexpr int kLanes = LANES * WARPS;
   __shared__ float2 place[2][WARPS];
   RowSum<LANES, WARPS> sum(place);
   const cxg_residual_desc &d = a.d;
   const int p = threadIdx.x & (kLanes - 1), width = d.width;
+  const bool with_f = d.f != nullptr, row_gate = d.gate_mode == CXG_GATE_ROW, next = d.next && d.dh != nullptr;
   dependency_wait();
-  float acc[kSums][kValues];
+  float acc[kSums][P::V];
 #pragma unroll
   for (int k = 0; k < kSums; ++k)
 #pragma unroll
-    for (int i = 0; i < kValues; ++i) acc[k][i] = 0.f;
+    for (int i = 0; i < P::V; ++i) acc[k][i] = 0.f;
   const Rows<LANES, WARPS> rows;
+  Raw<P> rx, rf, rg, ry, rh;
+  T rr = from_f32<T>(0.f);
+  auto load = [&](int64_t row) {
+    const int64_t at = row < d.n ? row : d.n - 1;
+    rx.load(d.x, at, width, p, kLanes);
+    if (with_f) rf.load(d.f, at, width, p, kLanes);
+    if (GATED) rg.load(d.gate, at, width, p, kLanes);
+    if (row_gate) rr = __ldg(static_cast<const T *>(d.gate) + at);
+    if (d.dy != nullptr) ry.load(d.dy, at, width, p, kLanes);
+    if (next) rh.load(d.dh, at, width, p, kLanes);
+  };
+  if (rows.first < d.n) load(rows.first + rows.sub);
   for (int64_t row0 = rows.first; row0 < d.n; row0 += rows.step) {
-    const int64_t row = row0 + rows.sub, at = row < d.n ? row : 0;
-    const bool in = row < d.n;
-    float y[kValues], n[kValues], s[kValues], ds[kValues], g[kValues], dh[kValues];
-    load_row<T, VEC>(y, d.x, at, width, p, kLanes);
-    if (d.f != nullptr) load_row<T, VEC>(n, d.f, at, width, p, kLanes);
-    if (d.gate_mode == CXG_GATE_VALUE) load_row<T, VEC>(s, d.gate, at, width, p, kLanes);
-    if (d.gate_mode == CXG_GATE_ROW) s[0] = to_f32(__ldg(static_cast<const T *>(d.gate) + at));
-    if (d.dy != nullptr)
-      load_row<T, VEC>(g, d.dy, at, width, p, kLanes);
-    else
+    const int64_t row = row0 + rows.sub;
+    const bool in = row < d.n;  // lanes without a row go through it with gradients of zero
+    float y[P::V], n[P::V], s[GATED ? P::V : 1], ds[GATED ? P::V : 1], g[P::V], dh[P::V];
+    rx.get(y);
+    if (with_f) rf.get(n);
+    if constexpr (GATED) rg.get(s);
+    const float g_row = to_f32(rr);
 #pragma unroll
-      for (int i = 0; i < kValues; ++i) g[i] = 0.f;
-    const bool next = d.next && d.dh != nullptr;
-    if (next) load_row<T, VEC>(dh, d.dh, at, width, p, kLanes);
-    if (!in) {  // lanes without a row go through it with gradients of zero
-#pragma unroll
-      for (int i = 0; i < kValues; ++i) g[i] = dh[i] = 0.f;
+    for (int i = 0; i < P::V; ++i) g[i] = dh[i] = 0.f;
+    if (in && d.dy != nullptr) ry.get(g);
+    if (in && next) rh.get(dh);
+    if (row0 + rows.step < d.n) load(row + rows.step);
+    float r2 = 0.f, scale[P::V];
+    if constexpr (!GATED) {
+      s[0] = 1.f, ds[0] = 0.f;
+      if (row_gate) sigmoid(g_row, &s[0], &ds[0]);
     }
-    float r2 = 0.f, scale[kValues];
-    if (d.f != nullptr) {
-      load_param<T, VEC>(scale, d.scale, 1.f, width, p, kLanes);
-      if (d.gate_mode == CXG_GATE_ROW) {
-        float s0, ds0;
-        sigmoid(s[0], &s0, &ds0);
+    if (with_f) {
+      load_param<P>(scale, d.scale, 1.f, width, p, kLanes);
+      if constexpr (GATED) {
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) s[i] = s0, ds[i] = ds0;
-      } else if (d.gate_mode == CXG_GATE_VALUE) {
-#pragma unroll
-        for (int i = 0; i < kValues; ++i) sigmoid(s[i], &s[i], &ds[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kValues; ++i) s[i] = 1.f, ds[i] = 0.f;
+        for (int i = 0; i < P::V; ++i) sigmoid(s[i], &s[i], &ds[i]);
       }
       if (d.post) {
-        r2 = normalise<T, VEC>(n, a, sum, p, kLanes);  // n is u2 from here on
-        float w2[kValues], b2[kValues];
-        load_param<T, VEC>(w2, d.post_weight, 1.f, width, p, kLanes);
-        load_param<T, VEC>(b2, d.post_bias, 0.f, width, p, kLanes);
+        r2 = normalise<P>(n, a, sum, p, kLanes);  // n is u2 from here on
+        float w2[P::V], b2[P::V];
+        load_param<P>(w2, d.post_weight, 1.f, width, p, kLanes);
+        load_param<P>(b2, d.post_bias, 0.f, width, p, kLanes);
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) y[i] = fmaf(scale[i] * s[i], fmaf(n[i], w2[i], b2[i]), y[i]);
+        for (int i = 0; i < P::V; ++i) y[i] = fmaf(scale[i] * s[GATED ? i : 0], fmaf(n[i], w2[i], b2[i]), y[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) y[i] = fmaf(scale[i] * s[i], n[i], y[i]);
+        for (int i = 0; i < P::V; ++i) y[i] = fmaf(scale[i] * s[GATED ? i : 0], n[i], y[i]);
       }
     }
     if (next) {
-      const float r1 = normalise<T, VEC>(y, a, sum, p, kLanes);  // y is u1 from here on
-      float t[kValues];
-      load_param<T, VEC>(t, d.next_weight, 1.f, width, p, kLanes);
+      const float r1 = normalise<P>(y, a, sum, p, kLanes);  // y is u1 from here on
+      float t[P::V];
+      load_param<P>(t, d.next_weight, 1.f, width, p, kLanes);
 #pragma unroll
-      for (int i = 0; i < kValues; ++i) {
+      for (int i = 0; i < P::V; ++i) {
         acc[3][i] = fmaf(dh[i], y[i], acc[3][i]);
-        acc[4][i] += dh[i];
+        if (BIASES) acc[4][i] += dh[i];
         t[i] *= dh[i];
       }
       back_through_norm(t, y, r1, a, sum);
 #pragma unroll
-      for (int i = 0; i < kValues; ++i) g[i] += t[i];
-    }
-    if (in && d.dx != nullptr) store_row<T, VEC>(d.dx, row, width, p, kLanes, g);
-    if (d.f != nullptr) {
-      float w2[kValues], b2[kValues], dg[kValues];
-      if (d.post) {
-        load_param<T, VEC>(w2, d.post_weight, 1.f, width, p, kLanes);
-        load_param<T, VEC>(b2, d.post_bias, 0.f, width, p, kLanes);
-      }
+      for (int i = 0; i < P::V; ++i) g[i] += t[i];
 #pragma unroll
-      for (int i = 0; i < kValues; ++i) {
-        const float v = d.post ? fmaf(n[i], w2[i], b2[i]) : n[i];
-        acc[0][i] = fmaf(g[i] * s[i], v, acc[0][i]);
-        g[i] *= scale[i];
-        dg[i] = g[i] * v * ds[i];
-        g[i] *= s[i];  // dn
+      for (int i = 0; i < P::V; ++i)
+        if (((i / P::N) * kLanes + p) * P::N >= width) g[i] = 0.f;
+    }
+    if (in && d.dx != nullptr) store_row<P>(d.dx, row, width, p, kLanes, g);
+    if (with_f) {
+      float w2[P::V], dg[P::V];
+#pragma unroll
+      for (int i = 0; i < P::V; ++i) dg[i] = n[i];
+      if (d.post) {
+        float b2[P::V];
+        load_param<P>(w2, d.post_weight, 1.f, width, p, kLanes);
+        load_param<P>(b2, d.post_bias, 0.f, width, p, kLanes);
+#pragma unroll
+        for (int i = 0; i < P::V; ++i) dg[i] = fmaf(n[i], w2[i], b2[i]);
       }
-      if (d.gate_mode == CXG_GATE_VALUE) {
-        if (in && d.dgate != nullptr) store_row<T, VEC>(d.dgate, row, width, p, kLanes, dg);
-      } else if (d.gate_mode == CXG_GATE_ROW) {
+      load_param<P>(scale, d.scale, 1.f, width, p, kLanes);
+#pragma unroll
+      for (int i = 0; i < P::V; ++i) {
+        acc[0][i] = fmaf(g[i] * s[GATED ? i : 0], dg[i], acc[0][i]);
+        g[i] *= scale[i];
+        dg[i] *= g[i] * ds[GATED ? i : 0];
+        g[i] *= s[GATED ? i : 0];  // dn
+      }
+      if constexpr (GATED) {
+        if (in && d.dgate != nullptr) store_row<P>(d.dgate, row, width, p, kLanes, dg);
+      } else if (row_gate) {
         float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) t += dg[i];
+        for (int i = 0; i < P::V; ++i) t += dg[i];
         t = sum.one(t);
         if (in && p == 0 && d.dgate != nullptr) static_cast<T *>(d.dgate)[row] = from_f32<T>(t);
       }
       if (d.post) {
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) {
+        for (int i = 0; i < P::V; ++i) {
           acc[1][i] = fmaf(g[i], n[i], acc[1][i]);
-          acc[2][i] += g[i];
+          if (BIASES) acc[2][i] += g[i];
           g[i] *= w2[i];
         }
         back_through_norm(g, n, r2, a, sum);
       }
-      if (in && d.df != nullptr) store_row<T, VEC>(d.df, row, width, p, kLanes, g);
+      if (in && d.df != nullptr) store_row<P>(d.df, row, width, p, kLanes, g);
     }
   }
   // the block's sums: lanes of a warp that hold the same columns, then the warps in order
   float *part = a.part + static_cast<int64_t>(blockIdx.x) * kSums * width;
   if constexpr (WARPS == 1) {
-    __shared__ float side[kBlock / 32][LANES * kValues];
+    __shared__ float side[kBlock / 32][LANES * P::V];
     const int warp = threadIdx.x >> 5;
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
+      if (!BIASES && (k == 2 || k == 4)) {
+        for (int c = threadIdx.x; c < width; c += kBlock) part[k * width + c] = 0.f;
+        continue;
+      }
 #pragma unroll
-      for (int i = 0; i < kValues; ++i)
+      for (int i = 0; i < P::V; ++i)
 #pragma unroll
         for (int o = LANES; o < 32; o <<= 1) acc[k][i] += __shfl_xor_sync(0xffffffffu, acc[k][i], o);
       if ((threadIdx.x & 31) < LANES) {
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) side[warp][((i / P::N) * kLanes + p) * P::N + i % P::N] = acc[k][i];
+        for (int i = 0; i < P::V; ++i) side[warp][((i / P::N) * kLanes + p) * P::N + i % P::N] = acc[k][i];
       }
       __syncthreads();
       for (int c = threadIdx.x; c < width; c += kBlock) {
@@ -430,63 +491,81 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, WARPS > 1 ? k
 #pragma unroll
     for (int k = 0; k < kSums; ++k)
 #pragma unroll
-      for (int i = 0; i < kValues; ++i) {
+      for (int i = 0; i < P::V; ++i) {
         const int c = ((i / P::N) * kLanes + p) * P::N + i % P::N;
         if (c < width) part[k * width + c] = acc[k][i];
       }
   }
 }
 
-// Lanes of a row: the smallest power of two, from 8 on, that holds it.
-int lanes_of(int width) {
+// Lanes of a row: the smallest power of two, from 8 on, that holds it (16 bytes a lane; 32 where 16 warps are not enough).
+int values_of(int dtype) { return dtype == CXG_F32 ? 4 : 8; }
+int lanes_of(int width, int dtype) {
   int lanes = 8;
-  while (lanes * kValues < width) lanes *= 2;
+  while (lanes < 32 * kMostWarps && lanes * values_of(dtype) < width) lanes *= 2;
   return lanes;
 }
-int rows_per_block(int width) { return lanes_of(width) > 32 ? 1 : kBlock / lanes_of(width); }
-int backward_blocks(int64_t n, int width) {
-  const int lanes = lanes_of(width), per_sm = lanes > 32 ? kMostWarps * 32 / lanes : 2;
-  const int64_t want = (n + rows_per_block(width) - 1) / rows_per_block(width);
-  return static_cast<int>(want < 1 ? 1 : want < kNumSM * per_sm ? want : kNumSM * per_sm);
+int rows_per_block(int lanes) { return lanes > 32 ? 1 : kBlock / lanes; }
+int backward_blocks(int64_t n, int lanes) {
+  const int64_t most = kNumSM * blocks_of(16, lanes > 32 ? lanes : kBlock);
+  const int64_t want = (n + rows_per_block(lanes) - 1) / rows_per_block(lanes);
+  return static_cast<int>(want < 1 ? 1 : want < most ? want : most);
 }
 
-template <typename T, bool VEC, typename Go>
-cudaError_t by_width(int width, Go go) {
-  switch (lanes_of(width)) {
-    case 8: return go.template run<T, 8, 1, VEC>();
-    case 16: return go.template run<T, 16, 1, VEC>();
-    case 32: return go.template run<T, 32, 1, VEC>();
-    case 64: return go.template run<T, 32, 2, VEC>();
-    case 128: return go.template run<T, 32, 4, VEC>();
-    case 256: return go.template run<T, 32, 8, VEC>();
-    default: return go.template run<T, 32, 16, VEC>();
+template <typename T, bool VEC, bool GATED, typename Go>
+cudaError_t by_width(int width, int dtype, Go go) {
+  switch (lanes_of(width, dtype)) {
+    case 8: return go.template run<T, 8, 1, VEC, 1, GATED>();
+    case 16: return go.template run<T, 16, 1, VEC, 1, GATED>();
+    case 32: return go.template run<T, 32, 1, VEC, 1, GATED>();
+    case 64: return go.template run<T, 32, 2, VEC, 1, GATED>();
+    case 128: return go.template run<T, 32, 4, VEC, 1, GATED>();
+    case 256: return go.template run<T, 32, 8, VEC, 1, GATED>();
+    default: break;
   }
+  if constexpr (sizeof(T) == 4)
+    if (width > 32 * kMostWarps * 4) return go.template run<T, 32, kMostWarps, VEC, 2, GATED>();
+  return go.template run<T, 32, kMostWarps, VEC, 1, GATED>();
+}
+template <typename T, typename Go>
+cudaError_t by_kind(const cxg_residual_desc &d, bool vec, Go go) {
+  const bool gated = d.gate_mode == CXG_GATE_VALUE;
+  if (vec) return gated ? by_width<T, true, true>(d.width, d.dtype, go) : by_width<T, true, false>(d.width, d.dtype, go);
+  return gated ? by_width<T, false, true>(d.width, d.dtype, go) : by_width<T, false, false>(d.width, d.dtype, go);
 }
 template <typename Go>
 cudaError_t by_type(const cxg_residual_desc &d, bool vec, Go go) {
-  if (d.dtype == CXG_F32) return vec ? by_width<float, true>(d.width, go) : by_width<float, false>(d.width, go);
-  return vec ? by_width<__nv_bfloat16, true>(d.width, go) : by_width<__nv_bfloat16, false>(d.width, go);
+  return d.dtype == CXG_F32 ? by_kind<float>(d, vec, go) : by_kind<__nv_bfloat16>(d, vec, go);
 }
 
 struct Forward {
   const ResArgs &a;
   cudaStream_t st;
-  template <typename T, int LANES, int WARPS, bool VEC>
+  template <typename T, int LANES, int WARPS, bool VEC, int VECTORS, bool GATED>
   cudaError_t run() const {
-    const int per = rows_per_block(a.d.width);
-    const int64_t want = (a.d.n + a.keep + per - 1) / per, most = static_cast<int64_t>(kNumSM) * (WARPS > 1 ? 64 / WARPS : 8);
-    return launch_dependent(residual_forward<T, LANES, WARPS, VEC>, static_cast<unsigned>(want < most ? want : most),
-                            WARPS > 1 ? 32 * WARPS : kBlock, 0, st, a);
+    const int per = rows_per_block(LANES * WARPS);
+    constexpr int kThreads = WARPS > 1 ? 32 * WARPS : kBlock;
+    const int64_t want = (a.d.n + a.keep + per - 1) / per, most = kNumSM * blocks_of(forward_warps(Place<T, VEC, VECTORS>::V, GATED), kThreads);
+    return launch_dependent(residual_forward<T, LANES, WARPS, VEC, VECTORS, GATED>, static_cast<unsigned>(want < most ? want : most),
+                            kThreads, 0, st, a);
   }
 };
 struct Backward {
   const ResArgs &a;
   cudaStream_t st;
-  int blocks;
-  template <typename T, int LANES, int WARPS, bool VEC>
-  cudaError_t run() const {
-    return launch_dependent(residual_backward<T, LANES, WARPS, VEC>, static_cast<unsigned>(blocks), WARPS > 1 ? 32 * WARPS : kBlock, 0,
+  int *blocks;
+  template <typename T, int LANES, int WARPS, bool VEC, int VECTORS, bool GATED, bool BIASES>
+  cudaError_t go() const {
+    constexpr int kThreads = WARPS > 1 ? 32 * WARPS : kBlock;
+    const int most = kNumSM * blocks_of(backward_warps(Place<T, VEC, VECTORS>::V, BIASES), kThreads);
+    if (*blocks > most) *blocks = most;
+    return launch_dependent(residual_backward<T, LANES, WARPS, VEC, VECTORS, GATED, BIASES>, static_cast<unsigned>(*blocks), kThreads, 0,
                             st, a);
+  }
+  template <typename T, int LANES, int WARPS, bool VEC, int VECTORS, bool GATED>
+  cudaError_t run() const {
+    return a.d.post_bias != nullptr || a.d.next_bias != nullptr ? go<T, LANES, WARPS, VEC, VECTORS, GATED, true>()
+                                                                : go<T, LANES, WARPS, VEC, VECTORS, GATED, false>();
   }
 };
 
@@ -541,11 +620,12 @@ extern "C" int cxg_residual_norm_forward(const cxg_residual_desc *d, void *strea
   return check_launch("cxg_residual_norm_forward");
 }
 
-extern "C" int cxg_residual_norm_backward_workspace_size(int64_t n, int width, size_t *bytes) {
+extern "C" int cxg_residual_norm_backward_workspace_size(int64_t n, int width, int dtype, size_t *bytes) {
   CXG_REQUIRE(bytes != nullptr, CXG_ENULL, "cxg_residual_norm_backward_workspace_size: bytes is NULL");
-  CXG_REQUIRE(n >= 0 && width > 0, CXG_EINVAL, "cxg_residual_norm_backward_workspace_size: bad sizes");
+  CXG_REQUIRE(n >= 0 && width > 0 && (dtype == CXG_F32 || dtype == CXG_BF16), CXG_EINVAL,
+              "cxg_residual_norm_backward_workspace_size: bad sizes or type");
   CXG_REQUIRE(width <= kMostWidth, CXG_EUNSUPPORTED, "cxg_residual_norm: rows of %d values, at most %d", width, kMostWidth);
-  *bytes = static_cast<size_t>(backward_blocks(n, width)) * kSums * width * sizeof(float);
+  *bytes = static_cast<size_t>(backward_blocks(n, lanes_of(width, dtype))) * kSums * width * sizeof(float);
   return CXG_OK;
 }
 
@@ -560,15 +640,15 @@ extern "C" int cxg_residual_norm_backward(const cxg_residual_desc *d, float *sum
     return CXG_OK;
   }
   size_t need = 0;
-  cxg_residual_norm_backward_workspace_size(d->n, d->width, &need);
+  cxg_residual_norm_backward_workspace_size(d->n, d->width, d->dtype, &need);
   CXG_REQUIRE(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, CXG_EWORKSPACE,
               "cxg_residual_norm_backward: workspace %zu bytes, need %zu", workspace_bytes, need);
   ResArgs a = {};
   a.d = *d;
   a.inv_width = 1.f / static_cast<float>(d->width);
   a.part = static_cast<float *>(workspace);
-  const int blocks = backward_blocks(d->n, d->width);
-  const cudaError_t e = by_type(*d, whole_vectors(*d), Backward{a, st, blocks});
+  int blocks = backward_blocks(d->n, lanes_of(d->width, d->dtype));
+  const cudaError_t e = by_type(*d, whole_vectors(*d), Backward{a, st, &blocks});
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_residual_norm_backward: %s", cudaGetErrorString(e));
   column_sum_join(a.part, sums, blocks, kSums * d->width, st);
   count_launches(2);

@@ -1,10 +1,11 @@
 // Writing and reading rows in 8 bits (rows8.cuh has the format): activations that a backward pass needs again, and caches of
 // features or of hidden states that are written and read by node id.
 //
-// Both directions are bound by memory. A lane takes the 16 bytes of one access on the side of the wide type: 4 fp32 or 8 bf16
-// values, so 8 or 4 lanes share a group of 32 and find its largest value in 3 or 2 shuffles. Lanes go along rows without
-// regard to where these end (the row of an item comes from a multiplication), so that no lane of a warp is idle for a width
-// that is no power of two, and every lane has several items in flight.
+// Both directions are bound by memory as long as they spend few instructions: a lane takes 8 values, so four lanes share a
+// group of 32 and find its largest value in two shuffles, and what an item costs by itself (its row and place, the row's
+// target, the address) is spread over these. Lanes go along rows without regard to where these end, so that none is idle for
+// a width that is no power of two; items are counted in 32 bits, larger matrices go in pieces. (4 fp32 values a lane, 64-bit
+// counts and a limit on every code were 140 instructions an item and twice the time of memory: 400,000 rows of 100 fp32 38 us.)
 #include "rows8.cuh"
 
 namespace cxg {
@@ -13,75 +14,126 @@ namespace {
 using namespace rows8;
 
 constexpr int kThreads = 256;
+constexpr int kValues = 8;                   // per item
+constexpr int kLanes = kGroup / kValues;     // of a group
+constexpr int kItems = 4;                    // per thread
+constexpr uint32_t kMostItems = 1u << 31;    // per launch
 
-template <typename T>
-struct Pack {
-  static constexpr int kN = 16 / static_cast<int>(sizeof(T));  // values per lane
-  static constexpr int kLanes = kGroup / kN;                   // lanes per group
+// Items of rows that have `per` each. The quotient by floor(2^32 / per) is at most one too small.
+struct Items {
+  uint32_t total, per, inverse;
+  __device__ __forceinline__ void place(uint32_t i, uint32_t *row, uint32_t *chunk) const {
+    uint32_t q = per > 1 ? __umulhi(i, inverse) : i, r = i - q * per;
+    if (r >= per) ++q, r -= per;
+    *row = q, *chunk = r;
+  }
 };
 
-// Up to kN values of a row from column c on; zeros behind the row.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_values(float *f, const T *row, int c, int width) {
-  constexpr int N = Pack<T>::kN;
-#pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = 0.f;
-  if (VEC) {
-    if (c < width) Vec<T>::to_float(f, Vec<T>::load(row + c));  // width is a multiple of N
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (c + i < width) f[i] = to_f32(__ldg(row + c + i));
-  }
+// How the wide side is accessed: value by value, in 16-byte vectors, in 32-byte ones.
+enum Access { kScalar, kVector, kWide };
+
+__device__ __forceinline__ void load32(float (&f)[8], const float *p) {
+  asm("ld.global.nc.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7])
+      : "l"(p));
+}
+__device__ __forceinline__ void store32(float *p, const float (&f)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]),
+               "f"(f[5]), "f"(f[6]), "f"(f[7])
+               : "memory");
 }
 
-// Rows [0, n) of x to the rows `to` names (itself without it; negative: nowhere); rows [n, n_end) are written as zeros.
-// owner: the row's entry is given back (write_at).
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) rows8_write(const T *x, int64_t ld, int64_t n, int64_t n_end, int width, Rows rows,
-                                                        uint8_t *codes, uint8_t *scales, const int64_t *to, int32_t *owner) {
-  constexpr int N = Pack<T>::kN, L = Pack<T>::kLanes;
-  constexpr int kItems = 4;
-  dependency_wait();
-  const int groups = static_cast<int>(rows.per) / L;
-  const uint64_t total = static_cast<uint64_t>(n_end) * rows.per;
-  const uint64_t step = static_cast<uint64_t>(gridDim.x) * kThreads;
-  for (uint64_t i0 = blockIdx.x * static_cast<uint64_t>(kThreads) + (threadIdx.x & ~31u); i0 < total; i0 += kItems * step) {
-    float f[kItems][N];
-    int64_t row[kItems], dst[kItems];
-    int chunk[kItems];
+// The larger of two absolute values, NaN where either is.
+__device__ __forceinline__ float top_of(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
+// 8 values of a row from column c on as they were loaded; zeros behind the row.
+template <typename T, Access A>
+struct Loaded {
+  float f[sizeof(T) == 4 ? 8 : 1];
+  uint32_t h[sizeof(T) == 4 ? 1 : 4];
+  __device__ __forceinline__ void load(const T *row, uint32_t c, uint32_t width, bool in) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const uint64_t i = i0 + k * step + (threadIdx.x & 31);
-      row[k] = i < total ? rows.row(i) : n_end;
-      chunk[k] = static_cast<int>(i - static_cast<uint64_t>(row[k]) * rows.per);
-      dst[k] = row[k] < n_end ? row[k] : -1;
-      if (to != nullptr && row[k] < n) dst[k] = __ldg(to + row[k]);
+      for (int i = 0; i < 8; ++i) f[i] = 0.f;
+      if (!in) return;
+      if constexpr (A == kWide) {
+        if (c < width) load32(f, row + c);
+      } else if constexpr (A == kVector) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4)
+          if (c + i < width) {
+            const float4 t = __ldg(reinterpret_cast<const float4 *>(row + c + i));
+            f[i] = t.x, f[i + 1] = t.y, f[i + 2] = t.z, f[i + 3] = t.w;
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i < width) f[i] = __ldg(row + c + i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = 0;
+      if (!in) return;
+      if constexpr (A != kScalar) {
+        if (c < width) {
+          const uint4 t = __ldg(reinterpret_cast<const uint4 *>(row + c));
+          h[0] = t.x, h[1] = t.y, h[2] = t.z, h[3] = t.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i < width) h[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(row) + c + i)) << (16 * (i & 1));
+      }
     }
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll
-    for (int k = 0; k < kItems; ++k)
-      load_values<T, VEC>(f[k], x + (row[k] < n ? row[k] : 0) * ld, row[k] < n ? chunk[k] * N : width, width);
-#pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < N; ++j) top = max(top, __float_as_uint(f[k][j]) & 0x7fffffffu);
-#pragma unroll
-      for (int d = 1; d < L; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const uint32_t e = scale_byte(top);
-      const float inv = e == kNotFinite ? 0.f : inverse_scale(e);
-      uint32_t w[N / 4];
-#pragma unroll
-      for (int j = 0; j < N / 4; ++j)
-        w[j] = e == kNotFinite ? 0u : pack_codes(code_bits(f[k][4 * j], inv), code_bits(f[k][4 * j + 1], inv),
-                                                 code_bits(f[k][4 * j + 2], inv), code_bits(f[k][4 * j + 3], inv));
-      if (dst[k] < 0) continue;
-      uint8_t *out = codes + dst[k] * (static_cast<int64_t>(groups) * kGroup) + chunk[k] * N;
-      if constexpr (N == 4)
-        *reinterpret_cast<uint32_t *>(out) = w[0];
+    for (int i = 0; i < 8; ++i)
+      if constexpr (sizeof(T) == 4)
+        v[i] = f[i];
       else
-        *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[N / 4 - 1]);
-      if (chunk[k] % L == 0) scales[dst[k] * groups + chunk[k] / L] = static_cast<uint8_t>(e);
+        v[i] = __uint_as_float(i & 1 ? h[i / 2] & 0xffff0000u : h[i / 2] << 16);
+  }
+};
+
+// Rows [0, n) of x to the rows `to` names (itself without it; negative: nowhere); rows from n on are written as zeros.
+// owner: the row's entry is given back (write_at).
+template <typename T, Access A>
+__global__ void __launch_bounds__(kThreads) rows8_write(const T *x, int64_t ld, uint32_t n, uint32_t width, Items items, uint8_t *codes,
+                                                        uint8_t *scales, const int64_t *to, int32_t *owner) {
+  dependency_wait();
+  const uint32_t groups = items.per / kLanes, first = blockIdx.x * (kThreads * kItems) + threadIdx.x;
+  Loaded<T, A> in[kItems];
+  int64_t dst[kItems];
+  uint32_t chunk[kItems];
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const uint32_t i = first + k * kThreads;
+    uint32_t row;
+    items.place(i, &row, &chunk[k]);
+    const bool have = i < items.total, of_x = have && row < n;
+    dst[k] = have ? static_cast<int64_t>(row) : int64_t{-1};
+    if (to != nullptr && of_x) dst[k] = __ldg(to + row);
+    in[k].load(x + (of_x ? row : 0) * ld, chunk[k] * kValues, width, of_x);
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    float v[8];
+    in[k].get(v);
+    float top = top_of(top_of(top_of(v[0], v[1]), top_of(v[2], v[3])), top_of(top_of(v[4], v[5]), top_of(v[6], v[7])));
+#pragma unroll
+    for (int d = 1; d < kLanes; d <<= 1) top = top_of(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const uint32_t e = scale_byte(__float_as_uint(top));
+    uint32_t w[2];
+    codes_of<8>(w, v, e);
+    if (dst[k] >= 0) {
+      const int64_t group = dst[k] * groups + (chunk[k] / kLanes);
+      *reinterpret_cast<uint2 *>(codes + group * kGroup + (chunk[k] % kLanes) * kValues) = make_uint2(w[0], w[1]);
+      if (chunk[k] % kLanes == 0) scales[group] = static_cast<uint8_t>(e);
       if (owner != nullptr && chunk[k] == 0) owner[dst[k]] = -1;
     }
   }
@@ -106,92 +158,106 @@ __global__ void __launch_bounds__(kThreads) rows8_settle(const int64_t *index, i
 }
 
 // out[i] = the values of row index[i] (of row i without an index; ids outside the rows read as zeros).
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) rows8_read(const uint8_t *codes, const uint8_t *scales, int64_t n_rows, int width,
-                                                       int groups, const int64_t *index, int64_t n, Rows rows, T *out, int64_t ld) {
-  constexpr int N = Pack<T>::kN, L = Pack<T>::kLanes;
-  constexpr int kItems = 4;
+template <typename T, Access A>
+__global__ void __launch_bounds__(kThreads) rows8_read(const uint8_t *codes, const uint8_t *scales, int64_t n_rows, uint32_t width,
+                                                       uint32_t groups, const int64_t *index, Items items, T *out, int64_t ld) {
   dependency_wait();
-  const uint64_t total = static_cast<uint64_t>(n) * rows.per;
-  const uint64_t step = static_cast<uint64_t>(gridDim.x) * kThreads;
-  for (uint64_t i0 = blockIdx.x * static_cast<uint64_t>(kThreads) + threadIdx.x; i0 < total; i0 += kItems * step) {
-    int64_t row[kItems], src[kItems];
-    int chunk[kItems];
+  const uint32_t first = blockIdx.x * (kThreads * kItems) + threadIdx.x;
+  int64_t src[kItems];
+  uint32_t row[kItems], chunk[kItems];
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const uint64_t i = i0 + k * step;
-      row[k] = i < total ? rows.row(i) : -1;
-      chunk[k] = row[k] < 0 ? 0 : static_cast<int>(i - static_cast<uint64_t>(row[k]) * rows.per);
-      src[k] = row[k] < 0 ? n_rows : index != nullptr ? __ldg(index + row[k]) : row[k];
-      if (static_cast<uint64_t>(src[k]) > static_cast<uint64_t>(n_rows)) src[k] = n_rows;  // the row of zeros
+  for (int k = 0; k < kItems; ++k) {
+    const uint32_t i = first + k * kThreads;
+    items.place(i, &row[k], &chunk[k]);
+    src[k] = n_rows;  // the row of zeros
+    if (i < items.total) {
+      const int64_t r = index != nullptr ? __ldg(index + row[k]) : static_cast<int64_t>(row[k]);
+      if (static_cast<uint64_t>(r) < static_cast<uint64_t>(n_rows)) src[k] = r;
     }
-    uint32_t w[kItems][N / 4], e[kItems];
+  }
+  uint2 w[kItems];
+  uint32_t e[kItems];
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const uint8_t *p = codes + src[k] * (static_cast<int64_t>(groups) * kGroup) + chunk[k] * N;
-      if constexpr (N == 4) {
-        w[k][0] = __ldg(reinterpret_cast<const uint32_t *>(p));
-      } else {
-        const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p));
-        w[k][0] = t.x, w[k][N / 4 - 1] = t.y;
-      }
-      e[k] = __ldg(scales + src[k] * groups + chunk[k] / L);
-    }
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t group = src[k] * groups + (chunk[k] / kLanes);
+    w[k] = __ldg(reinterpret_cast<const uint2 *>(codes + group * kGroup + (chunk[k] % kLanes) * kValues));
+    e[k] = __ldg(scales + group);
+  }
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      if (row[k] < 0) continue;
-      const float s = scale_of(e[k]);
-      float f[N];
+  for (int k = 0; k < kItems; ++k) {
+    if (first + k * kThreads >= items.total) break;
+    const float s = scale_of(e[k]);
+    float f[8];
+    code_values(f, w[k].x);
+    code_values(f + 4, w[k].y);
 #pragma unroll
-      for (int j = 0; j < N / 4; ++j) code_values(f + 4 * j, w[k][j]);
+    for (int j = 0; j < 8; ++j) f[j] *= s;
+    const uint32_t c = chunk[k] * kValues;
+    T *o = out + row[k] * ld + c;
+    if constexpr (A == kWide && sizeof(T) == 4) {
+      store32(o, f);
+    } else if constexpr (A != kScalar) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) f[j] *= s;
-      T *o = out + row[k] * ld + chunk[k] * N;
-      const int left = width - chunk[k] * N;
-      if (VEC) {
-        if (left > 0) Vec<T>::store_stream(o, Vec<T>::from_float(f));
-      } else {
+      for (int j = 0; j < 8; j += Vec<T>::kElems)
+        if (c + j < width) Vec<T>::store_stream(o + j, Vec<T>::from_float(f + j));
+    } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (j < left) o[j] = from_f32<T>(f[j]);
-      }
+      for (int j = 0; j < 8; ++j)
+        if (c + j < width) o[j] = from_f32<T>(f[j]);
     }
   }
 }
 
-unsigned grid_of(uint64_t items, int per_thread) {
-  const uint64_t want = (items + kThreads * per_thread - 1) / (kThreads * per_thread);
-  const uint64_t most = static_cast<uint64_t>(kNumSM) * 8;
-  return static_cast<unsigned>(want < 1 ? 1 : want < most ? want : most);
+template <typename T>
+Access access_of(const void *p, int64_t ld, int width) {
+  const uint64_t bits = reinterpret_cast<uintptr_t>(p) | (static_cast<uint64_t>(ld) * sizeof(T)) | (static_cast<uint64_t>(width) * sizeof(T));
+  return bits % 32 == 0 ? kWide : bits % 16 == 0 ? kVector : kScalar;
+}
+
+// go(first row, rows, items, blocks) for pieces of n rows with `per` items each.
+template <typename Go>
+void in_pieces(int64_t n, uint32_t per, Go go) {
+  const int64_t most = kMostItems / per;
+  for (int64_t r = 0; r < n; r += most) {
+    const int64_t rows = n - r < most ? n - r : most;
+    const Items items{static_cast<uint32_t>(rows * per), per, static_cast<uint32_t>((1ull << 32) / per)};
+    go(r, rows, items, (items.total + kThreads * kItems - 1) / (kThreads * kItems));
+    count_launches(1);
+  }
 }
 
 template <typename T>
-bool whole_vectors(const void *p, int64_t ld, int width) {
-  return (reinterpret_cast<uintptr_t>(p) | (static_cast<uint64_t>(ld) * sizeof(T)) | (static_cast<uint64_t>(width) * sizeof(T))) % 16 == 0;
-}
-
-template <typename T>
-void launch_write(const void *x, int64_t ld, int64_t n, int64_t n_end, int width, void *codes, void *scales, const int64_t *to,
+void launch_write(const void *x_, int64_t ld, int64_t n, int64_t n_end, int width, void *codes, void *scales, const int64_t *to,
                   int32_t *owner, cudaStream_t st) {
-  const Rows rows(static_cast<uint32_t>(groups_of(width) * Pack<T>::kLanes));
-  const unsigned grid = grid_of(static_cast<uint64_t>(n_end) * rows.per, 4);
-  auto go = [&](auto kernel) {
-    launch_dependent(kernel, grid, kThreads, 0, st, static_cast<const T *>(x), ld, n, n_end, width, rows,
-                     static_cast<uint8_t *>(codes), static_cast<uint8_t *>(scales), to, owner);
-  };
-  whole_vectors<T>(x, ld, width) ? go(rows8_write<T, true>) : go(rows8_write<T, false>);
+  const int groups = groups_of(width);
+  const T *x = static_cast<const T *>(x_);
+  in_pieces(n_end, static_cast<uint32_t>(groups * kLanes), [&](int64_t r, int64_t rows, const Items &items, unsigned blocks) {
+    const int64_t have = n - r < rows ? n - r : rows, at = to != nullptr ? 0 : r;
+    auto go = [&](auto kernel) {
+      launch_dependent(kernel, blocks, kThreads, 0, st, x + (have > 0 ? r * ld : 0), ld, static_cast<uint32_t>(have > 0 ? have : 0),
+                       static_cast<uint32_t>(width), items, static_cast<uint8_t *>(codes) + at * groups * kGroup,
+                       static_cast<uint8_t *>(scales) + at * groups, to != nullptr ? to + r : nullptr, owner);
+    };
+    const Access a = access_of<T>(x + (have > 0 ? r * ld : 0), ld, width);
+    a == kWide ? go(rows8_write<T, kWide>) : a == kVector ? go(rows8_write<T, kVector>) : go(rows8_write<T, kScalar>);
+  });
 }
 
 template <typename T>
-void launch_read(const void *codes, const void *scales, int64_t n_rows, int width, const int64_t *index, int64_t n, void *out,
+void launch_read(const void *codes, const void *scales, int64_t n_rows, int width, const int64_t *index, int64_t n, void *out_,
                  int64_t ld, cudaStream_t st) {
-  const Rows rows(static_cast<uint32_t>((width + Pack<T>::kN - 1) / Pack<T>::kN));
-  const unsigned grid = grid_of(static_cast<uint64_t>(n) * rows.per, 4);
-  auto go = [&](auto kernel) {
-    launch_dependent(kernel, grid, kThreads, 0, st, static_cast<const uint8_t *>(codes), static_cast<const uint8_t *>(scales),
-                     n_rows, width, groups_of(width), index, n, rows, static_cast<T *>(out), ld);
-  };
-  whole_vectors<T>(out, ld, width) ? go(rows8_read<T, true>) : go(rows8_read<T, false>);
+  const int groups = groups_of(width);
+  T *out = static_cast<T *>(out_);
+  in_pieces(n, static_cast<uint32_t>((width + kValues - 1) / kValues), [&](int64_t r, int64_t rows, const Items &items, unsigned blocks) {
+    const int64_t at = index != nullptr ? 0 : r;
+    auto go = [&](auto kernel) {
+      launch_dependent(kernel, blocks, kThreads, 0, st, static_cast<const uint8_t *>(codes) + at * groups * kGroup,
+                       static_cast<const uint8_t *>(scales) + at * groups, n_rows - at, static_cast<uint32_t>(width),
+                       static_cast<uint32_t>(groups), index != nullptr ? index + r : nullptr, items, out + r * ld, ld);
+    };
+    const Access a = access_of<T>(out + r * ld, ld, width);
+    a == kWide ? go(rows8_read<T, kWide>) : a == kVector ? go(rows8_read<T, kVector>) : go(rows8_read<T, kScalar>);
+  });
 }
 
 // What every entry point asks of a matrix of `width` columns.
@@ -217,7 +283,6 @@ extern "C" int cxg_rows8_write(const void *x, int dtype, int64_t ld, int64_t n, 
     launch_write<float>(x, ld, n, n_end, width, codes, scales, nullptr, nullptr, as_stream(stream));
   else
     launch_write<__nv_bfloat16>(x, ld, n, n_end, width, codes, scales, nullptr, nullptr, as_stream(stream));
-  count_launches(1);
   return check_launch("cxg_rows8_write");
 }
 
@@ -247,7 +312,7 @@ extern "C" int cxg_rows8_write_at(const void *x, int dtype, int64_t ld, int64_t 
     launch_write<float>(x, ld, n, n, width, codes, scales, to, owner, st);
   else
     launch_write<__nv_bfloat16>(x, ld, n, n, width, codes, scales, to, owner, st);
-  count_launches(3);
+  count_launches(2);
   return check_launch("cxg_rows8_write_at");
 }
 
@@ -263,6 +328,5 @@ extern "C" int cxg_rows8_read(const void *codes, const void *scales, int64_t row
     launch_read<float>(codes, scales, rows, width, index, n, out, ld, as_stream(stream));
   else
     launch_read<__nv_bfloat16>(codes, scales, rows, width, index, n, out, ld, as_stream(stream));
-  count_launches(1);
   return check_launch("cxg_rows8_read");
 }

@@ -32,14 +32,32 @@ __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_floa
 // x / s of finite groups: the product with 2^(254 - e - 127) is exact, or so small that it rounds to zero either way
 __device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
-// The code as the low byte of the result: adding 1.5 * 2^23 rounds to whole numbers, ties to even, and leaves their two's
-// complement in the low bits. The limit matters at the top of the range of fp32 alone, where e is kept at 248.
-__device__ __forceinline__ uint32_t code_bits(float x, float inv) {
-  return __float_as_uint(fminf(fmaxf(x * inv, -127.f), 127.f) + 12582912.f);
-}
+// The code as the low byte of the result: adding 1.5 * 2^23 to x / s (exact in front of the addition) rounds to whole numbers,
+// ties to even, and leaves their two's complement in the low bits.
+__device__ __forceinline__ uint32_t code_bits(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f)); }
 
 __device__ __forceinline__ uint32_t pack_codes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// The codes of N values of a group, four to a word. At the top of the range of fp32, where e is kept at 248, a code is limited.
+template <int N>
+__device__ __forceinline__ void codes_of(uint32_t (&w)[N / 4], const float (&v)[N], uint32_t e) {
+  const float inv = inverse_scale(e);
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) {
+    const float *f = v + 4 * j;
+    w[j] = pack_codes(code_bits(f[0], inv), code_bits(f[1], inv), code_bits(f[2], inv), code_bits(f[3], inv));
+  }
+  if (e >= 248) {
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+      uint32_t c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = code_bits(fminf(fmaxf(v[4 * j + i] * inverse_scale(248), -127.f), 127.f), 1.f);
+      w[j] = e == kNotFinite ? 0u : pack_codes(c[0], c[1], c[2], c[3]);
+    }
+  }
 }
 
 // Code i of a word as fp32: the code with its sign bit flipped is code + 128; as the low byte of 2^23 it is 2^23 + 128 + code.
@@ -51,14 +69,6 @@ __device__ __forceinline__ void code_values(float *f, uint32_t word) {
   const uint32_t w = word ^ 0x80808080u;
   f[0] = code_value<0>(w), f[1] = code_value<1>(w), f[2] = code_value<2>(w), f[3] = code_value<3>(w);
 }
-
-// Row of item i where every row has `per` items: i / per by a multiplication with ceil(2^64 / per), exact for i * per < 2^64.
-struct Rows {
-  uint64_t magic;
-  uint32_t per;
-  __host__ __device__ explicit Rows(uint32_t p = 1) : magic(p > 1 ? ~0ull / p + 1 : 0), per(p) {}
-  __device__ __forceinline__ int64_t row(uint64_t i) const { return static_cast<int64_t>(magic ? __umul64hi(i, magic) : i); }
-};
 
 }  // namespace rows8
 }  // namespace cxg

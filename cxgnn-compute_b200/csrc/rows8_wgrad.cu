@@ -26,8 +26,12 @@ using rows8::kGroup;
 constexpr int kPos = 64;           // rows per stage
 constexpr int kSpan = kPos * 128;  // bytes of a span: 64 columns of bf16, one row behind the other
 constexpr int kProdWarps = 8, kEpiWarps = 8;
-constexpr int kMmaWarp = kEpiWarps, kFirstProd = kMmaWarp + 1;
-constexpr int kThreads = 32 * (kEpiWarps + 1 + kProdWarps);
+constexpr int kMmaWarp = kEpiWarps, kFirstProd = kMmaWarp + 4;  // roles in whole groups of four warps, which share out registers
+constexpr int kThreads = 32 * (kFirstProd + kProdWarps);
+// Registers per thread: 96 at the launch (640 threads take 61,440); the producers, which hold two stages of loads, take 32 more
+// each from the group of the issuing warp and what is left over: 256 * 96 + 128 * 32 + 256 * 128 = 61,440. (With 96 for all,
+// loads of the second stage were spilled, which waits for each: 1077 us for 2.4 M rows of 100 x 128.)
+constexpr int kIssuerRegs = 32, kProducerRegs = 128;
 constexpr int kMaxStages = 4;
 constexpr int kSmemBudget = 220 * 1024;
 
@@ -71,26 +75,31 @@ __device__ __forceinline__ uint32_t two_values(uint32_t word, __nv_bfloat162 sca
 // hi, mid and lo of 8 fp32 values, as 8 bf16 each. Cutting instead of rounding keeps the sum exact (8 bits each). Infinities and
 // NaN go into hi alone (what is left of them would be NaN).
 __device__ __forceinline__ void three_parts(const float (&v)[8], uint32_t (&hi)[4], uint32_t (&mid)[4], uint32_t (&lo)[4]) {
-  uint32_t top = 0;
+  uint32_t h[8];
+  float r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  const bool finite = top < 0x7f800000u;
+  for (int i = 0; i < 8; ++i) {
+    h[i] = __float_as_uint(v[i]) & 0xffff0000u;
+    r[i] = v[i] - __uint_as_float(h[i]);
+  }
+  // a rest that is NaN: a value that is not finite (the rests themselves are far too small to add up to an infinity)
+  const float any = ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
+  if (any != any) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if ((h[i] & 0x7f800000u) == 0x7f800000u) r[i] = 0.f;
+      if (v[i] != v[i]) h[i] = 0x7fc00000u;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t h[2], m[2], l[2];
+    uint32_t m[2], l[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float f = v[2 * i + j];
-      h[j] = __float_as_uint(f) & 0xffff0000u;
-      float r = f - __uint_as_float(h[j]);
-      if (!finite) {
-        if ((h[j] & 0x7f800000u) == 0x7f800000u) r = 0.f;
-        if (f != f) h[j] = 0x7fc00000u;
-      }
-      m[j] = __float_as_uint(r) & 0xffff0000u;
-      l[j] = __float_as_uint(r - __uint_as_float(m[j]));
+      m[j] = __float_as_uint(r[2 * i + j]) & 0xffff0000u;
+      l[j] = __float_as_uint(r[2 * i + j] - __uint_as_float(m[j]));
     }
-    hi[i] = __byte_perm(h[0], h[1], 0x7632);
+    hi[i] = __byte_perm(h[2 * i], h[2 * i + 1], 0x7632);
     mid[i] = __byte_perm(m[0], m[1], 0x7632);
     lo[i] = __byte_perm(l[0], l[1], 0x7632);
   }
@@ -140,6 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
 
   if (warp >= kFirstProd) {
     // ================= producers =================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
     constexpr int kThr = 32 * kProdWarps;
     constexpr int kXUnits = kPos * 8 / kThr;                // 16 codes each
     constexpr int kUnitsPerRow = 8 * SPANS;                 // of dy: 8 values each
@@ -266,7 +276,9 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
         a.partial_db[static_cast<int64_t>(blockIdx.x) * a.n + g_at + pt] = t;
       }
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssuerRegs));
+    if (warp == kMmaWarp) {
     // ================= MMA issuer: the whole warp walks the tiles, one lane issues =================
     auto wait_all = [&](uint64_t *bar, uint32_t parity) {
       return __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, a.status, a.wait_cycles)) != 0;
@@ -311,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
       while (clock64() - t0 < 200000) {
       }
     }
+    }
   } else {
     // ================= epilogue: lane = column of the input, half of the columns of dy per four warps =================
     constexpr int kHalf = kCols / 2;
@@ -328,13 +341,13 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t taddr = tmem_d + (static_cast<uint32_t>((warp & 3) * 32) << 16) + buf * kAccCols + first;
 #pragma unroll
-      for (int c = 0; c < kHalf; c += 16) {
-        uint32_t v[16], w[16];
-        tmem_ld16(v, taddr + c);
-        if constexpr (kParts == 3) tmem_ld16(w, taddr + kCols + c);
+      for (int c = 0; c < kHalf; c += 8) {
+        uint32_t v[8], w[8];
+        tmem_ld8(v, taddr + c);
+        if constexpr (kParts == 3) tmem_ld8(w, taddr + kCols + c);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < 8; ++i)
           acc[c + i] += kParts == 3 ? __uint_as_float(v[i]) + __uint_as_float(w[i]) : __uint_as_float(v[i]);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -355,13 +368,17 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
   }
 }
 
-// dw[o][i] and db[o]: the blocks' partials in order, eight loads in flight.
-__global__ void __launch_bounds__(128) rows8_wgrad_join(const float *partial, const float *partial_db, float *dw, float *db, int k, int n,
-                                                        int k_blocks, int parts) {
+// dw[o][i] and db[o]: warp q of a block adds the partials q, q + 8, ... of 32 outputs, the eight sums are added in order. (A thread
+// per output and all its partials took 11 us for 148 partials of 128 x 100, a chain of loads.)
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(32 * kJoinWarps) rows8_wgrad_join(const float *partial, const float *partial_db, float *dw, float *db,
+                                                                    int k, int n, int k_blocks, int parts) {
   dependency_wait();
-  const int64_t i = blockIdx.x * 128ll + threadIdx.x, kn = static_cast<int64_t>(k) * n;
-  const float *p;
-  int64_t step;
+  __shared__ float side[kJoinWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t i = blockIdx.x * 32ll + lane, kn = static_cast<int64_t>(k) * n;
+  const float *p = nullptr;
+  int64_t step = 0;
   if (i < kn) {
     const int o = static_cast<int>(i / k), c = static_cast<int>(i % k);
     const int64_t pair = c / 128 + static_cast<int64_t>(k_blocks) * (o / 128);
@@ -370,23 +387,27 @@ __global__ void __launch_bounds__(128) rows8_wgrad_join(const float *partial, co
   } else if (db != nullptr && i < kn + n) {
     p = partial_db + (i - kn);
     step = n;
-  } else {
-    return;
   }
   float s = 0.f;
-  int q = 0;
-  for (; q + 8 <= parts; q += 8) {
-    float v[8];
+  if (p != nullptr) {
+    for (int q = warp; q < parts; q += 8 * kJoinWarps) {
+      float v[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = p[(q + u) * step];
+      for (int u = 0; u < 8; ++u) v[u] = q + u * kJoinWarps < parts ? p[(q + u * kJoinWarps) * step] : 0.f;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) s += v[u];
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
   }
-  for (; q < parts; ++q) s += p[q * step];
-  if (i < kn)
-    dw[i] = s;
-  else
-    db[i - kn] = s;
+  side[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && p != nullptr) {
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) s += side[w][lane];
+    if (i < kn)
+      dw[i] = s;
+    else
+      db[i - kn] = s;
+  }
 }
 
 __device__ int32_t r8_status;  // set when a bounded wait ran out, cleared by cxg_rows8_wgrad_status
@@ -461,7 +482,7 @@ extern "C" int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m,
         : by_spans(rows8_wgrad<__nv_bfloat16, false, 1>, rows8_wgrad<__nv_bfloat16, false, 2>);
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_wgrad: %s", cudaGetErrorString(e));
   const int64_t outs = static_cast<int64_t>(k) * n + (db != nullptr ? n : 0);
-  launch_dependent(rows8_wgrad_join, static_cast<unsigned>((outs + 127) / 128), 128, 0, st, a.partial, a.partial_db, dw, db, k, n,
+  launch_dependent(rows8_wgrad_join, static_cast<unsigned>((outs + 31) / 32), 32 * kJoinWarps, 0, st, a.partial, a.partial_db, dw, db, k, n,
                    k_blocks, parts);
   count_launches(2);
   return check_launch("cxg_rows8_wgrad");
