@@ -1067,7 +1067,7 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
       }
     Tensor sums = at::empty({5, x.size(1)}, x.options().dtype(at::kFloat));
     size_t bytes = 0;
-    check(lib.cxg_residual_norm_backward_workspace_size(d.n, d.width, d.dtype, &bytes), "cxg_residual_norm_backward_workspace_size");
+    check(lib.cxg_residual_norm_backward_workspace_size(d.n, d.width, &bytes), "cxg_residual_norm_backward_workspace_size");
     void *st = stream_of(x);
     {
       const Workspace ws = workspace_on(x.device().index(), st, static_cast<int64_t>(bytes), "");

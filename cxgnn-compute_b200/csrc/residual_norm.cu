@@ -10,105 +10,157 @@
 // y, the statistics and the normalised rows are computed again from x, f and gate: reading a row's statistics would save
 // two of its reductions, reading y instead of x nothing.
 //
-// Both are bound by memory: a row is read once, held in registers (16 bytes of every matrix per lane; a part of a warp, a warp
-// or up to 16 warps per row), and written once. A warp asks for its next row before it works on the one that it has: its
-// chains of shuffles (up to nine sums of a row, one behind the other, for the layer norms' gradients) are longer than what
-// the other warps of an SM cover. Parameters come out of L1 for every row; held in registers they cost a third of the warps.
+// Both would be bound by memory, but the arithmetic of a value is what it takes some care to hide behind it. A lane holds 8
+// values of a row (a part of a warp, a warp or up to 16 warps per row: what a row costs by itself, the chains of shuffles of
+// its sums above all, is shared by many values) as pairs for packed fp32 instructions; the next row is on its way into
+// shared memory meanwhile (16-byte asynchronous copies, each lane its own, so there is nothing to wait for but they).
 // Statistics, products and sums are fp32 whatever the rows' type; y is rounded when it is stored, h is computed from it before.
 // The sums over rows are kept per lane for the whole grid's pass, added up per block, and the blocks' sums are added in order
 // by a second kernel: the same bits on every run.
+#include <initializer_list>
+
 #include "rows8.cuh"
 
 namespace cxg {
 namespace {
 
+constexpr int kValues = 8;     // of a row per lane
+constexpr int kPairs = kValues / 2;
 constexpr int kSums = 5;       // dscale, dw2, db2, dw1, db1
 constexpr int kMostWarps = 16;
-constexpr int kMostWidth = 4096;
+constexpr int kMostWidth = kMostWarps * 32 * kValues;
 constexpr int kBlock = 128;    // threads where a row takes a warp or less
 
 struct ResArgs {
-  cxg_residual_desc d;
+  cxg_residual_desc d;  // scale and weights are there: missing ones point at ones
   float inv_width;
   float *part;       // backward: [gridDim.x][kSums][width]
   int keep, groups;  // forward: rows in 8 bits of h
 };
 
+// Stands for a scale or weight that is not given.
+struct alignas(16) Ones {
+  float v[kMostWidth];
+  constexpr Ones() : v() {
+    for (int i = 0; i < kMostWidth; ++i) v[i] = 1.f;
+  }
+};
+__device__ const Ones residual_ones{};
+
 // Where a lane's values lie: Q vectors of N values, the lanes' first vectors side by side, then their second ones. Rows that are
 // not whole 16-byte vectors are read value by value, as many per lane.
-template <typename T, bool VEC, int VECTORS>
+template <typename T, bool VEC, int LANES>
 struct Place {
   static constexpr int N = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
-  static constexpr int Q = VEC ? VECTORS : VECTORS * 16 / static_cast<int>(sizeof(T));
-  static constexpr int V = N * Q;  // values
+  static constexpr int Q = kValues / N;
+  static constexpr int kLanes = LANES;
   using Element = T;
   static constexpr bool kVec = VEC;
+  __device__ __forceinline__ static int column(int p, int i) { return (i / N * LANES + p) * N + i % N; }
 };
 
-// A lane's part of a row as it was loaded.
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// Rows on their way: per thread `tensors` x Q slots of 16 bytes for each of two rows.
 template <typename P>
-struct Raw {
-  using T = typename P::Element;
-  typename Vec<T>::Raw v[P::kVec ? P::Q : 1];
-  T e[P::kVec ? 1 : P::Q];
-  __device__ __forceinline__ void load(const void *base, int64_t row, int width, int p, int lanes) {
-    const T *src = static_cast<const T *>(base) + row * width;
+struct Stage {
+  uint32_t base, step;  // this thread's first slot; from a slot to the next
+  int tensors;
+  __device__ Stage(const void *smem, int n) : base(shared_address(smem) + threadIdx.x * 16), step(blockDim.x * 16), tensors(n) {}
+  __device__ __forceinline__ uint32_t slot(int turn, int tensor, int q) const {
+    return base + ((turn * tensors + tensor) * P::Q + q) * step;
+  }
+  // a row's offset in bytes, the lane's part included
+  __device__ __forceinline__ void request(int turn, int tensor, const void *matrix, int64_t offset, int p, int width) const {
+    using T = typename P::Element;
 #pragma unroll
     for (int q = 0; q < P::Q; ++q) {
-      const int c = (q * lanes + p) * P::N;
-      if constexpr (P::kVec) {
-        v[q] = {};
-        if (c < width) v[q] = Vec<T>::load(src + c);
+      const bool on = P::column(p, q * P::N) < width;
+      const uint8_t *src = static_cast<const uint8_t *>(matrix) + offset + q * (P::kLanes * 16);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot(turn, tensor, q)), "l"(on ? src : matrix), "r"(on ? 16 : 0)
+                   : "memory");
+    }
+  }
+  __device__ __forceinline__ void take(int turn, int tensor, Pair (&v)[kPairs]) const {
+    using T = typename P::Element;
+#pragma unroll
+    for (int q = 0; q < P::Q; ++q) {
+      if constexpr (sizeof(T) == 4) {
+        asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[2 * q]), "=l"(v[2 * q + 1]) : "r"(slot(turn, tensor, q)) : "memory");
       } else {
-        e[q] = from_f32<T>(0.f);
-        if (c < width) e[q] = __ldg(src + c);
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(slot(turn, tensor, q))
+                     : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
       }
     }
   }
-  __device__ __forceinline__ void get(float (&f)[P::V]) const {
-#pragma unroll
-    for (int q = 0; q < P::Q; ++q)
-      if constexpr (P::kVec)
-        Vec<T>::to_float(f + q * P::N, v[q]);
-      else
-        f[q] = to_f32(e[q]);
-  }
 };
 
+// Rows that are not whole vectors, straight from memory.
 template <typename P>
-__device__ __forceinline__ void store_row(void *base, int64_t row, int width, int p, int lanes, const float (&v)[P::V]) {
+__device__ __forceinline__ void read_row(Pair (&v)[kPairs], const void *matrix, int64_t row, int p, int width) {
   using T = typename P::Element;
-  T *dst = static_cast<T *>(base) + row * width;
+  const T *src = static_cast<const T *>(matrix) + row * width;
+  float f[kValues];
+#pragma unroll
+  for (int i = 0; i < kValues; ++i) f[i] = P::column(p, i) < width ? to_f32(__ldg(src + P::column(p, i))) : 0.f;
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
+}
+
+template <typename P>
+__device__ __forceinline__ void store_row(void *matrix, int64_t row, int p, int width, const Pair (&v)[kPairs]) {
+  using T = typename P::Element;
+  T *dst = static_cast<T *>(matrix) + row * width;
+  float f[kValues];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const float2 t = halves(v[i]);
+    f[2 * i] = t.x, f[2 * i + 1] = t.y;
+  }
 #pragma unroll
   for (int q = 0; q < P::Q; ++q) {
-    const int c = (q * lanes + p) * P::N;
+    const int c = P::column(p, q * P::N);
     if (c < width) {
       if constexpr (P::kVec)
-        Vec<T>::store_stream(dst + c, Vec<T>::from_float(v + q * P::N));
+        Vec<T>::store_stream(dst + c, Vec<T>::from_float(f + q * P::N));
       else
-        dst[c] = from_f32<T>(v[q]);
+        dst[c] = from_f32<T>(f[q]);
     }
   }
 }
 
-// A parameter's values at the lane's columns (`other` where there is no parameter; anything behind the row).
+// A parameter's values at the lane's columns (anything behind the row).
 template <typename P>
-__device__ __forceinline__ void load_param(float (&v)[P::V], const float *w, float other, int width, int p, int lanes) {
+__device__ __forceinline__ void load_param(Pair (&v)[kPairs], const float *w, int p, int width) {
 #pragma unroll
-  for (int i = 0; i < P::V; ++i) v[i] = other;
-  if (w == nullptr) return;
-#pragma unroll
-  for (int q = 0; q < P::Q; ++q) {
-    const int c = (q * lanes + p) * P::N;
-    if (c >= width) continue;
+  for (int i = 0; i < kPairs; i += P::kVec ? 2 : 1) {
+    const int c = P::column(p, 2 * i);
     if constexpr (P::kVec) {
-#pragma unroll
-      for (int i = 0; i < P::N; i += 4) {
-        const float4 t = __ldg(reinterpret_cast<const float4 *>(w + c + i));
-        v[q * P::N + i] = t.x, v[q * P::N + i + 1] = t.y, v[q * P::N + i + 2] = t.z, v[q * P::N + i + 3] = t.w;
-      }
+      const ulonglong2 t = __ldg(reinterpret_cast<const ulonglong2 *>(w + (c < width ? c : 0)));
+      v[i] = t.x, v[i + 1] = t.y;
     } else {
-      v[q] = __ldg(w + c);
+      const int e = P::column(p, 2 * i + 1);
+      v[i] = pair(__ldg(w + (c < width ? c : 0)), __ldg(w + (e < width ? e : 0)));
+    }
+  }
+}
+
+// Zeros behind the row.
+template <typename P>
+__device__ __forceinline__ void clear_behind(Pair (&v)[kPairs], int p, int width) {
+  if (width == P::kLanes * kValues) return;
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    if (P::kVec) {
+      if (P::column(p, 2 * i) >= width) v[i] = 0;
+    } else {
+      const float2 t = halves(v[i]);
+      v[i] = pair(P::column(p, 2 * i) < width ? t.x : 0.f, P::column(p, 2 * i + 1) < width ? t.y : 0.f);
     }
   }
 }
@@ -154,39 +206,51 @@ struct RowSum {
   }
 };
 
-// v becomes norm(v); returns the factor. Values behind the row (zeros before) stay zeros.
+// v becomes norm(v); returns the factor. Values behind the row are and stay zeros.
 template <typename P, typename Sum>
-__device__ __forceinline__ float normalise(float (&v)[P::V], const ResArgs &a, Sum &sum, int p, int lanes) {
+__device__ __forceinline__ float normalise(Pair (&v)[kPairs], const ResArgs &a, Sum &sum, int p) {
   if (a.d.layer) {
-    float t = 0.f;
+    const float mean = sum.one(sum2(add2(add2(v[0], v[1]), add2(v[2], v[3])))) * a.inv_width;
+    const Pair off = pair(-mean, -mean);
 #pragma unroll
-    for (int i = 0; i < P::V; ++i) t += v[i];
-    const float mean = sum.one(t) * a.inv_width;
-#pragma unroll
-    for (int q = 0; q < P::Q; ++q) {
-      const float off = (q * lanes + p) * P::N < a.d.width ? mean : 0.f;
-#pragma unroll
-      for (int i = 0; i < P::N; ++i) v[q * P::N + i] -= off;
-    }
+    for (int i = 0; i < kPairs; ++i) v[i] = add2(v[i], off);
+    clear_behind<P>(v, p, a.d.width);
   }
-  float t = 0.f;
+  const Pair t = add2(fma2(v[0], v[0], mul2(v[1], v[1])), fma2(v[2], v[2], mul2(v[3], v[3])));
+  const float r = __frsqrt_rn(fmaf(sum.one(sum2(t)), a.inv_width, a.d.eps));
+  const Pair rr = pair(r, r);
 #pragma unroll
-  for (int i = 0; i < P::V; ++i) t = fmaf(v[i], v[i], t);
-  const float r = __frsqrt_rn(fmaf(sum.one(t), a.inv_width, a.d.eps));
-#pragma unroll
-  for (int i = 0; i < P::V; ++i) v[i] *= r;
+  for (int i = 0; i < kPairs; ++i) v[i] = mul2(v[i], rr);
   return r;
 }
 
 // sigmoid and its derivative without cancellation: t = exp(-|g|), s = 1 / (1 + t) or t / (1 + t), s' = t / (1 + t)^2. The
-// reciprocal of 1 .. 2 is the hardware's, off by an ulp.
+// reciprocal of 1 .. 2 is the hardware's, off by an ulp. For bf16 rows the exponential is the hardware's 2^x of the product
+// rounded once (1e-6 of it at |g| = 16, where 2^-9 is what the result is rounded to).
+template <typename T>
 __device__ __forceinline__ void sigmoid(float g, float *s, float *ds) {
-  const float t = expf(-fabsf(g));
-  float q;
+  float t, q;
+  if constexpr (sizeof(T) == 2)
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fabsf(g) * -1.44269504f));
+  else
+    t = expf(-fabsf(g));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + t));
   const float tq = t * q;
   *s = g >= 0.f ? q : tq;
   *ds = tq * q;
+}
+// The gate's values become sigmoids, and their derivatives where there is room for them.
+template <typename T>
+__device__ __forceinline__ void sigmoids(Pair (&s)[kPairs], Pair *ds) {
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const float2 g = halves(s[i]);
+    float a, b, da, db;
+    sigmoid<T>(g.x, &a, &da);
+    sigmoid<T>(g.y, &b, &db);
+    s[i] = pair(a, b);
+    if (ds != nullptr) ds[i] = pair(da, db);
+  }
 }
 
 // Rows of the grid: `per` per block at a time; the lanes of a warp go through the loop together.
@@ -205,17 +269,18 @@ struct Rows {
 
 // h in 8 bits as it is stored, to row `row`; zeros where `in` is false.
 template <typename P>
-__device__ __forceinline__ void keep_row(const ResArgs &a, int64_t row, bool in, const float (&h)[P::V], int p, int lanes) {
+__device__ __forceinline__ void keep_row(const ResArgs &a, int64_t row, bool in, const Pair (&h)[kPairs], int p) {
   using T = typename P::Element;
   constexpr int kShare = rows8::kGroup / P::N;  // lanes that hold a group
 #pragma unroll
   for (int q = 0; q < P::Q; ++q) {
-    const int c = (q * lanes + p) * P::N;
+    const int c = P::column(p, q * P::N);
     float v[P::N];
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < P::N; ++i) {
-      v[i] = in && c < a.d.width ? to_f32(from_f32<T>(h[q * P::N + i])) : 0.f;
+      const float2 t = halves(h[(q * P::N + i) / 2]);
+      v[i] = in && c < a.d.width ? to_f32(from_f32<T>(i & 1 ? t.y : t.x)) : 0.f;
       top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
     }
 #pragma unroll
@@ -235,21 +300,21 @@ __device__ __forceinline__ void keep_row(const ResArgs &a, int64_t row, bool in,
   }
 }
 
-// Warps per SM: 64 registers a thread forward, 128 backward, 168 where eight values per lane meet five sums of each (with 128
-// registers these spill 250 bytes a lane).
-constexpr int forward_warps(int values, bool gated) { return values > 4 && gated ? 24 : 32; }
-constexpr int backward_warps(int values, bool biases) { return values > 4 && biases ? 12 : 16; }
-
-// Blocks per SM of `threads` threads with that many warps.
+// Warps per SM, by the registers a thread gets (80 forward, 128 backward), and blocks of `threads` threads with that many warps.
+constexpr int kForwardWarps = 24, kBackwardWarps = 16;
 constexpr int blocks_of(int warps, int threads) { return warps * 32 / threads > 0 ? warps * 32 / threads : 1; }
+// Shared memory of a block for two rows of so many matrices.
+template <typename P>
+constexpr int stage_bytes(int tensors, int threads) { return P::kVec ? 2 * tensors * P::Q * 16 * threads : 0; }
+constexpr int kForwardTensors = 3, kBackwardTensors = 5;
 
 // GATED: a gate per value.
-template <typename T, int LANES, int WARPS, bool VEC, int VECTORS, bool GATED>
-__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock,
-                                  blocks_of(forward_warps(Place<T, VEC, VECTORS>::V, GATED), WARPS > 1 ? 32 * WARPS : kBlock))
+template <typename T, int LANES, int WARPS, bool VEC, bool GATED>
+__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kForwardWarps, WARPS > 1 ? 32 * WARPS : kBlock))
     residual_forward(const __grid_constant__ ResArgs a) {
-  using P = Place<T, VEC, VECTORS>;
   constexpr int kLanes = LANES * WARPS;
+  using P = Place<T, VEC, kLanes>;
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float2 place[2][WARPS];
   RowSum<LANES, WARPS> sum(place);
   const cxg_residual_desc &d = a.d;
@@ -257,226 +322,279 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock,
   const bool with_f = d.f != nullptr, row_gate = d.gate_mode == CXG_GATE_ROW;
   dependency_wait();
   const Rows<LANES, WARPS> rows;
-  Raw<P> rx, rf, rg;
+  const Stage<P> stage(smem, kForwardTensors);
   T rr = from_f32<T>(0.f);
-  auto load = [&](int64_t row) {
+  auto request = [&](int turn, int64_t row) {
     const int64_t at = row < d.n ? row : d.n - 1;
-    rx.load(d.x, at, width, p, kLanes);
-    if (with_f) rf.load(d.f, at, width, p, kLanes);
-    if (GATED) rg.load(d.gate, at, width, p, kLanes);
+    if constexpr (VEC) {
+      const int64_t offset = at * width * static_cast<int64_t>(sizeof(T)) + p * 16;
+      stage.request(turn, 0, d.x, offset, p, width);
+      if (with_f) stage.request(turn, 1, d.f, offset, p, width);
+      if (GATED) stage.request(turn, 2, d.gate, offset, p, width);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     if (row_gate) rr = __ldg(static_cast<const T *>(d.gate) + at);
   };
   const int64_t n_end = d.n + a.keep;
-  if (rows.first < n_end) load(rows.first + rows.sub);
-  for (int64_t row0 = rows.first; row0 < n_end; row0 += rows.step) {
-    const int64_t row = row0 + rows.sub;
+  int turn = 0;
+  if (rows.first < n_end) request(0, rows.first + rows.sub);
+  for (int64_t row0 = rows.first; row0 < n_end; row0 += rows.step, turn ^= 1) {
+    const int64_t row = row0 + rows.sub, at = row < d.n ? row : d.n - 1;
     const bool in = row < d.n;
-    float y[P::V], n[P::V], s[P::V], one = 1.f, ds;
-    rx.get(y);
-    if (with_f) rf.get(n);
-    if (GATED) rg.get(s);
     const float g_row = to_f32(rr);
-    if (row0 + rows.step < n_end) load(row + rows.step);
+    Pair y[kPairs], n[kPairs], s[kPairs];
+    if constexpr (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (row0 + rows.step < n_end) request(turn ^ 1, row + rows.step);
+    auto take = [&](Pair(&v)[kPairs], int tensor, const void *matrix) {
+      if constexpr (VEC)
+        stage.take(turn, tensor, v);
+      else
+        read_row<P>(v, matrix, at, p, width);
+    };
+    take(y, 0, d.x);
     if (with_f) {
+      take(n, 1, d.f);
+      Pair w[kPairs], b[kPairs];
       if (d.post) {
-        normalise<P>(n, a, sum, p, kLanes);
-        float w[P::V], b[P::V];
-        load_param<P>(w, d.post_weight, 1.f, width, p, kLanes);
+        normalise<P>(n, a, sum, p);
+        load_param<P>(w, d.post_weight, p, width);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) n[i] = mul2(n[i], w[i]);
         if (d.post_bias != nullptr) {
-          load_param<P>(b, d.post_bias, 0.f, width, p, kLanes);
+          load_param<P>(b, d.post_bias, p, width);
 #pragma unroll
-          for (int i = 0; i < P::V; ++i) n[i] = fmaf(n[i], w[i], b[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < P::V; ++i) n[i] *= w[i];
+          for (int i = 0; i < kPairs; ++i) n[i] = add2(n[i], b[i]);
         }
       }
-      if (row_gate) sigmoid(g_row, &one, &ds);
+      load_param<P>(w, d.scale, p, width);
       if (GATED) {
+        take(s, 2, d.gate);
+        sigmoids<T>(s, nullptr);
 #pragma unroll
-        for (int i = 0; i < P::V; ++i) sigmoid(s[i], &s[i], &ds);
+        for (int i = 0; i < kPairs; ++i) w[i] = mul2(w[i], s[i]);
+      } else if (row_gate) {
+        float one, ds;
+        sigmoid<T>(g_row, &one, &ds);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) w[i] = mul2(w[i], pair(one, one));
       }
-      float scale[P::V];
-      load_param<P>(scale, d.scale, 1.f, width, p, kLanes);
 #pragma unroll
-      for (int i = 0; i < P::V; ++i) y[i] = fmaf(scale[i] * (GATED ? s[i] : one), n[i], y[i]);
-      if (d.y != nullptr && in) store_row<P>(d.y, row, width, p, kLanes, y);
+      for (int i = 0; i < kPairs; ++i) y[i] = fma2(w[i], n[i], y[i]);
+      clear_behind<P>(y, p, width);
+      if (d.y != nullptr && in) store_row<P>(d.y, row, p, width, y);
     }
     if (d.next) {
-      normalise<P>(y, a, sum, p, kLanes);
-      float w[P::V], b[P::V];
-      load_param<P>(w, d.next_weight, 1.f, width, p, kLanes);
-      load_param<P>(b, d.next_bias, 0.f, width, p, kLanes);
+      normalise<P>(y, a, sum, p);
+      Pair w[kPairs];
+      load_param<P>(w, d.next_weight, p, width);
+      if (d.next_bias != nullptr) {
+        Pair b[kPairs];
+        load_param<P>(b, d.next_bias, p, width);
 #pragma unroll
-      for (int i = 0; i < P::V; ++i) y[i] = fmaf(y[i], w[i], b[i]);
-      if (in) store_row<P>(d.h, row, width, p, kLanes, y);
+        for (int i = 0; i < kPairs; ++i) y[i] = fma2(y[i], w[i], b[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) y[i] = mul2(y[i], w[i]);
+      }
+      if (in) store_row<P>(d.h, row, p, width, y);
       if constexpr (VEC) {
-        if (a.keep) keep_row<P>(a, row, in, y, p, kLanes);
+        if (a.keep) keep_row<P>(a, row, in, y, p);
       }
     }
   }
 }
 
-// g becomes r (g - <g> - u <g u>) (without <g> where no mean was taken off)
-template <int V, typename Sum>
-__device__ __forceinline__ void back_through_norm(float (&g)[V], const float (&u)[V], float r, const ResArgs &a, Sum &sum) {
-  float t0 = 0.f, t1 = 0.f;
-#pragma unroll
-  for (int i = 0; i < V; ++i) t0 += g[i], t1 = fmaf(g[i], u[i], t1);
+// g becomes r (g - <g> - u <g u>) (without <g> where no mean was taken off); zeros behind the row
+template <typename P, typename Sum>
+__device__ __forceinline__ void back_through_norm(Pair (&g)[kPairs], const Pair (&u)[kPairs], float r, const ResArgs &a, Sum &sum, int p) {
+  const Pair t = add2(fma2(g[0], u[0], mul2(g[1], u[1])), fma2(g[2], u[2], mul2(g[3], u[3])));
   float mean = 0.f, dot;
   if (a.d.layer) {
-    const float2 t = sum.both(t0, t1);
-    mean = t.x * a.inv_width, dot = t.y * a.inv_width;
+    const float2 m = sum.both(sum2(add2(add2(g[0], g[1]), add2(g[2], g[3]))), sum2(t));
+    mean = m.x * a.inv_width, dot = m.y * a.inv_width;
   } else {
-    dot = sum.one(t1) * a.inv_width;
+    dot = sum.one(sum2(t)) * a.inv_width;
   }
+  const Pair rr = pair(r, r), dots = pair(-dot, -dot), means = pair(-mean, -mean);
 #pragma unroll
-  for (int i = 0; i < V; ++i) g[i] = r * (fmaf(-u[i], dot, g[i]) - mean);
+  for (int i = 0; i < kPairs; ++i) {
+    Pair v = fma2(u[i], dots, g[i]);
+    if (a.d.layer) v = add2(v, means);
+    g[i] = mul2(v, rr);
+  }
+  clear_behind<P>(g, p, a.d.width);
 }
 
 // BIASES: sums for them too.
-template <typename T, int LANES, int WARPS, bool VEC, int VECTORS, bool GATED, bool BIASES>
-__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock,
-                                  blocks_of(backward_warps(Place<T, VEC, VECTORS>::V, BIASES), WARPS > 1 ? 32 * WARPS : kBlock))
+template <typename T, int LANES, int WARPS, bool VEC, bool GATED, bool BIASES>
+__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBackwardWarps, WARPS > 1 ? 32 * WARPS : kBlock))
     residual_backward(const __grid_constant__ ResArgs a) {
-  using P = Place<T, VEC, VECTORS>;
   constexpr int kLanes = LANES * WARPS;
+  using P = Place<T, VEC, kLanes>;
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float2 place[2][WARPS];
   RowSum<LANES, WARPS> sum(place);
   const cxg_residual_desc &d = a.d;
   const int p = threadIdx.x & (kLanes - 1), width = d.width;
   const bool with_f = d.f != nullptr, row_gate = d.gate_mode == CXG_GATE_ROW, next = d.next && d.dh != nullptr;
   dependency_wait();
-  float acc[kSums][P::V];
+  Pair acc[kSums][kPairs];
 #pragma unroll
   for (int k = 0; k < kSums; ++k)
 #pragma unroll
-    for (int i = 0; i < P::V; ++i) acc[k][i] = 0.f;
+    for (int i = 0; i < kPairs; ++i) acc[k][i] = 0;
   const Rows<LANES, WARPS> rows;
-  Raw<P> rx, rf, rg, ry, rh;
+  const Stage<P> stage(smem, kBackwardTensors);
   T rr = from_f32<T>(0.f);
-  auto load = [&](int64_t row) {
+  auto request = [&](int turn, int64_t row) {
     const int64_t at = row < d.n ? row : d.n - 1;
-    rx.load(d.x, at, width, p, kLanes);
-    if (with_f) rf.load(d.f, at, width, p, kLanes);
-    if (GATED) rg.load(d.gate, at, width, p, kLanes);
+    if constexpr (VEC) {
+      const int64_t offset = at * width * static_cast<int64_t>(sizeof(T)) + p * 16;
+      stage.request(turn, 0, d.x, offset, p, width);
+      if (with_f) stage.request(turn, 1, d.f, offset, p, width);
+      if (GATED) stage.request(turn, 2, d.gate, offset, p, width);
+      if (d.dy != nullptr) stage.request(turn, 3, d.dy, offset, p, width);
+      if (next) stage.request(turn, 4, d.dh, offset, p, width);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     if (row_gate) rr = __ldg(static_cast<const T *>(d.gate) + at);
-    if (d.dy != nullptr) ry.load(d.dy, at, width, p, kLanes);
-    if (next) rh.load(d.dh, at, width, p, kLanes);
   };
-  if (rows.first < d.n) load(rows.first + rows.sub);
-  for (int64_t row0 = rows.first; row0 < d.n; row0 += rows.step) {
-    const int64_t row = row0 + rows.sub;
+  int turn = 0;
+  if (rows.first < d.n) request(0, rows.first + rows.sub);
+  for (int64_t row0 = rows.first; row0 < d.n; row0 += rows.step, turn ^= 1) {
+    const int64_t row = row0 + rows.sub, at = row < d.n ? row : d.n - 1;
     const bool in = row < d.n;  // lanes without a row go through it with gradients of zero
-    float y[P::V], n[P::V], s[GATED ? P::V : 1], ds[GATED ? P::V : 1], g[P::V], dh[P::V];
-    rx.get(y);
-    if (with_f) rf.get(n);
-    if constexpr (GATED) rg.get(s);
     const float g_row = to_f32(rr);
-#pragma unroll
-    for (int i = 0; i < P::V; ++i) g[i] = dh[i] = 0.f;
-    if (in && d.dy != nullptr) ry.get(g);
-    if (in && next) rh.get(dh);
-    if (row0 + rows.step < d.n) load(row + rows.step);
-    float r2 = 0.f, scale[P::V];
+    if constexpr (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (row0 + rows.step < d.n) request(turn ^ 1, row + rows.step);
+    auto take = [&](Pair(&v)[kPairs], int tensor, const void *matrix) {
+      if constexpr (VEC)
+        stage.take(turn, tensor, v);
+      else
+        read_row<P>(v, matrix, at, p, width);
+    };
+    Pair y[kPairs], n[kPairs], s[GATED ? kPairs : 1], ds[GATED ? kPairs : 1], g[kPairs], w[kPairs];
+    take(y, 0, d.x);
+    float r2 = 0.f;
     if constexpr (!GATED) {
-      s[0] = 1.f, ds[0] = 0.f;
-      if (row_gate) sigmoid(g_row, &s[0], &ds[0]);
+      float s0 = 1.f, ds0 = 0.f;
+      if (row_gate) sigmoid<T>(g_row, &s0, &ds0);
+      s[0] = pair(s0, s0), ds[0] = pair(ds0, ds0);
     }
     if (with_f) {
-      load_param<P>(scale, d.scale, 1.f, width, p, kLanes);
+      take(n, 1, d.f);
       if constexpr (GATED) {
-#pragma unroll
-        for (int i = 0; i < P::V; ++i) sigmoid(s[i], &s[i], &ds[i]);
+        take(s, 2, d.gate);
+        sigmoids<T>(s, ds);
       }
+      Pair t[kPairs];
       if (d.post) {
-        r2 = normalise<P>(n, a, sum, p, kLanes);  // n is u2 from here on
-        float w2[P::V], b2[P::V];
-        load_param<P>(w2, d.post_weight, 1.f, width, p, kLanes);
-        load_param<P>(b2, d.post_bias, 0.f, width, p, kLanes);
+        r2 = normalise<P>(n, a, sum, p);  // n is u2 from here on
+        load_param<P>(w, d.post_weight, p, width);
 #pragma unroll
-        for (int i = 0; i < P::V; ++i) y[i] = fmaf(scale[i] * s[GATED ? i : 0], fmaf(n[i], w2[i], b2[i]), y[i]);
+        for (int i = 0; i < kPairs; ++i) t[i] = mul2(n[i], w[i]);
+        if (BIASES && d.post_bias != nullptr) {
+          load_param<P>(w, d.post_bias, p, width);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) t[i] = add2(t[i], w[i]);
+        }
       } else {
 #pragma unroll
-        for (int i = 0; i < P::V; ++i) y[i] = fmaf(scale[i] * s[GATED ? i : 0], n[i], y[i]);
+        for (int i = 0; i < kPairs; ++i) t[i] = n[i];
       }
+      load_param<P>(w, d.scale, p, width);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) y[i] = fma2(mul2(w[i], s[GATED ? i : 0]), t[i], y[i]);
+      clear_behind<P>(y, p, width);
     }
+    if (in && d.dy != nullptr)
+      take(g, 3, d.dy);
+    else
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) g[i] = 0;
     if (next) {
-      const float r1 = normalise<P>(y, a, sum, p, kLanes);  // y is u1 from here on
-      float t[P::V];
-      load_param<P>(t, d.next_weight, 1.f, width, p, kLanes);
+      const float r1 = normalise<P>(y, a, sum, p);  // y is u1 from here on
+      Pair dh[kPairs];
+      if (in)
+        take(dh, 4, d.dh);
+      else
 #pragma unroll
-      for (int i = 0; i < P::V; ++i) {
-        acc[3][i] = fmaf(dh[i], y[i], acc[3][i]);
-        if (BIASES) acc[4][i] += dh[i];
-        t[i] *= dh[i];
+        for (int i = 0; i < kPairs; ++i) dh[i] = 0;
+      load_param<P>(w, d.next_weight, p, width);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        acc[3][i] = fma2(dh[i], y[i], acc[3][i]);
+        if (BIASES) acc[4][i] = add2(acc[4][i], dh[i]);
+        dh[i] = mul2(dh[i], w[i]);
       }
-      back_through_norm(t, y, r1, a, sum);
+      back_through_norm<P>(dh, y, r1, a, sum, p);
 #pragma unroll
-      for (int i = 0; i < P::V; ++i) g[i] += t[i];
-#pragma unroll
-      for (int i = 0; i < P::V; ++i)
-        if (((i / P::N) * kLanes + p) * P::N >= width) g[i] = 0.f;
+      for (int i = 0; i < kPairs; ++i) g[i] = add2(g[i], dh[i]);
     }
-    if (in && d.dx != nullptr) store_row<P>(d.dx, row, width, p, kLanes, g);
+    if (in && d.dx != nullptr) store_row<P>(d.dx, row, p, width, g);
     if (with_f) {
-      float w2[P::V], dg[P::V];
-#pragma unroll
-      for (int i = 0; i < P::V; ++i) dg[i] = n[i];
+      Pair w2[kPairs], t[kPairs];
       if (d.post) {
-        float b2[P::V];
-        load_param<P>(w2, d.post_weight, 1.f, width, p, kLanes);
-        load_param<P>(b2, d.post_bias, 0.f, width, p, kLanes);
+        load_param<P>(w2, d.post_weight, p, width);
 #pragma unroll
-        for (int i = 0; i < P::V; ++i) dg[i] = fmaf(n[i], w2[i], b2[i]);
+        for (int i = 0; i < kPairs; ++i) t[i] = mul2(n[i], w2[i]);
+        if (BIASES && d.post_bias != nullptr) {
+          load_param<P>(w, d.post_bias, p, width);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) t[i] = add2(t[i], w[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) t[i] = n[i];
       }
-      load_param<P>(scale, d.scale, 1.f, width, p, kLanes);
+      load_param<P>(w, d.scale, p, width);
 #pragma unroll
-      for (int i = 0; i < P::V; ++i) {
-        acc[0][i] = fmaf(g[i] * s[GATED ? i : 0], dg[i], acc[0][i]);
-        g[i] *= scale[i];
-        dg[i] *= g[i] * ds[GATED ? i : 0];
-        g[i] *= s[GATED ? i : 0];  // dn
+      for (int i = 0; i < kPairs; ++i) {
+        acc[0][i] = fma2(mul2(g[i], s[GATED ? i : 0]), t[i], acc[0][i]);
+        g[i] = mul2(g[i], w[i]);
+        t[i] = mul2(mul2(t[i], g[i]), ds[GATED ? i : 0]);  // dgate
+        g[i] = mul2(g[i], s[GATED ? i : 0]);               // dn
       }
       if constexpr (GATED) {
-        if (in && d.dgate != nullptr) store_row<P>(d.dgate, row, width, p, kLanes, dg);
+        if (in && d.dgate != nullptr) store_row<P>(d.dgate, row, p, width, t);
       } else if (row_gate) {
-        float t = 0.f;
-#pragma unroll
-        for (int i = 0; i < P::V; ++i) t += dg[i];
-        t = sum.one(t);
-        if (in && p == 0 && d.dgate != nullptr) static_cast<T *>(d.dgate)[row] = from_f32<T>(t);
+        clear_behind<P>(t, p, width);
+        const float dg = sum.one(sum2(add2(add2(t[0], t[1]), add2(t[2], t[3]))));
+        if (in && p == 0 && d.dgate != nullptr) static_cast<T *>(d.dgate)[row] = from_f32<T>(dg);
       }
       if (d.post) {
 #pragma unroll
-        for (int i = 0; i < P::V; ++i) {
-          acc[1][i] = fmaf(g[i], n[i], acc[1][i]);
-          if (BIASES) acc[2][i] += g[i];
-          g[i] *= w2[i];
+        for (int i = 0; i < kPairs; ++i) {
+          acc[1][i] = fma2(g[i], n[i], acc[1][i]);
+          if (BIASES) acc[2][i] = add2(acc[2][i], g[i]);
+          g[i] = mul2(g[i], w2[i]);
         }
-        back_through_norm(g, n, r2, a, sum);
+        back_through_norm<P>(g, n, r2, a, sum, p);
       }
-      if (in && d.df != nullptr) store_row<P>(d.df, row, width, p, kLanes, g);
+      if (in && d.df != nullptr) store_row<P>(d.df, row, p, width, g);
     }
   }
   // the block's sums: lanes of a warp that hold the same columns, then the warps in order
   float *part = a.part + static_cast<int64_t>(blockIdx.x) * kSums * width;
-  if constexpr (WARPS == 1) {
-    __shared__ float side[kBlock / 32][LANES * P::V];
-    const int warp = threadIdx.x >> 5;
+  [[maybe_unused]] __shared__ float side[WARPS == 1 ? kBlock / 32 : 1][WARPS == 1 ? LANES * kValues : 1];
 #pragma unroll
-    for (int k = 0; k < kSums; ++k) {
+  for (int k = 0; k < kSums; ++k) {
+    float f[kValues];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const float2 t = halves(acc[k][i]);
+      f[2 * i] = t.x, f[2 * i + 1] = t.y;
+    }
+    if constexpr (WARPS == 1) {
       if (!BIASES && (k == 2 || k == 4)) {
         for (int c = threadIdx.x; c < width; c += kBlock) part[k * width + c] = 0.f;
         continue;
       }
 #pragma unroll
-      for (int i = 0; i < P::V; ++i)
+      for (int i = 0; i < kValues; ++i) {
 #pragma unroll
-        for (int o = LANES; o < 32; o <<= 1) acc[k][i] += __shfl_xor_sync(0xffffffffu, acc[k][i], o);
-      if ((threadIdx.x & 31) < LANES) {
-#pragma unroll
-        for (int i = 0; i < P::V; ++i) side[warp][((i / P::N) * kLanes + p) * P::N + i % P::N] = acc[k][i];
+        for (int o = LANES; o < 32; o <<= 1) f[i] += __shfl_xor_sync(0xffffffffu, f[i], o);
+        if ((threadIdx.x & 31) < LANES) side[threadIdx.x >> 5][P::column(p, i)] = f[i];
       }
       __syncthreads();
       for (int c = threadIdx.x; c < width; c += kBlock) {
@@ -486,88 +604,99 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock,
         part[k * width + c] = t;
       }
       __syncthreads();
+    } else {
+#pragma unroll
+      for (int i = 0; i < kValues; ++i)
+        if (P::column(p, i) < width) part[k * width + P::column(p, i)] = f[i];
     }
-  } else {
-#pragma unroll
-    for (int k = 0; k < kSums; ++k)
-#pragma unroll
-      for (int i = 0; i < P::V; ++i) {
-        const int c = ((i / P::N) * kLanes + p) * P::N + i % P::N;
-        if (c < width) part[k * width + c] = acc[k][i];
-      }
   }
 }
 
-// Lanes of a row: the smallest power of two, from 8 on, that holds it (16 bytes a lane; 32 where 16 warps are not enough).
-int values_of(int dtype) { return dtype == CXG_F32 ? 4 : 8; }
-int lanes_of(int width, int dtype) {
+// Lanes of a row: the smallest power of two, from 8 on, that holds it.
+int lanes_of(int width) {
   int lanes = 8;
-  while (lanes < 32 * kMostWarps && lanes * values_of(dtype) < width) lanes *= 2;
+  while (lanes * kValues < width) lanes *= 2;
   return lanes;
 }
 int rows_per_block(int lanes) { return lanes > 32 ? 1 : kBlock / lanes; }
-int backward_blocks(int64_t n, int lanes) {
-  const int64_t most = kNumSM * blocks_of(16, lanes > 32 ? lanes : kBlock);
+int blocks_for(int64_t n, int lanes, int warps) {
+  const int64_t most = kNumSM * blocks_of(warps, lanes > 32 ? lanes : kBlock);
   const int64_t want = (n + rows_per_block(lanes) - 1) / rows_per_block(lanes);
   return static_cast<int>(want < 1 ? 1 : want < most ? want : most);
 }
 
 template <typename T, bool VEC, bool GATED, typename Go>
-cudaError_t by_width(int width, int dtype, Go go) {
-  switch (lanes_of(width, dtype)) {
-    case 8: return go.template run<T, 8, 1, VEC, 1, GATED>();
-    case 16: return go.template run<T, 16, 1, VEC, 1, GATED>();
-    case 32: return go.template run<T, 32, 1, VEC, 1, GATED>();
-    case 64: return go.template run<T, 32, 2, VEC, 1, GATED>();
-    case 128: return go.template run<T, 32, 4, VEC, 1, GATED>();
-    case 256: return go.template run<T, 32, 8, VEC, 1, GATED>();
-    default: break;
+cudaError_t by_width(int width, Go go) {
+  switch (lanes_of(width)) {
+    case 8: return go.template run<T, 8, 1, VEC, GATED>();
+    case 16: return go.template run<T, 16, 1, VEC, GATED>();
+    case 32: return go.template run<T, 32, 1, VEC, GATED>();
+    case 64: return go.template run<T, 32, 2, VEC, GATED>();
+    case 128: return go.template run<T, 32, 4, VEC, GATED>();
+    case 256: return go.template run<T, 32, 8, VEC, GATED>();
+    default: return go.template run<T, 32, 16, VEC, GATED>();
   }
-  if constexpr (sizeof(T) == 4)
-    if (width > 32 * kMostWarps * 4) return go.template run<T, 32, kMostWarps, VEC, 2, GATED>();
-  return go.template run<T, 32, kMostWarps, VEC, 1, GATED>();
 }
 template <typename T, typename Go>
 cudaError_t by_kind(const cxg_residual_desc &d, bool vec, Go go) {
   const bool gated = d.gate_mode == CXG_GATE_VALUE;
-  if (vec) return gated ? by_width<T, true, true>(d.width, d.dtype, go) : by_width<T, true, false>(d.width, d.dtype, go);
-  return gated ? by_width<T, false, true>(d.width, d.dtype, go) : by_width<T, false, false>(d.width, d.dtype, go);
+  if (vec) return gated ? by_width<T, true, true>(d.width, go) : by_width<T, true, false>(d.width, go);
+  return gated ? by_width<T, false, true>(d.width, go) : by_width<T, false, false>(d.width, go);
 }
 template <typename Go>
 cudaError_t by_type(const cxg_residual_desc &d, bool vec, Go go) {
   return d.dtype == CXG_F32 ? by_kind<float>(d, vec, go) : by_kind<__nv_bfloat16>(d, vec, go);
 }
 
+template <typename P, typename Kernel>
+cudaError_t launch(Kernel kernel, int tensors, int threads, int blocks, const ResArgs &a, cudaStream_t st) {
+  const int smem = stage_bytes<P>(tensors, threads);
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_dependent(kernel, static_cast<unsigned>(blocks), threads, static_cast<size_t>(smem), st, a);
+}
+
 struct Forward {
   const ResArgs &a;
   cudaStream_t st;
-  template <typename T, int LANES, int WARPS, bool VEC, int VECTORS, bool GATED>
+  template <typename T, int LANES, int WARPS, bool VEC, bool GATED>
   cudaError_t run() const {
-    const int per = rows_per_block(LANES * WARPS);
-    constexpr int kThreads = WARPS > 1 ? 32 * WARPS : kBlock;
-    const int64_t want = (a.d.n + a.keep + per - 1) / per, most = kNumSM * blocks_of(forward_warps(Place<T, VEC, VECTORS>::V, GATED), kThreads);
-    return launch_dependent(residual_forward<T, LANES, WARPS, VEC, VECTORS, GATED>, static_cast<unsigned>(want < most ? want : most),
-                            kThreads, 0, st, a);
+    return launch<Place<T, VEC, LANES * WARPS>>(residual_forward<T, LANES, WARPS, VEC, GATED>, kForwardTensors,
+                                                WARPS > 1 ? 32 * WARPS : kBlock,
+                                                blocks_for(a.d.n + a.keep, LANES * WARPS, kForwardWarps), a, st);
   }
 };
 struct Backward {
   const ResArgs &a;
   cudaStream_t st;
-  int *blocks;
-  template <typename T, int LANES, int WARPS, bool VEC, int VECTORS, bool GATED, bool BIASES>
+  int blocks;
+  template <typename T, int LANES, int WARPS, bool VEC, bool GATED, bool BIASES>
   cudaError_t go() const {
-    constexpr int kThreads = WARPS > 1 ? 32 * WARPS : kBlock;
-    const int most = kNumSM * blocks_of(backward_warps(Place<T, VEC, VECTORS>::V, BIASES), kThreads);
-    if (*blocks > most) *blocks = most;
-    return launch_dependent(residual_backward<T, LANES, WARPS, VEC, VECTORS, GATED, BIASES>, static_cast<unsigned>(*blocks), kThreads, 0,
-                            st, a);
+    return launch<Place<T, VEC, LANES * WARPS>>(residual_backward<T, LANES, WARPS, VEC, GATED, BIASES>, kBackwardTensors,
+                                                WARPS > 1 ? 32 * WARPS : kBlock, blocks, a, st);
   }
-  template <typename T, int LANES, int WARPS, bool VEC, int VECTORS, bool GATED>
+  template <typename T, int LANES, int WARPS, bool VEC, bool GATED>
   cudaError_t run() const {
-    return a.d.post_bias != nullptr || a.d.next_bias != nullptr ? go<T, LANES, WARPS, VEC, VECTORS, GATED, true>()
-                                                                : go<T, LANES, WARPS, VEC, VECTORS, GATED, false>();
+    return a.d.post_bias != nullptr || a.d.next_bias != nullptr ? go<T, LANES, WARPS, VEC, GATED, true>()
+                                                                : go<T, LANES, WARPS, VEC, GATED, false>();
   }
 };
+
+// The launch's arguments: missing scales and weights are ones.
+cudaError_t arguments(const cxg_residual_desc &d, ResArgs *a) {
+  *a = {};
+  a->d = d;
+  a->inv_width = 1.f / static_cast<float>(d.width);
+  a->groups = rows8::groups_of(d.width);
+  if (d.scale != nullptr && d.post_weight != nullptr && d.next_weight != nullptr) return cudaSuccess;
+  void *ones = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&ones, residual_ones);
+  for (const float **w : {&a->d.scale, &a->d.post_weight, &a->d.next_weight})
+    if (*w == nullptr) *w = static_cast<const float *>(ones);
+  return e;
+}
 
 // Rows of whole 16-byte vectors: all matrices, and the parameters, which are fp32.
 bool whole_vectors(const cxg_residual_desc &d) {
@@ -609,23 +738,20 @@ extern "C" int cxg_residual_norm_forward(const cxg_residual_desc *d, void *strea
               CXG_EINVAL, "cxg_residual_norm_forward: rows in 8 bits are kept of h, in whole 16-byte vectors");
   if (d->n == 0 && !keep) return CXG_OK;
   CXG_REQUIRE(d->n > 0, CXG_EINVAL, "cxg_residual_norm_forward: no rows to keep");
-  ResArgs a = {};
-  a.d = *d;
-  a.inv_width = 1.f / static_cast<float>(d->width);
+  ResArgs a;
+  cudaError_t e = arguments(*d, &a);
   a.keep = keep ? 1 : 0;
-  a.groups = rows8::groups_of(d->width);
-  const cudaError_t e = by_type(*d, whole_vectors(*d), Forward{a, as_stream(stream)});
+  if (e == cudaSuccess) e = by_type(*d, whole_vectors(*d), Forward{a, as_stream(stream)});
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_residual_norm_forward: %s", cudaGetErrorString(e));
   count_launches(1);
   return check_launch("cxg_residual_norm_forward");
 }
 
-extern "C" int cxg_residual_norm_backward_workspace_size(int64_t n, int width, int dtype, size_t *bytes) {
+extern "C" int cxg_residual_norm_backward_workspace_size(int64_t n, int width, size_t *bytes) {
   CXG_REQUIRE(bytes != nullptr, CXG_ENULL, "cxg_residual_norm_backward_workspace_size: bytes is NULL");
-  CXG_REQUIRE(n >= 0 && width > 0 && (dtype == CXG_F32 || dtype == CXG_BF16), CXG_EINVAL,
-              "cxg_residual_norm_backward_workspace_size: bad sizes or type");
+  CXG_REQUIRE(n >= 0 && width > 0, CXG_EINVAL, "cxg_residual_norm_backward_workspace_size: bad sizes");
   CXG_REQUIRE(width <= kMostWidth, CXG_EUNSUPPORTED, "cxg_residual_norm: rows of %d values, at most %d", width, kMostWidth);
-  *bytes = static_cast<size_t>(backward_blocks(n, lanes_of(width, dtype))) * kSums * width * sizeof(float);
+  *bytes = static_cast<size_t>(blocks_for(n, lanes_of(width), kBackwardWarps)) * kSums * width * sizeof(float);
   return CXG_OK;
 }
 
@@ -640,15 +766,14 @@ extern "C" int cxg_residual_norm_backward(const cxg_residual_desc *d, float *sum
     return CXG_OK;
   }
   size_t need = 0;
-  cxg_residual_norm_backward_workspace_size(d->n, d->width, d->dtype, &need);
+  cxg_residual_norm_backward_workspace_size(d->n, d->width, &need);
   CXG_REQUIRE(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, CXG_EWORKSPACE,
               "cxg_residual_norm_backward: workspace %zu bytes, need %zu", workspace_bytes, need);
-  ResArgs a = {};
-  a.d = *d;
-  a.inv_width = 1.f / static_cast<float>(d->width);
+  ResArgs a;
+  cudaError_t e = arguments(*d, &a);
   a.part = static_cast<float *>(workspace);
-  int blocks = backward_blocks(d->n, lanes_of(d->width, d->dtype));
-  const cudaError_t e = by_type(*d, whole_vectors(*d), Backward{a, st, &blocks});
+  const int blocks = blocks_for(d->n, lanes_of(d->width), kBackwardWarps);
+  if (e == cudaSuccess) e = by_type(*d, whole_vectors(*d), Backward{a, st, blocks});
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_residual_norm_backward: %s", cudaGetErrorString(e));
   column_sum_join(a.part, sums, blocks, kSums * d->width, st);
   count_launches(2);

@@ -25,15 +25,16 @@ using rows8::kGroup;
 
 constexpr int kPos = 64;           // rows per stage
 constexpr int kSpan = kPos * 128;  // bytes of a span: 64 columns of bf16, one row behind the other
-constexpr int kProdWarps = 8, kEpiWarps = 8;
+constexpr int kProdWarps = 16, kEpiWarps = 8;
 constexpr int kMmaWarp = kEpiWarps, kFirstProd = kMmaWarp + 4;  // roles in whole groups of four warps, which share out registers
 constexpr int kThreads = 32 * (kFirstProd + kProdWarps);
-// Registers per thread: 96 at the launch (640 threads take 61,440); the producers, which hold two stages of loads, take 32 more
-// each from the group of the issuing warp and what is left over: 256 * 96 + 128 * 32 + 256 * 128 = 61,440. (With 96 for all,
-// loads of the second stage were spilled, which waits for each: 1077 us for 2.4 M rows of 100 x 128.)
-constexpr int kIssuerRegs = 32, kProducerRegs = 128;
+// Registers per thread: 72 at the launch (896 threads take 64,512), where the producers stay; the epilogue, whose lanes hold 64
+// sums each, takes 24 more each from the group of the issuing warp: 256 * 96 + 128 * 24 + 512 * 72 = 64,512. (Eight producer
+// warps with two stages of loads in 128 registers each left the chip idle between their dependent instructions: 400,000 rows
+// of 100 x 128 fp32 115 us; with 96 registers for all of them, loads were spilled, which waits for each: 202 us.)
+constexpr int kIssuerRegs = 24, kEpilogueRegs = 96;
 constexpr int kMaxStages = 4;
-constexpr int kSmemBudget = 220 * 1024;
+constexpr int kSmemBudget = 216 * 1024;
 
 struct R8Args {
   const uint8_t *codes, *scales;
@@ -72,36 +73,35 @@ __device__ __forceinline__ uint32_t two_values(uint32_t word, __nv_bfloat162 sca
   return out;
 }
 
-// hi, mid and lo of 8 fp32 values, as 8 bf16 each. Cutting instead of rounding keeps the sum exact (8 bits each). Infinities and
-// NaN go into hi alone (what is left of them would be NaN).
-__device__ __forceinline__ void three_parts(const float (&v)[8], uint32_t (&hi)[4], uint32_t (&mid)[4], uint32_t (&lo)[4]) {
-  uint32_t h[8];
-  float r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    h[i] = __float_as_uint(v[i]) & 0xffff0000u;
-    r[i] = v[i] - __uint_as_float(h[i]);
-  }
-  // a rest that is NaN: a value that is not finite (the rests themselves are far too small to add up to an infinity)
-  const float any = ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
-  if (any != any) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if ((h[i] & 0x7f800000u) == 0x7f800000u) r[i] = 0.f;
-      if (v[i] != v[i]) h[i] = 0x7fc00000u;
-    }
-  }
+// hi, mid and lo of 8 fp32 values (four pairs), as 8 bf16 each. Cutting instead of rounding keeps the sum exact (8 bits each).
+// Infinities and NaN go into hi alone (what is left of them would be NaN).
+__device__ __forceinline__ void three_parts(const Pair (&v)[4], uint32_t (&hi)[4], uint32_t (&mid)[4], uint32_t (&lo)[4]) {
+  const Pair minus = pair(-1.f, -1.f);
+  auto upper = [](Pair p) { return static_cast<Pair>(p & 0xffff0000ffff0000ull); };
+  Pair h[4], r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t m[2], l[2];
+    h[i] = upper(v[i]);
+    r[i] = fma2(h[i], minus, v[i]);
+  }
+  // a rest that is NaN: a value that is not finite (the rests themselves are far too small to add up to an infinity)
+  const float any = sum2(add2(add2(r[0], r[1]), add2(r[2], r[3])));
+  if (any != any) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      m[j] = __float_as_uint(r[2 * i + j]) & 0xffff0000u;
-      l[j] = __float_as_uint(r[2 * i + j] - __uint_as_float(m[j]));
+    for (int i = 0; i < 4; ++i) {
+      float2 f = halves(v[i]), a = halves(h[i]), b = halves(r[i]);
+      if ((__float_as_uint(f.x) & 0x7f800000u) == 0x7f800000u) a.x = f.x != f.x ? __uint_as_float(0x7fc00000u) : f.x, b.x = 0.f;
+      if ((__float_as_uint(f.y) & 0x7f800000u) == 0x7f800000u) a.y = f.y != f.y ? __uint_as_float(0x7fc00000u) : f.y, b.y = 0.f;
+      h[i] = pair(a.x, a.y), r[i] = pair(b.x, b.y);
     }
-    hi[i] = __byte_perm(h[2 * i], h[2 * i + 1], 0x7632);
-    mid[i] = __byte_perm(m[0], m[1], 0x7632);
-    lo[i] = __byte_perm(l[0], l[1], 0x7632);
+  }
+  auto pack = [](Pair p) { return __byte_perm(static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32), 0x7632); };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const Pair m = upper(r[i]);
+    hi[i] = pack(h[i]);
+    mid[i] = pack(m);
+    lo[i] = pack(fma2(m, minus, r[i]));
   }
 }
 
@@ -149,124 +149,128 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
 
   if (warp >= kFirstProd) {
     // ================= producers =================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+    // Every thread has a unit of 16 codes and one or two of 8 values of dy per stage. What it has loaded of the next stage
+    // replaces a unit as soon as this one is written, so that a load has a whole stage's time to arrive.
     constexpr int kThr = 32 * kProdWarps;
-    constexpr int kXUnits = kPos * 8 / kThr;                // 16 codes each
-    constexpr int kUnitsPerRow = 8 * SPANS;                 // of dy: 8 values each
+    constexpr int kUnitsPerRow = 8 * SPANS;                 // of dy
     constexpr int kGUnits = kPos * kUnitsPerRow / kThr;
+    constexpr int kGRows = kThr / kUnitsPerRow;             // rows from a thread's unit to its next
+    static_assert(kPos * 8 == kThr, "a unit of codes per thread");
     const int pt = tid - 32 * kFirstProd;
-    const int xu = pt & 7, gu = pt % kUnitsPerRow;
+    const int xu = pt & 7, gu = pt % kUnitsPerRow, xrow = pt >> 3, grow = pt / kUnitsPerRow;
     const int xcol = x_at + xu * 16, gcol = g_at + gu * 8;
     const bool x_in = xcol < a.pitch;
-    struct Raw {
-      uint4 codes[kXUnits];
-      uint32_t scale[kXUnits];
-      uint32_t dy[kGUnits][sizeof(T) == 4 ? 8 : 4];
-    };
-    auto load = [&](int64_t tile, Raw &r) {
-#pragma unroll
-      for (int j = 0; j < kXUnits; ++j) {
-        const int64_t row = tile * kPos + (pt >> 3) + j * (kThr / 8);
-        r.codes[j] = make_uint4(0, 0, 0, 0);
-        r.scale[j] = 0;
-        if (x_in && tile < tile_hi && row < a.m) {
-          r.codes[j] = __ldg(reinterpret_cast<const uint4 *>(a.codes + row * a.pitch + xcol));
-          r.scale[j] = __ldg(a.scales + row * a.groups + xcol / kGroup);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kGUnits; ++j) {
-        const int64_t row = tile * kPos + pt / kUnitsPerRow + j * (kThr / kUnitsPerRow);
-        constexpr int W = sizeof(T) == 4 ? 8 : 4;
-#pragma unroll
-        for (int i = 0; i < W; ++i) r.dy[j][i] = 0;
-        if (tile >= tile_hi || row >= a.m) continue;
-        const T *p = static_cast<const T *>(a.dy) + row * a.ld + gcol;
-        if constexpr (VEC) {
-#pragma unroll
-          for (int i = 0; i < W; i += 4)
-            if (gcol + i < a.n) {
-              const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p + i));
-              r.dy[j][i] = v.x, r.dy[j][i + 1] = v.y, r.dy[j][i + 2] = v.z, r.dy[j][i + 3] = v.w;
-            }
-        } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (gcol + i < a.n) r.dy[j][i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (gcol + i < a.n) r.dy[j][i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(p) + i)) << (16 * (i & 1));
-        }
+    const int64_t row_end = tile_hi * kPos < a.m ? tile_hi * kPos : a.m;  // of this block
+    int64_t row = tile_lo * kPos;                                         // first of the stage that is loaded
+    const uint8_t *codes = a.codes + (row + xrow) * a.pitch + xcol, *scales = a.scales + (row + xrow) * a.groups + xcol / kGroup;
+    const T *dy = static_cast<const T *>(a.dy) + (row + grow) * a.ld + gcol;
+    uint4 rc;
+    uint32_t rs;
+    constexpr int W = sizeof(T) == 4 ? 8 : 4;
+    uint32_t rg[kGUnits][W];
+    auto load_codes = [&]() {
+      rc = make_uint4(0, 0, 0, 0);
+      rs = 0;
+      if (x_in && row + xrow < row_end) {
+        rc = __ldg(reinterpret_cast<const uint4 *>(codes));
+        rs = __ldg(scales);
       }
     };
-    float db[8] = {};
-    auto put = [&](const Raw &r, uint32_t stage) {
+    auto load_dy = [&](int j) {
 #pragma unroll
-      for (int j = 0; j < kXUnits; ++j) {
-        const int row = (pt >> 3) + j * (kThr / 8);
-        const __nv_bfloat162 s = __float2bfloat162_rn(rows8::scale_of(r.scale[j]));
-        const uint32_t w[4] = {r.codes[j].x, r.codes[j].y, r.codes[j].z, r.codes[j].w};
-        uint32_t v[8];
+      for (int i = 0; i < W; ++i) rg[j][i] = 0;
+      if (row + grow + j * kGRows >= row_end) return;
+      const T *p = dy + static_cast<int64_t>(j * kGRows) * a.ld;
+      if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[2 * i] = two_values<0>(w[i], s), v[2 * i + 1] = two_values<1>(w[i], s);
-        const uint32_t span = stage + (xu >> 2) * kSpan;
-        const int c = (xu & 3) * 2, odd = xu >> 2;  // the second span's lanes start with their odd chunk: other banks
-        const uint32_t first = span + swizzled_offset<false>(row, c + odd), second = span + swizzled_offset<false>(row, c + 1 - odd);
-        if (odd) {
-          st_shared16(first, v[4], v[5], v[6], v[7]);
-          st_shared16(second, v[0], v[1], v[2], v[3]);
-        } else {
-          st_shared16(first, v[0], v[1], v[2], v[3]);
-          st_shared16(second, v[4], v[5], v[6], v[7]);
-        }
+        for (int i = 0; i < W; i += 4)
+          if (gcol + i < a.n) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p + i));
+            rg[j][i] = v.x, rg[j][i + 1] = v.y, rg[j][i + 2] = v.z, rg[j][i + 3] = v.w;
+          }
+      } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (gcol + i < a.n) rg[j][i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (gcol + i < a.n) rg[j][i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(p) + i)) << (16 * (i & 1));
       }
+    };
+    auto onward = [&]() {
+      row += kPos;
+      codes += static_cast<int64_t>(kPos) * a.pitch;
+      scales += static_cast<int64_t>(kPos) * a.groups;
+      dy += static_cast<int64_t>(kPos) * a.ld;
+    };
+    // where a unit goes, from the start of a stage
+    const int odd = xu >> 2;  // the second span's lanes start with their odd chunk: other banks
+    const uint32_t x_first = (xu >> 2) * kSpan + swizzled_offset<false>(xrow, (xu & 3) * 2 + odd);
+    const uint32_t x_second = (xu >> 2) * kSpan + swizzled_offset<false>(xrow, (xu & 3) * 2 + 1 - odd);
+    const uint32_t g_first = (2 + (gu >> 3)) * kSpan + swizzled_offset<false>(grow, gu & 7);
+    static_assert(kGRows % 8 == 0, "the swizzle repeats every eight rows");
+    Pair db[4] = {};
+    auto put_codes = [&](uint32_t stage) {
+      const __nv_bfloat162 s = __float2bfloat162_rn(rows8::scale_of(rs));
+      const uint32_t w[4] = {rc.x, rc.y, rc.z, rc.w};
+      uint32_t v[8];
 #pragma unroll
-      for (int j = 0; j < kGUnits; ++j) {
-        const int row = pt / kUnitsPerRow + j * (kThr / kUnitsPerRow);
-        const uint32_t at = stage + (2 + (gu >> 3)) * kSpan + swizzled_offset<false>(row, gu & 7);
-        if constexpr (sizeof(T) == 4) {
-          float v[8];
-          uint32_t hi[4], mid[4], lo[4];
+      for (int i = 0; i < 4; ++i) v[2 * i] = two_values<0>(w[i], s), v[2 * i + 1] = two_values<1>(w[i], s);
+      st_shared16(stage + (odd ? x_second : x_first), v[0], v[1], v[2], v[3]);
+      st_shared16(stage + (odd ? x_first : x_second), v[4], v[5], v[6], v[7]);
+    };
+    auto put_dy = [&](int j, uint32_t stage) {
+      const uint32_t at = stage + g_first + j * kGRows * 128;
+      if constexpr (sizeof(T) == 4) {
+        Pair v[4];
+        uint32_t hi[4], mid[4], lo[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.dy[j][i]), db[i] += v[i];
-          three_parts(v, hi, mid, lo);
-          st_shared16(at, hi[0], hi[1], hi[2], hi[3]);
-          st_shared16(at + SPANS * kSpan, mid[0], mid[1], mid[2], mid[3]);
-          st_shared16(at + 2 * SPANS * kSpan, lo[0], lo[1], lo[2], lo[3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) db[i] += __uint_as_float(i & 1 ? r.dy[j][i / 2] & 0xffff0000u : r.dy[j][i / 2] << 16);
-          st_shared16(at, r.dy[j][0], r.dy[j][1], r.dy[j][2], r.dy[j][3]);
+        for (int i = 0; i < 4; ++i) {
+          v[i] = pair(__uint_as_float(rg[j][2 * i]), __uint_as_float(rg[j][2 * i + 1]));
+          db[i] = add2(db[i], v[i]);
         }
+        three_parts(v, hi, mid, lo);
+        st_shared16(at, hi[0], hi[1], hi[2], hi[3]);
+        st_shared16(at + SPANS * kSpan, mid[0], mid[1], mid[2], mid[3]);
+        st_shared16(at + 2 * SPANS * kSpan, lo[0], lo[1], lo[2], lo[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          db[i] = add2(db[i], pair(__uint_as_float(rg[j][i] << 16), __uint_as_float(rg[j][i] & 0xffff0000u)));
+        st_shared16(at, rg[j][0], rg[j][1], rg[j][2], rg[j][3]);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
     Ring ring(a.stages);
-    bool alive = true;
-    auto hand_over = [&](const Raw &r) {
+    load_codes();
+#pragma unroll
+    for (int j = 0; j < kGUnits; ++j) load_dy(j);
+    for (int64_t tile = tile_lo; tile < tile_hi; ++tile) {
       const int s = ring.stage;
-      if (ring.reused()) alive = wait_bar(&bars.empty[s], ring.emptied(), abort_flag, a.status, a.wait_cycles);
-      if (!alive) return;
-      put(r, base + static_cast<uint32_t>(s) * kStageBytes);
+      if (ring.reused() && !wait_bar(&bars.empty[s], ring.emptied(), abort_flag, a.status, a.wait_cycles)) break;
+      const uint32_t stage = base + static_cast<uint32_t>(s) * kStageBytes;
+      onward();
+      put_codes(stage);
+      load_codes();
+#pragma unroll
+      for (int j = 0; j < kGUnits; ++j) {
+        put_dy(j, stage);
+        load_dy(j);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       if (!(a.test_stall && ring.round == 0 && s == 0)) mbar_arrive(&bars.full[s]);
       ring.next();
-    };
-    Raw one, two;
-    load(tile_lo, one);
-    for (int64_t tile = tile_lo; tile < tile_hi && alive; tile += 2) {
-      load(tile + 1, two);
-      hand_over(one);
-      if (!alive || tile + 1 >= tile_hi) break;
-      load(tile + 2, one);
-      hand_over(two);
     }
     if (a.partial_db != nullptr && x_at == 0) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
+        float2 t = halves(db[i]);
 #pragma unroll
-        for (int o = kUnitsPerRow; o < 32; o <<= 1) db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
-        if (lane < kUnitsPerRow) db_side[warp - kFirstProd][gu * 8 + i] = db[i];
+        for (int o = kUnitsPerRow; o < 32; o <<= 1) {
+          t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
+          t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
+        }
+        if (lane < kUnitsPerRow) db_side[warp - kFirstProd][gu * 8 + 2 * i] = t.x, db_side[warp - kFirstProd][gu * 8 + 2 * i + 1] = t.y;
       }
       asm volatile("bar.sync 1, %0;" ::"n"(32 * kProdWarps) : "memory");
       if (pt < kCols && g_at + pt < a.n) {
@@ -325,6 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
     }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
     // ================= epilogue: lane = column of the input, half of the columns of dy per four warps =================
     constexpr int kHalf = kCols / 2;
     float acc[kHalf];
