@@ -804,7 +804,8 @@ at::ScalarType row_type(const std::string &who, at::ScalarType t) {
   return t;
 }
 
-Tensor dequantize(const Tensor &codes, const Tensor &scales, int64_t width, const optional<Tensor> &index, at::ScalarType type) {
+Tensor dequantize(const Tensor &codes, const Tensor &scales, int64_t width, const optional<Tensor> &index, at::ScalarType type,
+                  int64_t num_rows) {
   row_type("dequantize_rows", type);
   c10::cuda::CUDAGuard guard(codes.device());
   const int64_t rows = codes.size(0) - 1;
@@ -813,7 +814,8 @@ Tensor dequantize(const Tensor &codes, const Tensor &scales, int64_t width, cons
     same_device(codes, *index, "index");
     if (index->dim() != 1) fail("dequantize_rows: index must be a vector");
   }
-  Tensor out = at::empty({index ? index->size(0) : rows, width}, codes.options().dtype(type));
+  if (num_rows < 0 || num_rows > rows) fail("dequantize_rows: " + std::to_string(num_rows) + " rows of " + std::to_string(rows));
+  Tensor out = at::empty({index ? index->size(0) : num_rows, width}, codes.options().dtype(type));
   check(lib.cxg_rows8_read(codes.data_ptr(), scales.data_ptr(), rows, static_cast<int>(width),
                            index ? index->data_ptr<int64_t>() : nullptr, out.size(0), out.data_ptr(), code_of(out), width,
                            stream_of(codes)),
@@ -948,7 +950,7 @@ Tensor linear_kept8(Tensor x, Tensor w, optional<Tensor> bias, optional<Tensor> 
   if (add) same_device(x, *add, "add");
   if (codes) {
     same_device(x, *codes, "kept");
-    if (codes->size(0) - 1 != x.size(0) || codes->size(1) != lib.cxg_rows8_pitch(static_cast<int>(x.size(1))))
+    if (codes->size(0) - 1 < x.size(0) || codes->size(1) != lib.cxg_rows8_pitch(static_cast<int>(x.size(1))))
       fail("linear_kept8: kept must hold the rows of x");
   }
   c10::cuda::CUDAGuard guard(x.device());

@@ -3,6 +3,8 @@
 `cxgnncomp_backend` module next to this package, which calls the sm_100a library."""
 from cxgnncomp_backend import (edge_attention, sage_sum_forward_edge_value, gather, sage_sum_forward, aggr_rel,
                                sage_mean_forward, rel_schedule, target_aggr)
+from cxgnncomp_backend import (Rows8, quantize_rows, dequantize_rows, rows8_aggregate, rows8_weight_grad, linear_kept8,
+                               residual_norm)
 
 from .schedule import (neighbor_grouping, neighbor_grouping_gpu, partition_2d, reorder_by, remove_from_graph,
                        remove_from_graph_by_edge)
@@ -13,7 +15,7 @@ from .graph_kernel import SpMMValOP
 from .typed_linear import (TypedLinearE2EOP, TypedLinearS2EOP, TypedLinearS2DMMAggrOP, TypedLinearS2DAggrMMOP,
                            TypedLinearS2DSort, TypedLinearNaiveS2D, TypedLinearS2DPushOP, SelectMMS2EOP)
 from .codegen import typed_matmul, spmm_torch, Tuner, compare, prof
-from .model import SAGE, GCN, GAT, GIN, RGCN, GNN, get_conv_from_str, get_model_from_str
+from .model import SAGE, GCN, GAT, GIN, RGCN, GNN, ResidualGNN, get_conv_from_str, get_model_from_str
 from .batch import Batch
 from .sampler import NeighborSampler
 from .neighbor_lstm import NeighborLstmOneByOneOP, NeighborLstmOP, NeighborLstmPadOP

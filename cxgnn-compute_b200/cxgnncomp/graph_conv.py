@@ -79,10 +79,15 @@ class AggrDirectedOP(torch.autograd.Function):
 
 
 class MySageConv(torch.nn.Module):
-    """GraphSAGE, mean aggregator (graph_conv.py:117-159)."""
+    """GraphSAGE, mean aggregator (graph_conv.py:117-159). Not in the reference: x may be a cxgnncomp_backend.Rows8 (features
+    held in 8 bits, constants); with kept8 the backward pass keeps what the two transforms read in 8 bits instead of the
+    matrices (the weights' gradients are those of the rows in 8 bits, all others as without)."""
 
-    def __init__(self, in_channels, hidden_channels, root_weight=True, bias=True):
+    kept8 = False  # of modules that were saved without it
+
+    def __init__(self, in_channels, hidden_channels, root_weight=True, bias=True, kept8=False):
         super().__init__()
+        self.kept8 = kept8
         self.in_channels = in_channels
         self.hidden_channels = hidden_channels
         self.root_weight = root_weight
@@ -96,7 +101,12 @@ class MySageConv(torch.nn.Module):
         if self.root_weight:
             self.lin_r.reset_parameters()
 
-    def forward(self, x, ptr, idx, num_node):
+    def forward(self, x, ptr, idx, num_node, kept=None):
+        """kept: a Rows8 of x, where the caller has one (for kept8)."""
+        if isinstance(x, cxgnncomp_backend.Rows8):
+            return self._forward_rows8(x, ptr, idx, num_node)
+        if self.kept8 and _plain(self.lin_l) and (not self.root_weight or _plain(self.lin_r)):
+            return self._forward_kept8(x, ptr, idx, num_node, kept)
         if self.root_weight and _plain(self.lin_l) and _plain(self.lin_r):
             out = cxgnncomp_backend.sage_layer(x, ptr, idx, self.lin_l.weight, self.lin_r.weight, self.lin_l.bias, num_node,
                                                self.in_channels <= self.hidden_channels)
@@ -110,6 +120,31 @@ class MySageConv(torch.nn.Module):
             root = x[:num_node] if num_node not in (0, x.shape[0]) else x
             out = self.lin_r(root, add=out) if isinstance(self.lin_r, Linear) else out + self.lin_r(root)
         return out
+
+
+    def _root(self, rows, ptr, num_node):
+        """How many rows the layer has."""
+        return num_node if num_node > 0 else min(rows, ptr.shape[0] - 1)
+
+    def _forward_rows8(self, rows, ptr, idx, num_node):
+        n, dtype = self._root(rows.rows, ptr, num_node), self.lin_l.weight.dtype
+        mean = cxgnncomp_backend.rows8_aggregate(rows, ptr, idx, n, reduce="mean", dtype=dtype)
+        root = cxgnncomp_backend.dequantize_rows(rows, num_rows=n, dtype=dtype) if self.root_weight else None
+        if self.kept8 and _plain(self.lin_l) and (not self.root_weight or _plain(self.lin_r)):
+            out = cxgnncomp_backend.linear_kept8(mean, self.lin_l.weight, self.lin_l.bias)
+            return out if root is None else cxgnncomp_backend.linear_kept8(root, self.lin_r.weight, add=out, kept=rows)
+        out = self.lin_l(mean)
+        return out if root is None else self.lin_r(root, add=out) if isinstance(self.lin_r, Linear) else out + self.lin_r(root)
+
+    def _forward_kept8(self, x, ptr, idx, num_node, kept):
+        linear = cxgnncomp_backend.linear_kept8
+        if self.in_channels > self.hidden_channels:
+            out = sage_mean_forward(linear(x, self.lin_l.weight, self.lin_l.bias, kept=kept), ptr, idx, num_node)
+        else:
+            out = linear(sage_mean_forward(x, ptr, idx, num_node), self.lin_l.weight, self.lin_l.bias)
+        if not self.root_weight:
+            return out
+        return linear(x[:out.shape[0]], self.lin_r.weight, add=out, kept=kept)
 
 
 class MyGINConv(torch.nn.Module):

@@ -557,7 +557,9 @@ def sample_batch(graph_ptr, graph_idx, seeds, fanouts, seed, local_of, marks, ho
 
 
 def take_rows(x, rows):
-    """x[rows] for a 2-D x: one gathering kernel where no gradient is asked for."""
+    """x[rows] for a 2-D x: one gathering kernel where no gradient is asked for. x may be a Rows8: its values in float32."""
+    if isinstance(x, Rows8):
+        return dequantize_rows(x, rows)
     if (isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2 and x.is_contiguous() and not x.requires_grad
             and x.element_size() % 2 == 0):
         return _native.gather_rows(x, rows)

@@ -80,10 +80,13 @@ def quantize_rows(x, out=None, index=None):
     return out
 
 
-def dequantize_rows(rows, index=None, dtype=torch.float32):
-    """The values of the rows, or of rows[index[i]] (int64 [n]; ids outside the rows give zeros), in float32 or bfloat16."""
+def dequantize_rows(rows, index=None, dtype=torch.float32, num_rows=None):
+    """The values of all rows, of the first num_rows, or of rows[index[i]] (int64 [n]; ids outside the rows give zeros), in
+    float32 or bfloat16."""
     _rows8(rows, "dequantize_rows")
-    return _native.rows8_dequantize(rows.codes, rows.scales, rows.width, index, dtype)
+    if index is not None and num_rows is not None:
+        raise RuntimeError("dequantize_rows: either an index or a number of rows")
+    return _native.rows8_dequantize(rows.codes, rows.scales, rows.width, index, dtype, rows.rows if num_rows is None else int(num_rows))
 
 
 def rows8_aggregate(rows, ptr, idx, num_node, reduce="sum", edge_value=None, dtype=torch.float32):
@@ -109,8 +112,8 @@ def rows8_weight_grad(rows, grad, bias=False):
 def linear_kept8(x, weight, bias=None, add=None, kept=None):
     """x @ weight^T (+ bias) (+ add) for x [n, in] and weight [out, in], all float32 or all bfloat16, whose backward pass keeps x
     in 8 bits instead of x itself: result and x's gradient are those of `linear`, the weight's gradient that of the rows in 8
-    bits. kept: x in 8 bits where the caller has it already (it must not be written before the backward pass). Once
-    differentiable."""
+    bits. kept: rows in 8 bits whose first n are x, where the caller has them already (not to be written before the backward
+    pass). Once differentiable."""
     if kept is not None:
         _rows8(kept, "linear_kept8")
         if kept.width != x.shape[-1]:

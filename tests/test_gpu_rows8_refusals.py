@@ -26,6 +26,8 @@ def test_rows(cuda):
     _raises("matrix", lambda: be.quantize_rows(x[:, :0]))
     _raises("CUDA", lambda: be.quantize_rows(x, out=rows, index=at.cpu()))
     _raises("dtype", lambda: be.dequantize_rows(rows, dtype=torch.float16))
+    _raises("9 rows of 8", lambda: be.dequantize_rows(rows, num_rows=9))
+    _raises("either", lambda: be.dequantize_rows(rows, index=at, num_rows=3))
     _raises("bad sizes", lambda: be.Rows8(-1, 4))
     _raises("bad sizes", lambda: be.Rows8(4, 0))
     _raises("transform", lambda: torch.vmap(lambda t: be.quantize_rows(t).codes)(randn((3, 4, 32), 1).cuda()))
@@ -62,7 +64,7 @@ def test_linear_and_weight_grad(cuda):
     _raises("weight must be", lambda: lin(x, w[:, :31]))
     _raises("bias must be", lambda: lin(x, w, randn((9,), 1).cuda()))
     _raises("shape of the result", lambda: lin(x, w, add=randn((10, 9), 1).cuda()))
-    _raises("rows of x", lambda: lin(x[:9], w, kept=rows))
+    _raises("rows of x", lambda: lin(x, w, kept=be.quantize_rows(x[:9])))
     _raises("rows of x", lambda: lin(x, w, kept=be.Rows8(10, 40)))
     _raises("CUDA", lambda: lin(x, w.cpu()))
     with torch.autocast("cuda", dtype=torch.float16):
