@@ -855,23 +855,24 @@ Tensor rows8_aggregate(const Tensor &codes, const Tensor &scales, int64_t width,
   return y;
 }
 
-// (dy^T . rows [n, width], column sums of dy [n] or none), fp32
-std::pair<Tensor, Tensor> rows8_weight_grad(const Tensor &codes, const Tensor &scales, int64_t width, const Tensor &dy_in, bool bias) {
+// (dy^T . rows [n, width], column sums of dy [n] or none), summed in fp32
+std::pair<Tensor, Tensor> rows8_weight_grad(const Tensor &codes, const Tensor &scales, int64_t width, const Tensor &dy_in, bool bias,
+                                            at::ScalarType type) {
   if (for_torch(dy_in)) fail(std::string("rows8_weight_grad") + kTransform);
   const Tensor dy = row_matrix(dy_in, "grad");
   same_device(codes, dy, "grad");
   const int64_t m = dy.size(0), n = dy.size(1);
   if (m > codes.size(0) - 1) fail("rows8_weight_grad: grad has " + std::to_string(m) + " rows, there are " + std::to_string(codes.size(0) - 1));
   c10::cuda::CUDAGuard guard(dy.device());
-  const auto opt = dy.options().dtype(at::kFloat);
+  const auto opt = dy.options().dtype(type);
   Tensor dw = at::empty({n, width}, opt), db = bias ? at::empty({n}, opt) : Tensor();
   size_t need = 0;
   check(lib.cxg_rows8_wgrad_workspace_size(m, static_cast<int>(width), static_cast<int>(n), &need), "cxg_rows8_wgrad_workspace_size");
   void *st = stream_of(dy);
   const Workspace ws = workspace_on(dy.device().index(), st, static_cast<int64_t>(need), "");
   check(lib.cxg_rows8_wgrad(codes.data_ptr(), scales.data_ptr(), m, static_cast<int>(width), dy.data_ptr(), code_of(dy), row_step(dy),
-                            static_cast<int>(n), 0, dw.data_ptr<float>(), bias ? db.data_ptr<float>() : nullptr, ws.data(),
-                            ws.bytes(), st),
+                            static_cast<int>(n), 0, dw.data_ptr(), bias ? db.data_ptr() : nullptr, code_of(dw), ws.data(), ws.bytes(),
+                            st),
         "cxg_rows8_wgrad");
   return {dw, db};
 }
@@ -896,7 +897,6 @@ class LinearKept8Function : public torch::autograd::Function<LinearKept8Function
       held = quantize(x);
     ctx->save_for_backward({w, held.codes, held.scales});
     ctx->saved_data["bias"] = bias.has_value();
-    ctx->saved_data["bias_bf16"] = bias && bias->scalar_type() == at::kBFloat16;
     ctx->saved_data["add"] = add.has_value();
     return plain_linear(x, w, bias, add);
   }
@@ -915,13 +915,12 @@ class LinearKept8Function : public torch::autograd::Function<LinearKept8Function
                ? linear_product(g, w, true, c10::nullopt, c10::nullopt)
                : at::mm(g, w);
     if (ctx->needs_input_grad(1)) {
-      const auto grad = rows8_weight_grad(saved[1], saved[2], w.size(1), g, need_db);
-      dw = grad.first.to(w.scalar_type());
+      const auto grad = rows8_weight_grad(saved[1], saved[2], w.size(1), g, need_db, w.scalar_type());
+      dw = grad.first;
       db = grad.second;
     } else if (need_db) {
-      db = g.sum(0, false, at::kFloat);
+      db = g.sum(0, false, at::kFloat).to(g.scalar_type());
     }
-    if (need_db) db = db.to(ctx->saved_data["bias_bf16"].toBool() ? at::kBFloat16 : at::kFloat);
     return {dx, dw, db, need_add ? grads[0] : Tensor(), Tensor(), Tensor()};
   }
 };
@@ -1517,7 +1516,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rows8_dequantize", &dequantize);
   m.def("rows8_aggregate", &rows8_aggregate);
   m.def("rows8_weight_grad", [](const Tensor &codes, const Tensor &scales, int64_t width, const Tensor &dy, bool bias) {
-    const auto g = rows8_weight_grad(codes, scales, width, dy, bias);
+    const auto g = rows8_weight_grad(codes, scales, width, dy, bias, at::kFloat);
     return std::make_pair(g.first, bias ? optional<Tensor>(g.second) : c10::nullopt);
   });
   m.def("linear_kept8", &linear_kept8);

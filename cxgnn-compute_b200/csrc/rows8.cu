@@ -1,9 +1,10 @@
 // Writing and reading rows in 8 bits (rows8.cuh has the format): activations that a backward pass needs again, and caches of
 // features or of hidden states that are written and read by node id.
 //
-// Both directions are bound by memory as long as they spend few instructions: a lane takes 8 values, so four lanes share a
-// group of 32 and find its largest value in two shuffles, and what an item costs by itself (its row and place, the row's
-// target, the address) is spread over these. Lanes go along rows without regard to where these end, so that none is idle for
+// Both directions are bound by memory as long as they spend few instructions and have enough of it on the way: a lane writes
+// from 32 bytes of values (8 fp32, 16 bf16: four or two lanes share a group of 32 and find its largest value in two shuffles
+// or one) and reads 16 codes, and what an item costs by itself (its row and place, the row's target, the address) is spread
+// over these. Lanes go along rows without regard to where these end, so that none is idle for
 // a width that is no power of two; items are counted in 32 bits, larger matrices go in pieces. (4 fp32 values a lane, 64-bit
 // counts and a limit on every code were 140 instructions an item and twice the time of memory: 400,000 rows of 100 fp32 38 us.)
 #include "rows8.cuh"
@@ -14,9 +15,12 @@ namespace {
 using namespace rows8;
 
 constexpr int kThreads = 256;
-constexpr int kValues = 8;                   // per item
-constexpr int kLanes = kGroup / kValues;     // of a group
-constexpr int kItems = 4;                    // per thread
+template <typename T>
+constexpr int kWritten = 32 / static_cast<int>(sizeof(T));  // values of an item that is written
+template <typename T>
+constexpr int kSharing = kGroup / kWritten<T>;              // lanes of a group
+constexpr int kRead = 16;                                   // codes of an item that is read
+constexpr int kItems = 4;                                   // per thread
 constexpr uint32_t kMostItems = 1u << 31;    // per launch
 
 // Items of rows that have `per` each. The quotient by floor(2^32 / per) is at most one too small.
@@ -32,14 +36,14 @@ struct Items {
 // How the wide side is accessed: value by value, in 16-byte vectors, in 32-byte ones.
 enum Access { kScalar, kVector, kWide };
 
-__device__ __forceinline__ void load32(float (&f)[8], const float *p) {
-  asm("ld.global.nc.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-      : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7])
+__device__ __forceinline__ void load32(uint32_t (&w)[8], const void *p) {
+  asm("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
       : "l"(p));
 }
-__device__ __forceinline__ void store32(float *p, const float (&f)[8]) {
-  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]),
-               "f"(f[5]), "f"(f[6]), "f"(f[7])
+__device__ __forceinline__ void store32(void *p, const uint32_t *w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+               "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
 
@@ -50,53 +54,42 @@ __device__ __forceinline__ float top_of(float a, float b) {
   return r;
 }
 
-// 8 values of a row from column c on as they were loaded; zeros behind the row.
+// The values of a row from column c on as they were loaded; zeros behind the row.
 template <typename T, Access A>
 struct Loaded {
-  float f[sizeof(T) == 4 ? 8 : 1];
-  uint32_t h[sizeof(T) == 4 ? 1 : 4];
+  static constexpr int V = kWritten<T>;
+  uint32_t w[8];
   __device__ __forceinline__ void load(const T *row, uint32_t c, uint32_t width, bool in) {
-    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = 0.f;
-      if (!in) return;
-      if constexpr (A == kWide) {
-        if (c < width) load32(f, row + c);
-      } else if constexpr (A == kVector) {
+    for (int i = 0; i < 8; ++i) w[i] = 0;
+    if (!in) return;
+    if constexpr (A == kWide) {
+      if (c < width) load32(w, row + c);
+    } else if constexpr (A == kVector) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 4)
-          if (c + i < width) {
-            const float4 t = __ldg(reinterpret_cast<const float4 *>(row + c + i));
-            f[i] = t.x, f[i + 1] = t.y, f[i + 2] = t.z, f[i + 3] = t.w;
-          }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c + i < width) f[i] = __ldg(row + c + i);
-      }
+      for (int i = 0; i < 2; ++i)
+        if (c + i * (V / 2) < width) {
+          const uint4 t = __ldg(reinterpret_cast<const uint4 *>(row + c + i * (V / 2)));
+          w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
+        }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = 0;
-      if (!in) return;
-      if constexpr (A != kScalar) {
-        if (c < width) {
-          const uint4 t = __ldg(reinterpret_cast<const uint4 *>(row + c));
-          h[0] = t.x, h[1] = t.y, h[2] = t.z, h[3] = t.w;
+      for (int i = 0; i < V; ++i)
+        if (c + i < width) {
+          if constexpr (sizeof(T) == 4)
+            w[i] = __ldg(reinterpret_cast<const uint32_t *>(row) + c + i);
+          else
+            w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(row) + c + i)) << (16 * (i & 1));
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c + i < width) h[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(row) + c + i)) << (16 * (i & 1));
-      }
     }
   }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
+  __device__ __forceinline__ void get(float (&v)[V]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < V; ++i)
       if constexpr (sizeof(T) == 4)
-        v[i] = f[i];
+        v[i] = __uint_as_float(w[i]);
       else
-        v[i] = __uint_as_float(i & 1 ? h[i / 2] & 0xffff0000u : h[i / 2] << 16);
+        v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
   }
 };
 
@@ -105,8 +98,9 @@ struct Loaded {
 template <typename T, Access A>
 __global__ void __launch_bounds__(kThreads) rows8_write(const T *x, int64_t ld, uint32_t n, uint32_t width, Items items, uint8_t *codes,
                                                         uint8_t *scales, const int64_t *to, int32_t *owner) {
+  constexpr int V = kWritten<T>, L = kSharing<T>;
   dependency_wait();
-  const uint32_t groups = items.per / kLanes, first = blockIdx.x * (kThreads * kItems) + threadIdx.x;
+  const uint32_t groups = items.per / L, first = blockIdx.x * (kThreads * kItems) + threadIdx.x;
   Loaded<T, A> in[kItems];
   int64_t dst[kItems];
   uint32_t chunk[kItems];
@@ -118,22 +112,28 @@ __global__ void __launch_bounds__(kThreads) rows8_write(const T *x, int64_t ld, 
     const bool have = i < items.total, of_x = have && row < n;
     dst[k] = have ? static_cast<int64_t>(row) : int64_t{-1};
     if (to != nullptr && of_x) dst[k] = __ldg(to + row);
-    in[k].load(x + (of_x ? row : 0) * ld, chunk[k] * kValues, width, of_x);
+    in[k].load(x + (of_x ? row : 0) * ld, chunk[k] * V, width, of_x);
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    float v[8];
+    float v[V];
     in[k].get(v);
-    float top = top_of(top_of(top_of(v[0], v[1]), top_of(v[2], v[3])), top_of(top_of(v[4], v[5]), top_of(v[6], v[7])));
+    float top = top_of(v[0], v[1]);
 #pragma unroll
-    for (int d = 1; d < kLanes; d <<= 1) top = top_of(top, __shfl_xor_sync(0xffffffffu, top, d));
+    for (int j = 2; j < V; j += 2) top = top_of(top, top_of(v[j], v[j + 1]));
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) top = top_of(top, __shfl_xor_sync(0xffffffffu, top, d));
     const uint32_t e = scale_byte(__float_as_uint(top));
-    uint32_t w[2];
-    codes_of<8>(w, v, e);
+    uint32_t w[V / 4];
+    codes_of<V>(w, v, e);
     if (dst[k] >= 0) {
-      const int64_t group = dst[k] * groups + (chunk[k] / kLanes);
-      *reinterpret_cast<uint2 *>(codes + group * kGroup + (chunk[k] % kLanes) * kValues) = make_uint2(w[0], w[1]);
-      if (chunk[k] % kLanes == 0) scales[group] = static_cast<uint8_t>(e);
+      const int64_t group = dst[k] * groups + (chunk[k] / L);
+      uint8_t *out = codes + group * kGroup + (chunk[k] % L) * V;
+      if constexpr (V == 8)
+        *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
+      else
+        *reinterpret_cast<uint4 *>(out) = make_uint4(w[0], w[1], w[V / 4 - 2], w[V / 4 - 1]);
+      if (chunk[k] % L == 0) scales[group] = static_cast<uint8_t>(e);
       if (owner != nullptr && chunk[k] == 0) owner[dst[k]] = -1;
     }
   }
@@ -175,34 +175,52 @@ __global__ void __launch_bounds__(kThreads) rows8_read(const uint8_t *codes, con
       if (static_cast<uint64_t>(r) < static_cast<uint64_t>(n_rows)) src[k] = r;
     }
   }
-  uint2 w[kItems];
+  uint4 w[kItems];
   uint32_t e[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const int64_t group = src[k] * groups + (chunk[k] / kLanes);
-    w[k] = __ldg(reinterpret_cast<const uint2 *>(codes + group * kGroup + (chunk[k] % kLanes) * kValues));
+    const int64_t group = src[k] * groups + chunk[k] / (kGroup / kRead);
+    w[k] = __ldg(reinterpret_cast<const uint4 *>(codes + group * kGroup + (chunk[k] % (kGroup / kRead)) * kRead));
     e[k] = __ldg(scales + group);
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     if (first + k * kThreads >= items.total) break;
     const float s = scale_of(e[k]);
-    float f[8];
+    float f[kRead];
     code_values(f, w[k].x);
     code_values(f + 4, w[k].y);
+    code_values(f + 8, w[k].z);
+    code_values(f + 12, w[k].w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] *= s;
-    const uint32_t c = chunk[k] * kValues;
+    for (int j = 0; j < kRead; ++j) f[j] *= s;
+    const uint32_t c = chunk[k] * kRead;
     T *o = out + row[k] * ld + c;
-    if constexpr (A == kWide && sizeof(T) == 4) {
-      store32(o, f);
-    } else if constexpr (A != kScalar) {
+    if constexpr (A == kWide) {
+      constexpr int V = kWritten<T>;  // values of 32 bytes
 #pragma unroll
-      for (int j = 0; j < 8; j += Vec<T>::kElems)
+      for (int j = 0; j < kRead; j += V)
+        if (c + j < width) {
+          uint32_t v[8];
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(f[j + i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint4 t = Vec<T>::from_float(f + j + 8 * i);
+              v[4 * i] = t.x, v[4 * i + 1] = t.y, v[4 * i + 2] = t.z, v[4 * i + 3] = t.w;
+            }
+          }
+          store32(o + j, v);
+        }
+    } else if constexpr (A == kVector) {
+#pragma unroll
+      for (int j = 0; j < kRead; j += Vec<T>::kElems)
         if (c + j < width) Vec<T>::store_stream(o + j, Vec<T>::from_float(f + j));
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < kRead; ++j)
         if (c + j < width) o[j] = from_f32<T>(f[j]);
     }
   }
@@ -231,7 +249,7 @@ void launch_write(const void *x_, int64_t ld, int64_t n, int64_t n_end, int widt
                   int32_t *owner, cudaStream_t st) {
   const int groups = groups_of(width);
   const T *x = static_cast<const T *>(x_);
-  in_pieces(n_end, static_cast<uint32_t>(groups * kLanes), [&](int64_t r, int64_t rows, const Items &items, unsigned blocks) {
+  in_pieces(n_end, static_cast<uint32_t>(groups * kSharing<T>), [&](int64_t r, int64_t rows, const Items &items, unsigned blocks) {
     const int64_t have = n - r < rows ? n - r : rows, at = to != nullptr ? 0 : r;
     auto go = [&](auto kernel) {
       launch_dependent(kernel, blocks, kThreads, 0, st, x + (have > 0 ? r * ld : 0), ld, static_cast<uint32_t>(have > 0 ? have : 0),
@@ -248,7 +266,7 @@ void launch_read(const void *codes, const void *scales, int64_t n_rows, int widt
                  int64_t ld, cudaStream_t st) {
   const int groups = groups_of(width);
   T *out = static_cast<T *>(out_);
-  in_pieces(n, static_cast<uint32_t>((width + kValues - 1) / kValues), [&](int64_t r, int64_t rows, const Items &items, unsigned blocks) {
+  in_pieces(n, static_cast<uint32_t>((width + kRead - 1) / kRead), [&](int64_t r, int64_t rows, const Items &items, unsigned blocks) {
     const int64_t at = index != nullptr ? 0 : r;
     auto go = [&](auto kernel) {
       launch_dependent(kernel, blocks, kThreads, 0, st, static_cast<const uint8_t *>(codes) + at * groups * kGroup,

@@ -376,8 +376,9 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
 // dw[o][i] and db[o]: warp q of a block adds the partials q, q + 8, ... of 32 outputs, the eight sums are added in order. (A thread
 // per output and all its partials took 11 us for 148 partials of 128 x 100, a chain of loads.)
 constexpr int kJoinWarps = 8;
-__global__ void __launch_bounds__(32 * kJoinWarps) rows8_wgrad_join(const float *partial, const float *partial_db, float *dw, float *db,
-                                                                    int k, int n, int k_blocks, int parts) {
+template <typename T>
+__global__ void __launch_bounds__(32 * kJoinWarps) rows8_wgrad_join(const float *partial, const float *partial_db, T *dw, T *db, int k,
+                                                                    int n, int k_blocks, int parts) {
   dependency_wait();
   __shared__ float side[kJoinWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -409,9 +410,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) rows8_wgrad_join(const float 
 #pragma unroll
     for (int w = 1; w < kJoinWarps; ++w) s += side[w][lane];
     if (i < kn)
-      dw[i] = s;
+      dw[i] = from_f32<T>(s);
     else
-      db[i - kn] = s;
+      db[i - kn] = from_f32<T>(s);
   }
 }
 
@@ -437,17 +438,19 @@ extern "C" int cxg_rows8_wgrad_workspace_size(int64_t m, int k, int n, size_t *b
 }
 
 extern "C" int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m, int k, const void *dy, int dtype, int64_t ld, int n,
-                               uint32_t flags, float *dw, float *db, void *workspace, size_t workspace_bytes, void *stream) {
-  CXG_REQUIRE(m >= 0 && k > 0 && n > 0 && ld >= n && (dtype == CXG_F32 || dtype == CXG_BF16), CXG_EINVAL,
-              "cxg_rows8_wgrad: bad sizes or type");
+                               uint32_t flags, void *dw, void *db, int out_dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  CXG_REQUIRE(m >= 0 && k > 0 && n > 0 && ld >= n && (dtype == CXG_F32 || dtype == CXG_BF16) &&
+                  (out_dtype == CXG_F32 || out_dtype == CXG_BF16),
+              CXG_EINVAL, "cxg_rows8_wgrad: bad sizes or type");
   CXG_REQUIRE(dw != nullptr, CXG_ENULL, "cxg_rows8_wgrad: dw is NULL");
   const int k_blocks = (k + 127) / 128, n_blocks = (n + 127) / 128;
   CXG_REQUIRE(static_cast<int64_t>(k_blocks) * n_blocks <= 65535 && static_cast<int64_t>(k) * n < (1ll << 31), CXG_EUNSUPPORTED,
               "cxg_rows8_wgrad: a weight of %d x %d", n, k);
   cudaStream_t st = as_stream(stream);
   if (m == 0) {
-    cudaError_t e = cudaMemsetAsync(dw, 0, sizeof(float) * static_cast<size_t>(k) * n, st);
-    if (e == cudaSuccess && db != nullptr) e = cudaMemsetAsync(db, 0, sizeof(float) * n, st);
+    const size_t size = out_dtype == CXG_F32 ? 4 : 2;
+    cudaError_t e = cudaMemsetAsync(dw, 0, size * static_cast<size_t>(k) * n, st);
+    if (e == cudaSuccess && db != nullptr) e = cudaMemsetAsync(db, 0, size * n, st);
     return e == cudaSuccess ? CXG_OK : set_error(CXG_ECUDA, "cxg_rows8_wgrad: %s", cudaGetErrorString(e));
   }
   CXG_REQUIRE(codes && scales && dy, CXG_ENULL, "cxg_rows8_wgrad: NULL argument");
@@ -487,8 +490,13 @@ extern "C" int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m,
         : by_spans(rows8_wgrad<__nv_bfloat16, false, 1>, rows8_wgrad<__nv_bfloat16, false, 2>);
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_wgrad: %s", cudaGetErrorString(e));
   const int64_t outs = static_cast<int64_t>(k) * n + (db != nullptr ? n : 0);
-  launch_dependent(rows8_wgrad_join, static_cast<unsigned>((outs + 31) / 32), 32 * kJoinWarps, 0, st, a.partial, a.partial_db, dw, db, k, n,
-                   k_blocks, parts);
+  const unsigned join_blocks = static_cast<unsigned>((outs + 31) / 32);
+  if (out_dtype == CXG_F32)
+    launch_dependent(rows8_wgrad_join<float>, join_blocks, 32 * kJoinWarps, 0, st, a.partial, a.partial_db, static_cast<float *>(dw),
+                     static_cast<float *>(db), k, n, k_blocks, parts);
+  else
+    launch_dependent(rows8_wgrad_join<__nv_bfloat16>, join_blocks, 32 * kJoinWarps, 0, st, a.partial, a.partial_db,
+                     static_cast<__nv_bfloat16 *>(dw), static_cast<__nv_bfloat16 *>(db), k, n, k_blocks, parts);
   count_launches(2);
   return check_launch("cxg_rows8_wgrad");
 }

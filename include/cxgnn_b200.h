@@ -698,13 +698,13 @@ int cxg_rows8_aggregate_workspace_size(int64_t nnz, int width, int split_edges, 
 int cxg_rows8_aggregate(const void *codes, const void *scales, int64_t n_src, int width, const void *ptr, int ptr_bytes,
                         const void *idx, int idx_bytes, const float *edge_val, int64_t n_dst, int64_t nnz, int reduce,
                         int split_edges, void *y, int y_dtype, void *workspace, size_t workspace_bytes, void *stream);
-/* dw [n, k] = dy^T . rows, db [n] = column sums of dy (NULL: not wanted), both fp32: the gradients of a linear transform whose
-   input (m rows of width k) was kept in 8 bits. dy: [m, n], rows ld values apart. The rows are exact bf16 operands of the
+/* dw [n, k] = dy^T . rows, db [n] = column sums of dy (NULL: not wanted), summed in fp32, rounded once to out_dtype: the gradients
+   of a linear transform whose input (m rows of width k) was kept in 8 bits. dy: [m, n], rows ld values apart. The rows are exact bf16 operands of the
    tensor core; fp32 dy is cut into three bf16 parts, which hold all of its bits. flags: 0 or CXG_WGRAD_TEST_STALL. The status of its bounded waits:
    cxg_rows8_wgrad_status. */
 int cxg_rows8_wgrad_workspace_size(int64_t m, int k, int n, size_t *bytes);
-int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m, int k, const void *dy, int dtype, int64_t ld, int n, uint32_t flags, float *dw,
-                    float *db, void *workspace, size_t workspace_bytes, void *stream);
+int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m, int k, const void *dy, int dtype, int64_t ld, int n,
+                    uint32_t flags, void *dw, void *db, int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
 int cxg_rows8_wgrad_status(void *stream);
 
 /*

@@ -193,11 +193,11 @@ def test_waits_that_run_out_are_reported(cuda):
     want = be.rows8_weight_grad(rows, g)
     be.check_device_status("linear")
     vp, i64, ci, sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
-    fn = be._sig("cxg_rows8_wgrad", [vp, vp, i64, ci, vp, ci, i64, ci, ctypes.c_uint32, vp, vp, vp, sz, vp])
+    fn = be._sig("cxg_rows8_wgrad", [vp, vp, i64, ci, vp, ci, i64, ci, ctypes.c_uint32, vp, vp, ci, vp, sz, vp])
     ws, dw = torch.empty(1 << 22, dtype=torch.uint8, device="cuda"), torch.zeros(64, 64, device="cuda")
     be.set_wait_limit_cycles(2_000_000)
     try:
-        assert fn(rows.codes.data_ptr(), rows.scales.data_ptr(), 500, 64, g.data_ptr(), 0, 64, 64, 1, dw.data_ptr(), None,
+        assert fn(rows.codes.data_ptr(), rows.scales.data_ptr(), 500, 64, g.data_ptr(), 0, 64, 64, 1, dw.data_ptr(), None, 0,
                   ws.data_ptr(), ws.numel(), None) == 0
         torch.cuda.synchronize()
     finally:

@@ -66,13 +66,14 @@ def test_weight_grad():
     need = sz(0)
     assert size(1000, 100, 47, ctypes.byref(need)) == 0 and need.value >= 16 * 128 * 128 * 4
     assert size(1000, 0, 47, ctypes.byref(need)) == EINVAL
-    call = _fn("cxg_rows8_wgrad", [vp, vp, i64, ci, vp, ci, i64, ci, u32, vp, vp, vp, sz, vp])
-    assert call(P, P, 1000, 100, P, 0, 47, 47, 0, None, None, P, 1 << 30, None) == ENULL
-    assert call(P, P, 1000, 100, P, 0, 46, 47, 0, P, None, P, 1 << 30, None) == EINVAL
-    assert call(P, P, 1000, 100, P, 3, 47, 47, 0, P, None, P, 1 << 30, None) == EINVAL
-    assert call(P, P, 1000, 100, None, 0, 47, 47, 0, P, None, P, 1 << 30, None) == ENULL
-    assert call(P, P, 1000, 100, P, 0, 47, 47, 0, P, None, P, 100, None) == EWORKSPACE
-    assert call(P, P, 1000, 60000, P, 0, 60000, 60000, 0, P, None, P, 1 << 60, None) == EUNSUPPORTED
+    call = _fn("cxg_rows8_wgrad", [vp, vp, i64, ci, vp, ci, i64, ci, u32, vp, vp, ci, vp, sz, vp])
+    assert call(P, P, 1000, 100, P, 0, 47, 47, 0, None, None, 0, P, 1 << 30, None) == ENULL
+    assert call(P, P, 1000, 100, P, 0, 46, 47, 0, P, None, 0, P, 1 << 30, None) == EINVAL
+    assert call(P, P, 1000, 100, P, 3, 47, 47, 0, P, None, 0, P, 1 << 30, None) == EINVAL
+    assert call(P, P, 1000, 100, None, 0, 47, 47, 0, P, None, 0, P, 1 << 30, None) == ENULL
+    assert call(P, P, 1000, 100, P, 0, 47, 47, 0, P, None, 0, P, 100, None) == EWORKSPACE
+    assert call(P, P, 1000, 60000, P, 0, 60000, 60000, 0, P, None, 0, P, 1 << 60, None) == EUNSUPPORTED
+    assert call(P, P, 1000, 100, P, 0, 47, 47, 0, P, None, 2, P, 1 << 30, None) == EINVAL
 
 
 def test_residual_norm():
