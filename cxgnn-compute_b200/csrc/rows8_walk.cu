@@ -312,6 +312,9 @@ bool dispatch(const Rows8Args &r, int out_dtype, cudaStream_t st, int *resident)
 }
 
 constexpr int kMostWidth = 2048;
+// Graphs for one launch of clusters: one / three launches (us), mean, fp32: 13,264 edges, 33 columns 18.4 / 31.6, 256 20.4 / 31.7;
+// 40,000 edges, 128 24.6 / 37.9, 256 30.7 / 37.9; 60,000, 128 28.6 / 37.9, 256 36.8 / 35.9; 84,000, 64 34.8 / 33.9.
+constexpr int64_t kSmallEdges = 65536, kSmallBytes = 12 << 20;
 
 int tile_edges(const Rows8Args &r, int64_t nnz, int split_edges) {
   if (split_edges > 0) return split_edges;
@@ -377,6 +380,15 @@ extern "C" int cxg_rows8_aggregate(const void *codes, const void *scales, int64_
   a.partials = reinterpret_cast<float *>(ws + L.partials);
   a.max_tiles = L.max_tiles;
   cudaStream_t st = as_stream(stream);
+  // small graphs, as those of cxg_spmm_csr, in one launch of clusters
+  if (nnz <= kSmallEdges && nnz * a.x_pitch <= kSmallBytes && n_dst <= small_most_rows() && width <= 256 && a.tile == 64) {
+    WalkArgs small = a;
+    small.x = codes, small.x_rows = scales, small.rel_stride = n_src;
+    if (small_launch_rows8(small, y_dtype, st)) {
+      count_launches(1);
+      return check_launch("cxg_rows8_aggregate (small)");
+    }
+  }
   walk_plan_run(a, st);
   if (!dispatch(r, y_dtype, st, nullptr)) return set_error(CXG_ECUDA, "cxg_rows8_aggregate: %s", cudaGetErrorString(cudaGetLastError()));
   const cudaError_t e = walk_fix_run(a, y_dtype, st);

@@ -17,6 +17,7 @@
 
 #include <algorithm>
 
+#include "rows8.cuh"
 #include "spmm_walk_impl.cuh"
 
 namespace cg = cooperative_groups;
@@ -38,10 +39,88 @@ constexpr int kClusters = 14;     // at most: what fits on the chip at once (of 
 constexpr int kRowsPerCluster = 2048;  // so that their pointers fit (200 rows of 400 edges and 28,000 of none: they may not)
 static_assert(kClusters * kRowsPerCluster < kSmallThreads * (kSmallThreads - 1), "two rounds of probes find a row");
 
-template <typename T, int VB, int G, int NV>
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) walk_small(const __grid_constant__ WalkArgs a, int clusters) {
+// What the rows are read from: EL values per vector of a lane, sums of them in an A, what a lane has loaded of a row in a Loaded.
+// Rows of x in vectors of VB bytes.
+template <typename T, int VB>
+struct DenseRows {
   using A = Acc<T, VB>;
-  constexpr int EL = A::EL, NG = 32 / G, kGroups = kCtas * kWarps * NG;
+  static constexpr int EL = A::EL;
+  using Loaded = Words<(VB + 3) / 4>;
+  const uint8_t *x;
+  uint32_t pitch;
+  DenseRows() = default;
+  __device__ __forceinline__ DenseRows(const WalkArgs &a, int vector)
+      : x(static_cast<const uint8_t *>(a.x) + (vector * VB < a.row_bytes ? vector * VB : (a.row_bytes - 1) / VB * VB)),
+        pitch(static_cast<uint32_t>(a.row_bytes)) {}
+  __device__ __forceinline__ static uint32_t id(const WalkArgs &a, uint32_t e) {
+    return walk::load_id_low(static_cast<const uint8_t *>(a.idx) + static_cast<uint64_t>(e) * static_cast<uint32_t>(a.idx_bytes));
+  }
+  __device__ __forceinline__ static uint32_t no_id(const WalkArgs &) { return 0u; }
+  __device__ __forceinline__ void load(Loaded &v, uint32_t row) const { walk::load_row_bytes<VB>(v, x + static_cast<uint64_t>(row) * pitch); }
+  __device__ __forceinline__ static void add(A &acc, const Loaded &v, float weight) { acc.fma(v, weight); }
+  __device__ __forceinline__ static void store(const WalkArgs &a, int row, int vector, const float *f) {
+    if (vector * VB < a.row_bytes)
+      walk::store_row_bytes<T, VB>(static_cast<uint8_t *>(a.y) + static_cast<uint64_t>(row) * static_cast<uint32_t>(a.row_bytes) + vector * VB, f);
+  }
+};
+// Rows in 8 bits (a.x: the codes, a.x_rows: the scales, a.rel_stride: how many; a.x_pitch: of the codes, a.row_bytes: of y), four
+// codes at a time; ids outside stand for the row of zeros behind the last.
+template <typename T>
+struct CodedRows {
+  static constexpr int EL = 4;
+  struct A {
+    Pair p[2];
+    __device__ __forceinline__ void zero() { p[0] = p[1] = 0; }
+    __device__ __forceinline__ void get(float *f) const {
+      const float2 a = halves(p[0]), b = halves(p[1]);
+      f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+    }
+  };
+  struct Loaded {
+    uint32_t codes, scale;
+  };
+  const uint8_t *codes, *scales;
+  uint32_t pitch;
+  CodedRows() = default;
+  __device__ __forceinline__ CodedRows(const WalkArgs &a, int vector) : pitch(static_cast<uint32_t>(a.x_pitch)) {
+    const int c = vector * EL < a.x_pitch ? vector * EL : a.x_pitch - EL;
+    codes = static_cast<const uint8_t *>(a.x) + c;
+    scales = static_cast<const uint8_t *>(a.x_rows) + c / rows8::kGroup;
+  }
+  __device__ __forceinline__ static uint32_t id(const WalkArgs &a, uint32_t e) {
+    const uint64_t id = a.idx_bytes == 8 ? static_cast<uint64_t>(__ldg(static_cast<const int64_t *>(a.idx) + e))
+                                         : static_cast<uint64_t>(static_cast<int64_t>(__ldg(static_cast<const int32_t *>(a.idx) + e)));
+    return id < static_cast<uint64_t>(a.rel_stride) ? static_cast<uint32_t>(id) : no_id(a);
+  }
+  __device__ __forceinline__ static uint32_t no_id(const WalkArgs &a) { return static_cast<uint32_t>(a.rel_stride); }
+  __device__ __forceinline__ void load(Loaded &v, uint32_t row) const {
+    v.codes = __ldg(reinterpret_cast<const uint32_t *>(codes + static_cast<uint64_t>(row) * pitch));
+    v.scale = __ldg(scales + static_cast<uint64_t>(row) * (pitch / rows8::kGroup));
+  }
+  __device__ __forceinline__ static void add(A &acc, const Loaded &v, float weight) {
+    float f[4];
+    rows8::code_values(f, v.codes);
+    const float s = rows8::scale_of(v.scale) * weight;
+    acc.p[0] = fma2(pair(f[0], f[1]), pair(s, s), acc.p[0]);
+    acc.p[1] = fma2(pair(f[2], f[3]), pair(s, s), acc.p[1]);
+  }
+  __device__ __forceinline__ static void store(const WalkArgs &a, int row, int vector, const float *f) {
+    const int left = a.width - vector * EL;
+    T *y = static_cast<T *>(a.y) + static_cast<int64_t>(row) * a.width + vector * EL;
+    if (left >= EL && (reinterpret_cast<uintptr_t>(y) & (EL * sizeof(T) - 1)) == 0) {
+      walk::store_row_bytes<T, EL * static_cast<int>(sizeof(T))>(reinterpret_cast<uint8_t *>(y), f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < EL; ++i)
+        if (i < left) y[i] = from_f32<T>(f[i]);
+    }
+  }
+};
+
+template <typename Source, int G, int NV>
+__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) walk_small(const __grid_constant__ WalkArgs a, int clusters) {
+  using A = typename Source::A;
+  constexpr int EL = Source::EL, NG = 32 / G, kGroups = kCtas * kWarps * NG;
   constexpr int U = NV == 1 && EL <= 4 ? 16 : 8;  // edges in flight per lane
   __shared__ uint32_t slice[kSliceRows + 1];
   __shared__ __align__(16) uint32_t id_stage[kWarps][NG * kPitch];
@@ -49,7 +128,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, lg = lane & (G - 1), warp = tid >> 5;
   const int rank = static_cast<int>(cluster.block_rank()), me = static_cast<int>(blockIdx.x) / kCtas;
-  const int n = static_cast<int>(a.n_dst), rb = a.row_bytes;
+  const int n = static_cast<int>(a.n_dst);
   auto ptr_at = [&](int r) { return walk::load_ptr_low(a.ptr, r, a.ptr_bytes); };
   dependency_wait();
 
@@ -95,15 +174,13 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
     return lo - 1;
   };
 
-  auto on = [&](int q) { return (lg + q * G) * VB < rb; };
-  const uint8_t *xq[NV];
+  auto on = [&](int q) { return (lg + q * G) * EL < a.width; };
+  Source source[NV];
 #pragma unroll
-  for (int q = 0; q < NV; ++q) xq[q] = static_cast<const uint8_t *>(a.x) + (on(q) ? (lg + q * G) * VB : (rb - 1) / VB * VB);
+  for (int q = 0; q < NV; ++q) source[q] = Source(a, lg + q * G);
   auto store = [&](int i, const float (&f)[NV][EL]) {
-    uint8_t *dst = static_cast<uint8_t *>(a.y) + static_cast<uint64_t>(r_lo + i) * static_cast<uint32_t>(rb) + lg * VB;
 #pragma unroll
-    for (int q = 0; q < NV; ++q)
-      if (on(q)) walk::store_row_bytes<T, VB>(dst + q * G * VB, f[q]);
+    for (int q = 0; q < NV; ++q) Source::store(a, r_lo + i, lg + q * G, f[q]);
   };
   auto zero_row = [&](int i) {
     const float z[NV][EL] = {};
@@ -156,10 +233,10 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
 #pragma unroll
       for (int j = 0; j < kPitch / G; ++j) {
         const int pos = j * G + lg;
-        id[j] = 0u, val[j] = 1.f;  // times one is exact
+        id[j] = Source::no_id(a), val[j] = 1.f;  // times one is exact
         if (pos < len) {
           const uint32_t e = begin + pos;
-          id[j] = walk::load_id_low(static_cast<const uint8_t *>(a.idx) + static_cast<uint64_t>(e) * static_cast<uint32_t>(a.idx_bytes));
+          id[j] = Source::id(a, e);
           if (a.edge_val != nullptr) val[j] = __ldg(a.edge_val + e);
         }
       }
@@ -179,12 +256,12 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
     const int longest = G == 32 ? len : __reduce_max_sync(0xffffffffu, len);
 #pragma unroll 1
     for (int p = 0; p < longest; p += U) {
-      Words<(VB + 3) / 4> v[U][NV];
+      typename Source::Loaded v[U][NV];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const uint64_t off = static_cast<uint64_t>(ids[p + u]) * static_cast<uint32_t>(rb);
+        const uint32_t id = ids[p + u];
 #pragma unroll
-        for (int q = 0; q < NV; ++q) walk::load_row_bytes<VB>(v[u][q], xq[q] + off);
+        for (int q = 0; q < NV; ++q) source[q].load(v[u][q], id);
       }
       float weights[U];
 #pragma unroll
@@ -199,7 +276,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
           if (u >= q0 && u < q1) {
             const float weight = weights[u];
 #pragma unroll
-            for (int q = 0; q < NV; ++q) acc[q].fma(v[u][q], weight);
+            for (int q = 0; q < NV; ++q) Source::add(acc[q], v[u][q], weight);
           }
         q0 = q1;
         const int pos = p + q1;
@@ -287,9 +364,9 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
   }
 }
 
-template <typename T, int VB>
-bool launch_small(const WalkArgs &a, cudaStream_t st) {
-  const int vectors = (a.row_bytes + VB - 1) / VB;
+// Rows of `vectors` vectors of a lane.
+template <typename Source, int kMost>
+bool launch_small(const WalkArgs &a, int vectors, cudaStream_t st) {
   auto go = [&](auto kernel, int g) {
     const int64_t groups = kCtas * kWarps * (32 / g);
     int64_t clusters = (a.nnz + 8 * groups - 1) / (8 * groups);
@@ -297,13 +374,17 @@ bool launch_small(const WalkArgs &a, cudaStream_t st) {
     clusters = clusters < 1 ? 1 : clusters > kClusters ? kClusters : clusters;
     return launch_dependent(kernel, static_cast<unsigned>(clusters * kCtas), kSmallThreads, 0, st, a, static_cast<int>(clusters)) == cudaSuccess;
   };
-  if (vectors <= 8) return go(walk_small<T, VB, 8, 1>, 8);
-  if (vectors <= 16) return go(walk_small<T, VB, 16, 1>, 16);
-  if (vectors <= 32) return go(walk_small<T, VB, 32, 1>, 32);
-  if (vectors <= 64) return go(walk_small<T, VB, 32, 2>, 32);
-  if constexpr (VB < 16)
-    if (vectors <= 128) return go(walk_small<T, VB, 32, 4>, 32);
+  if (vectors <= 8) return go(walk_small<Source, 8, 1>, 8);
+  if (vectors <= 16) return go(walk_small<Source, 16, 1>, 16);
+  if (vectors <= 32) return go(walk_small<Source, 32, 1>, 32);
+  if (vectors <= 64) return go(walk_small<Source, 32, 2>, 32);
+  if constexpr (kMost > 64)
+    if (vectors <= 128) return go(walk_small<Source, 32, 4>, 32);
   return false;
+}
+template <typename T, int VB>
+bool launch_small(const WalkArgs &a, cudaStream_t st) {
+  return launch_small<DenseRows<T, VB>, (VB < 16 ? 128 : 64)>(a, (a.row_bytes + VB - 1) / VB, st);
 }
 
 }  // namespace
@@ -316,6 +397,11 @@ bool small_launch(const WalkArgs &a, int dtype, int vb, cudaStream_t st) {
          : vb == 8 ? launch_small<__nv_bfloat16, 8>(a, st)
          : vb == 4 ? launch_small<__nv_bfloat16, 4>(a, st)
                    : launch_small<__nv_bfloat16, 2>(a, st);
+}
+
+bool small_launch_rows8(const WalkArgs &a, int y_dtype, cudaStream_t st) {
+  const int vectors = (a.width + 3) / 4;
+  return y_dtype == CXG_F32 ? launch_small<CodedRows<float>, 64>(a, vectors, st) : launch_small<CodedRows<__nv_bfloat16>, 64>(a, vectors, st);
 }
 
 int small_most_rows() { return kClusters * kRowsPerCluster; }

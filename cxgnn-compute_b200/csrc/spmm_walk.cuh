@@ -93,6 +93,9 @@ size_t walk_copy_bytes(const cxg_spmm_desc *d, int64_t n_src);
 // bytes or 128 of fewer, up to small_most_rows() of them. False: no kernel for it.
 bool small_launch(const WalkArgs &a, int dtype, int vb, cudaStream_t st);
 int small_most_rows();
+// The same over rows in 8 bits: a.x codes, a.x_rows scales, a.x_pitch pitch of the codes, a.rel_stride how many rows; y of type
+// y_dtype, rows of up to 256 values.
+bool small_launch_rows8(const WalkArgs &a, int y_dtype, cudaStream_t st);
 
 // One launcher per element type and vector width, each in a translation unit of its own. False: no kernel for it. With
 // resident_tiles set nothing is launched: it receives the number of tiles that are walked at the same time.
