@@ -10,7 +10,7 @@
 // producer warps load 16 bytes at a time a whole stage ahead, convert, and write the operands where the tensor core reads
 // them. One instruction multiplies A by [hi | mid], another adds A by lo to mid's accumulator. An accumulator takes
 // `chunk` stages, as the tensor core's additions cut off what an fp32 addition rounds (its error grows with the number of
-// additions); the epilogue warps, each lane a column of the input, keep the sums of the chunks in registers.
+// additions); the epilogue warps, each lane a column of the input, add the chunks up in shared memory.
 //
 // A block owns a contiguous range of rows of one pair of 128-column blocks; its sums go to a partial of its own and a second
 // kernel adds the partials in order: the same bits on every run. Every wait is bounded (see tensor_core.cuh).
@@ -28,11 +28,11 @@ constexpr int kSpan = kPos * 128;  // bytes of a span: 64 columns of bf16, one r
 constexpr int kProdWarps = 16, kEpiWarps = 8;
 constexpr int kMmaWarp = kEpiWarps, kFirstProd = kMmaWarp + 4;  // roles in whole groups of four warps, which share out registers
 constexpr int kThreads = 32 * (kFirstProd + kProdWarps);
-// Registers per thread: 72 at the launch (896 threads take 64,512), where the producers stay; the epilogue, whose lanes hold 64
-// sums each, takes 24 more each from the group of the issuing warp: 256 * 96 + 128 * 24 + 512 * 72 = 64,512. (Eight producer
-// warps with two stages of loads in 128 registers each left the chip idle between their dependent instructions: 400,000 rows
-// of 100 x 128 fp32 115 us; with 96 registers for all of them, loads were spilled, which waits for each: 202 us.)
-constexpr int kIssuerRegs = 24, kEpilogueRegs = 96;
+// Registers per thread: 72 at the launch (896 threads take 64,512). The producers, which hold two stages of loads, take 24 more
+// each from the others: 256 * 40 + 128 * 24 + 512 * 96 = 62,464. (One stage of loads in 72 registers: 85 us for 400,000 rows of
+// 100 x 128 fp32, 25 of them waiting for loads; eight warps with two stages in 128 registers left the chip idle between their
+// dependent instructions: 115 us; with 96 registers for all of them, loads were spilled, which waits for each: 202 us.)
+constexpr int kIssuerRegs = 24, kEpilogueRegs = 40, kProducerRegs = 96;
 constexpr int kMaxStages = 4;
 constexpr int kSmemBudget = 216 * 1024;
 
@@ -105,8 +105,9 @@ __device__ __forceinline__ void three_parts(const Pair (&v)[4], uint32_t (&hi)[4
   }
 }
 
-// SPANS: 64-column spans of a block of dy. VEC: rows of dy are whole 16-byte vectors.
-template <typename T, bool VEC, int SPANS>
+// SPANS: 64-column spans of a block of dy. VECTOR: bytes of the vectors that rows of dy are read in, all of them whole (0: value
+// by value). 32-byte vectors of fp32 take half the passes through L1 that pairs of 16-byte ones do.
+template <typename T, int VECTOR, int SPANS>
 __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant__ R8Args a) {
   constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
   constexpr int kCols = 64 * SPANS;
@@ -122,6 +123,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int x_at = static_cast<int>(blockIdx.y % a.k_blocks) * 128, g_at = static_cast<int>(blockIdx.y / a.k_blocks) * 128;
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  float *const sums = reinterpret_cast<float *>(smem_raw + (base - smem_addr(smem_raw)) + static_cast<size_t>(a.stages) * kStageBytes);  // [kCols][128]
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_slot)), "r"(kTmem)
                  : "memory");
@@ -148,9 +150,10 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
   const int64_t tile_lo = n_tiles * blockIdx.x / gridDim.x, tile_hi = n_tiles * (blockIdx.x + 1) / gridDim.x;
 
   if (warp >= kFirstProd) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
     // ================= producers =================
-    // Every thread has a unit of 16 codes and one or two of 8 values of dy per stage. What it has loaded of the next stage
-    // replaces a unit as soon as this one is written, so that a load has a whole stage's time to arrive.
+    // Every thread has a unit of 16 codes and one or two of 8 values of dy per stage. What it loads of the stage after the next
+    // replaces a unit as soon as this one is written, so that a load has two stages' time to arrive.
     constexpr int kThr = 32 * kProdWarps;
     constexpr int kUnitsPerRow = 8 * SPANS;                 // of dy
     constexpr int kGUnits = kPos * kUnitsPerRow / kThr;
@@ -164,38 +167,46 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
     int64_t row = tile_lo * kPos;                                         // first of the stage that is loaded
     const uint8_t *codes = a.codes + (row + xrow) * a.pitch + xcol, *scales = a.scales + (row + xrow) * a.groups + xcol / kGroup;
     const T *dy = static_cast<const T *>(a.dy) + (row + grow) * a.ld + gcol;
-    uint4 rc;
-    uint32_t rs;
     constexpr int W = sizeof(T) == 4 ? 8 : 4;
-    uint32_t rg[kGUnits][W];
-    auto load_codes = [&]() {
-      rc = make_uint4(0, 0, 0, 0);
-      rs = 0;
+    struct Raw {  // of a stage, as it was loaded
+      uint4 codes;
+      uint32_t scale;
+      uint32_t dy[kGUnits][W];
+    };
+    auto load_codes = [&](Raw &raw) {
+      raw.codes = make_uint4(0, 0, 0, 0);
+      raw.scale = 0;
       if (x_in && row + xrow < row_end) {
-        rc = __ldg(reinterpret_cast<const uint4 *>(codes));
-        rs = __ldg(scales);
+        raw.codes = __ldg(reinterpret_cast<const uint4 *>(codes));
+        raw.scale = __ldg(scales);
       }
     };
-    auto load_dy = [&](int j) {
+    auto load_dy = [&](Raw &raw, int j) {
+      uint32_t(&v)[W] = raw.dy[j];
 #pragma unroll
-      for (int i = 0; i < W; ++i) rg[j][i] = 0;
+      for (int i = 0; i < W; ++i) v[i] = 0;
       if (row + grow + j * kGRows >= row_end) return;
       const T *p = dy + static_cast<int64_t>(j * kGRows) * a.ld;
-      if constexpr (VEC) {
+      if constexpr (VECTOR == 32) {
+        if (gcol < a.n)
+          asm("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+              : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4 % W]), "=r"(v[5 % W]), "=r"(v[6 % W]), "=r"(v[7 % W])
+              : "l"(p));
+      } else if constexpr (VECTOR == 16) {
 #pragma unroll
         for (int i = 0; i < W; i += 4)
           if (gcol + i < a.n) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p + i));
-            rg[j][i] = v.x, rg[j][i + 1] = v.y, rg[j][i + 2] = v.z, rg[j][i + 3] = v.w;
+            const uint4 t = __ldg(reinterpret_cast<const uint4 *>(p + i));
+            v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
           }
       } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (gcol + i < a.n) rg[j][i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+          if (gcol + i < a.n) v[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (gcol + i < a.n) rg[j][i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(p) + i)) << (16 * (i & 1));
+          if (gcol + i < a.n) v[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(p) + i)) << (16 * (i & 1));
       }
     };
     auto onward = [&]() {
@@ -211,57 +222,75 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
     const uint32_t g_first = (2 + (gu >> 3)) * kSpan + swizzled_offset<false>(grow, gu & 7);
     static_assert(kGRows % 8 == 0, "the swizzle repeats every eight rows");
     Pair db[4] = {};
-    auto put_codes = [&](uint32_t stage) {
-      const __nv_bfloat162 s = __float2bfloat162_rn(rows8::scale_of(rs));
-      const uint32_t w[4] = {rc.x, rc.y, rc.z, rc.w};
+    const bool want_db = a.partial_db != nullptr && x_at == 0;
+    auto put_codes = [&](const Raw &raw, uint32_t stage) {
+      const __nv_bfloat162 s = __float2bfloat162_rn(rows8::scale_of(raw.scale));
+      const uint32_t w[4] = {raw.codes.x, raw.codes.y, raw.codes.z, raw.codes.w};
       uint32_t v[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[2 * i] = two_values<0>(w[i], s), v[2 * i + 1] = two_values<1>(w[i], s);
       st_shared16(stage + (odd ? x_second : x_first), v[0], v[1], v[2], v[3]);
       st_shared16(stage + (odd ? x_first : x_second), v[4], v[5], v[6], v[7]);
     };
-    auto put_dy = [&](int j, uint32_t stage) {
+    auto put_dy = [&](const Raw &raw, int j, uint32_t stage) {
+      const uint32_t(&r)[W] = raw.dy[j];
       const uint32_t at = stage + g_first + j * kGRows * 128;
       if constexpr (sizeof(T) == 4) {
         Pair v[4];
         uint32_t hi[4], mid[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          v[i] = pair(__uint_as_float(rg[j][2 * i]), __uint_as_float(rg[j][2 * i + 1]));
-          db[i] = add2(db[i], v[i]);
+          v[i] = pair(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+        }
+        if (want_db) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) db[i] = add2(db[i], v[i]);
         }
         three_parts(v, hi, mid, lo);
         st_shared16(at, hi[0], hi[1], hi[2], hi[3]);
         st_shared16(at + SPANS * kSpan, mid[0], mid[1], mid[2], mid[3]);
         st_shared16(at + 2 * SPANS * kSpan, lo[0], lo[1], lo[2], lo[3]);
       } else {
+        if (want_db) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          db[i] = add2(db[i], pair(__uint_as_float(rg[j][i] << 16), __uint_as_float(rg[j][i] & 0xffff0000u)));
-        st_shared16(at, rg[j][0], rg[j][1], rg[j][2], rg[j][3]);
+          for (int i = 0; i < 4; ++i)
+            db[i] = add2(db[i], pair(__uint_as_float(r[i] << 16), __uint_as_float(r[i] & 0xffff0000u)));
+        }
+        st_shared16(at, r[0], r[1], r[2], r[3]);
       }
     };
     Ring ring(a.stages);
-    load_codes();
+    auto load = [&](Raw &raw) {
+      load_codes(raw);
 #pragma unroll
-    for (int j = 0; j < kGUnits; ++j) load_dy(j);
-    for (int64_t tile = tile_lo; tile < tile_hi; ++tile) {
-      const int s = ring.stage;
-      if (ring.reused() && !wait_bar(&bars.empty[s], ring.emptied(), abort_flag, a.status, a.wait_cycles)) break;
-      const uint32_t stage = base + static_cast<uint32_t>(s) * kStageBytes;
+      for (int j = 0; j < kGUnits; ++j) load_dy(raw, j);
       onward();
-      put_codes(stage);
-      load_codes();
+    };
+    auto hand_over = [&](Raw &raw) {
+      const int s = ring.stage;
+      if (ring.reused() && !wait_bar(&bars.empty[s], ring.emptied(), abort_flag, a.status, a.wait_cycles)) return false;
+      const uint32_t stage = base + static_cast<uint32_t>(s) * kStageBytes;
+      put_codes(raw, stage);
+      load_codes(raw);
 #pragma unroll
       for (int j = 0; j < kGUnits; ++j) {
-        put_dy(j, stage);
-        load_dy(j);
+        put_dy(raw, j, stage);
+        load_dy(raw, j);
       }
+      onward();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       if (!(a.test_stall && ring.round == 0 && s == 0)) mbar_arrive(&bars.full[s]);
       ring.next();
+      return true;
+    };
+    Raw even, odd_raw;
+    load(even);
+    load(odd_raw);
+    for (int64_t tile = tile_lo; tile < tile_hi; tile += 2) {
+      if (!hand_over(even)) break;
+      if (tile + 1 < tile_hi && !hand_over(odd_raw)) break;
     }
-    if (a.partial_db != nullptr && x_at == 0) {
+    if (want_db) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float2 t = halves(db[i]);
@@ -329,12 +358,9 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
     }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
     // ================= epilogue: lane = column of the input, half of the columns of dy per four warps =================
     constexpr int kHalf = kCols / 2;
-    float acc[kHalf];
-#pragma unroll
-    for (int c = 0; c < kHalf; ++c) acc[c] = 0.f;
     const int first = (warp >> 2) * kHalf, row = (warp & 3) * 32 + lane;
     const int64_t n_chunks = (tile_hi - tile_lo + a.chunk - 1) / a.chunk;
     bool alive = true;
@@ -345,24 +371,26 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
       if (!alive) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t taddr = tmem_d + (static_cast<uint32_t>((warp & 3) * 32) << 16) + buf * kAccCols + first;
-#pragma unroll
-      for (int c = 0; c < kHalf; c += 8) {
+      float *sum = sums + first * 128 + row;
+#pragma unroll 1
+      for (int c = 0; c < kHalf; c += 8, sum += 8 * 128) {
         uint32_t v[8], w[8];
         tmem_ld8(v, taddr + c);
         if constexpr (kParts == 3) tmem_ld8(w, taddr + kCols + c);
+        float old[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) old[i] = chunk > 0 ? sum[i * 128] : 0.f;
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          acc[c + i] += kParts == 3 ? __uint_as_float(v[i]) + __uint_as_float(w[i]) : __uint_as_float(v[i]);
+          sum[i * 128] = old[i] + (kParts == 3 ? __uint_as_float(v[i]) + __uint_as_float(w[i]) : __uint_as_float(v[i]));
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       mbar_arrive(&bars.acc_empty[buf]);
     }
     if (alive && x_at + row < a.k) {
       float *out = a.partial + ((static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 128 + first) * 128 + row;
-#pragma unroll
-      for (int c = 0; c < kHalf; ++c)
-        if (g_at + first + c < a.n) out[c * 128] = acc[c];
+      for (int c = 0; c < kHalf && g_at + first + c < a.n; ++c) out[c * 128] = sums[(first + c) * 128 + row];
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -469,13 +497,14 @@ extern "C" int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m,
   a.wait_cycles = wait_limit_cycles();
   const int spans = n > 64 ? 2 : 1;
   const int stage = (2 + (dtype == CXG_F32 ? 3 : 1) * spans) * kSpan;
-  a.stages = (kSmemBudget - 1024) / stage < kMaxStages ? (kSmemBudget - 1024) / stage : kMaxStages;
+  const int sums = 64 * spans * 128 * static_cast<int>(sizeof(float)), fit = (kSmemBudget - 1024 - sums) / stage;
+  a.stages = fit < kMaxStages ? fit : kMaxStages;
   a.chunk = (dtype == CXG_F32 ? 512 : 1024) / kPos;
-  const int smem = 1024 + a.stages * stage;
+  const int smem = 1024 + a.stages * stage + sums;
   void *word = nullptr;
   cudaError_t e = cudaGetSymbolAddress(&word, r8_status);
   a.status = static_cast<int32_t *>(word);
-  const bool vec = (static_cast<uint64_t>(ld) * elem | static_cast<uint64_t>(n) * elem | reinterpret_cast<uintptr_t>(dy)) % 16 == 0;
+  const uint64_t bits = static_cast<uint64_t>(ld) * elem | static_cast<uint64_t>(n) * elem | reinterpret_cast<uintptr_t>(dy);
   const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(k_blocks * n_blocks));
   auto go = [&](auto kernel) {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -483,11 +512,12 @@ extern "C" int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m,
   };
   auto by_spans = [&](auto one, auto two) { spans == 1 ? go(one) : go(two); };
   if (dtype == CXG_F32)
-    vec ? by_spans(rows8_wgrad<float, true, 1>, rows8_wgrad<float, true, 2>)
-        : by_spans(rows8_wgrad<float, false, 1>, rows8_wgrad<float, false, 2>);
+    bits % 32 == 0   ? by_spans(rows8_wgrad<float, 32, 1>, rows8_wgrad<float, 32, 2>)
+    : bits % 16 == 0 ? by_spans(rows8_wgrad<float, 16, 1>, rows8_wgrad<float, 16, 2>)
+                     : by_spans(rows8_wgrad<float, 0, 1>, rows8_wgrad<float, 0, 2>);
   else
-    vec ? by_spans(rows8_wgrad<__nv_bfloat16, true, 1>, rows8_wgrad<__nv_bfloat16, true, 2>)
-        : by_spans(rows8_wgrad<__nv_bfloat16, false, 1>, rows8_wgrad<__nv_bfloat16, false, 2>);
+    bits % 16 == 0 ? by_spans(rows8_wgrad<__nv_bfloat16, 16, 1>, rows8_wgrad<__nv_bfloat16, 16, 2>)
+                   : by_spans(rows8_wgrad<__nv_bfloat16, 0, 1>, rows8_wgrad<__nv_bfloat16, 0, 2>);
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_wgrad: %s", cudaGetErrorString(e));
   const int64_t outs = static_cast<int64_t>(k) * n + (db != nullptr ? n : 0);
   const unsigned join_blocks = static_cast<unsigned>((outs + 31) / 32);
