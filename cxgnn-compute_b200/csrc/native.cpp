@@ -763,7 +763,7 @@ Held held_zeros(int64_t rows, int64_t width, at::Device device) {
   if (!device.is_cuda()) fail("Rows8: the device must be a CUDA device (this backend has no CPU path)");
   c10::cuda::CUDAGuard guard(device);
   Held h = held_like(rows, width, device);
-  h.codes.zero_();
+  h.codes.fill_(128);
   h.scales.zero_();
   return h;
 }

@@ -4,8 +4,9 @@
 // 2^-7 of the group's largest value. Seven bits and a power of two are exact in fp32 and in bf16. A group with a value that
 // is not finite has e = 255 and c = 0: 2^128 is read as infinity, and zero times it is NaN, with no test where rows are read.
 //
-// In memory: codes [rows + 1][pitch] bytes, pitch = width in whole groups of 32, zeros behind the width; scales
-// [rows + 1][pitch / 32] bytes. The last row is of zeros: what ids outside the rows stand for. (One scale per group and not per
+// In memory: codes [rows + 1][pitch] bytes c + 128 (which saves every reader a flip of the sign), pitch = width in whole groups of
+// 32, zeros (128) behind the width; scales [rows + 1][pitch / 32] bytes. The last row is of zeros: what ids outside the rows
+// stand for. (One scale per group and not per
 // row: activations behind a ReLU differ by orders of magnitude along a row. Scales in an array of their own: rows of codes
 // then start on whole sectors, and the scales of a million rows of 128 stay in L2.)
 #pragma once
@@ -65,9 +66,10 @@ __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_floa
 // x / s of finite groups: the product with 2^(254 - e - 127) is exact, or so small that it rounds to zero either way
 __device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
-// The code as the low byte of the result: adding 1.5 * 2^23 to x / s (exact in front of the addition) rounds to whole numbers,
-// ties to even, and leaves their two's complement in the low bits.
-__device__ __forceinline__ uint32_t code_bits(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f)); }
+// c + 128 as the low byte of the result: adding 1.5 * 2^23 to x / s (exact in front of the addition) rounds to whole numbers,
+// ties to even, and leaves them in the low bits.
+__device__ __forceinline__ uint32_t code_bits(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f + 128.f)); }
+constexpr uint32_t kZeroCodes = 0x80808080u;
 
 __device__ __forceinline__ uint32_t pack_codes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
@@ -88,19 +90,18 @@ __device__ __forceinline__ void codes_of(uint32_t (&w)[N / 4], const float (&v)[
       uint32_t c[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[i] = code_bits(fminf(fmaxf(v[4 * j + i] * inverse_scale(248), -127.f), 127.f), 1.f);
-      w[j] = e == kNotFinite ? 0u : pack_codes(c[0], c[1], c[2], c[3]);
+      w[j] = e == kNotFinite ? kZeroCodes : pack_codes(c[0], c[1], c[2], c[3]);
     }
   }
 }
 
-// Code i of a word as fp32: the code with its sign bit flipped is code + 128; as the low byte of 2^23 it is 2^23 + 128 + code.
+// Code i of a word as fp32: as the low byte of 2^23 it is 2^23 + 128 + c.
 template <int I>
-__device__ __forceinline__ float code_value(uint32_t flipped) {
-  return __uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7440 | I)) - 8388736.f;
+__device__ __forceinline__ float code_value(uint32_t word) {
+  return __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7440 | I)) - 8388736.f;
 }
 __device__ __forceinline__ void code_values(float *f, uint32_t word) {
-  const uint32_t w = word ^ 0x80808080u;
-  f[0] = code_value<0>(w), f[1] = code_value<1>(w), f[2] = code_value<2>(w), f[3] = code_value<3>(w);
+  f[0] = code_value<0>(word), f[1] = code_value<1>(word), f[2] = code_value<2>(word), f[3] = code_value<3>(word);
 }
 
 }  // namespace rows8

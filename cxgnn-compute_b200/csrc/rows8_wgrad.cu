@@ -58,12 +58,12 @@ __device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b,
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// Two neighbouring codes (bytes 2 * H and 2 * H + 1 of a word) times the scale, as two bf16. With c = low - 128 * sign:
-// 0x4300 | (c & 0x7f) is 128 + low and 0x4300 | (c & 0x80) is 128 + 128 * sign in bf16, and their difference is exact.
+// Two neighbouring codes (bytes b = c + 128 of a word, 2 * H and 2 * H + 1) times the scale, as two bf16. 0x4300 | (b & 0x7f) is
+// 128 + (b & 0x7f) in bf16, and 0x4300 | (~b & 0x80) is 256 where c is negative, else 128: their difference is c, exactly.
 template <int H>
 __device__ __forceinline__ uint32_t two_values(uint32_t word, __nv_bfloat162 scale) {
   const uint32_t w = __byte_perm(word, 0x43434343u, H == 0 ? 0x4140 : 0x4342);
-  const uint32_t lo = w & 0xff7fff7fu, hi = w & 0xff80ff80u;
+  const uint32_t lo = w & 0xff7fff7fu, hi = (w & 0xff80ff80u) ^ 0x00800080u;
   __nv_bfloat162 a, b;
   __builtin_memcpy(&a, &lo, 4);
   __builtin_memcpy(&b, &hi, 4);

@@ -673,8 +673,8 @@ int cxg_spmm_csr_static_status(void *stream);
  * rounded to nearest, ties to even. The values are exact in fp32 and bf16, and off by at most s / 2, at most 2^-7 of the
  * group's largest. A group with a value that is not finite (e = 255) reads as NaN throughout.
  *
- * codes: [rows + 1][cxg_rows8_pitch(width)] bytes, 16-byte aligned, zeros behind the width; scales: [rows + 1][pitch / 32]
- * bytes. The row behind the last is of zeros: it is what ids outside [0, rows) are read as.
+ * codes: [rows + 1][cxg_rows8_pitch(width)] bytes c + 128, 16-byte aligned, 128 behind the width; scales: [rows + 1][pitch / 32]
+ * bytes, 4-byte aligned. The row behind the last is of zeros: it is what ids outside [0, rows) are read as.
  */
 int cxg_rows8_pitch(int width);
 /* Rows [0, n) of x ([n, width], row i at x + i * ld values; CXG_F32 or CXG_BF16) to rows [0, n); zero_row: row n is written
