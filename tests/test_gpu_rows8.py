@@ -101,6 +101,20 @@ def test_write_at_and_read_at(cuda, width, dtype):
     assert _same(be.dequantize_rows(cache, index=ids.cuda(), dtype=dtype), picked)
 
 
+@pytest.mark.parametrize("n", [1, 1023, 1025, 4096, 4097, 30000])
+def test_equal_ids_of_any_number_of_rows(cuda, n):
+    """Every id comes about three times; the last of its rows is told by its values."""
+    import cxgnncomp_backend as be
+    ids = torch.randint(0, max(1, n // 3), (n,), generator=torch.Generator().manual_seed(n))
+    x = (torch.arange(n) % 127 + 1).float().unsqueeze(1).expand(n, 5).contiguous()  # whole numbers up to 127: exact
+    cache = be.Rows8(max(1, n // 3), 5)
+    be.quantize_rows(x.cuda(), out=cache, index=ids.cuda())
+    want = torch.zeros(max(1, n // 3), 5)
+    for i, r in enumerate(ids.tolist()):
+        want[r] = x[i]
+    assert torch.equal(be.dequantize_rows(cache).cpu(), want)
+
+
 def test_first_rows_and_empty_calls(cuda):
     import cxgnncomp_backend as be
     cache = be.Rows8(10, 40)
