@@ -718,6 +718,28 @@ const char *const kTransform = " does not take tensors of a transform (vmap, for
 
 int code_of(const Tensor &t) { return t.scalar_type() == at::kFloat ? CXG_F32 : CXG_BF16; }
 
+// Whether the backward pass that a call records would lead from a graph capture into another stream's nodes: those of a leaf
+// that an eager graph still holds, or of a tensor that was computed outside the capture. torch's engine then makes the other
+// stream wait for a captured event, which ends the process.
+void recorded_in_capture(const char *who, const Tensor &t) {
+  if (!t.defined() || !t.requires_grad() || !at::GradMode::is_enabled()) return;
+  const auto stream = c10::cuda::getCurrentCUDAStream(t.device().index());
+  if (!capture_of(stream.stream())) return;
+  const auto node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto of = node->stream();
+  if (of && *of != stream.unwrap())
+    fail(std::string(who) + ": under capture, with gradients recorded, of a tensor whose graph belongs to another stream and is still "
+                            "alive: drop what was computed from it before the capture");
+}
+void recorded_in_capture(const char *who, const optional<Tensor> &t) {
+  if (t) recorded_in_capture(who, *t);
+}
+template <typename... T>
+void all_recorded_in_capture(const char *who, const T &...t) {
+  (recorded_in_capture(who, t), ...);
+}
+
 // A matrix of rows that lie any distance apart, each in one piece; a copy of any other.
 Tensor row_matrix(const Tensor &t, const char *name) {
   if (!t.is_cuda()) fail(std::string(name) + " must be a CUDA tensor (this backend has no CPU path)");
@@ -953,6 +975,7 @@ Tensor linear_kept8(Tensor x, Tensor w, optional<Tensor> bias, optional<Tensor> 
       fail("linear_kept8: kept must hold the rows of x");
   }
   c10::cuda::CUDAGuard guard(x.device());
+  all_recorded_in_capture("linear_kept8", x, w, bias, add);
   c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);
   if (recorded(x, w, bias, add))
     return LinearKept8Function::apply(x, w, bias, add, codes, scales);
@@ -1124,6 +1147,7 @@ std::vector<optional<Tensor>> residual_norm(const Tensor &x_in, const optional<T
     if (!per_row && gate->sizes() != x.sizes()) fail("residual_norm: gate must have the shape of x, or one value per row");
   }
   c10::cuda::CUDAGuard guard(x.device());
+  all_recorded_in_capture("residual_norm", x_in, f_in, gate_in, scale_in, post_weight, post_bias, next_weight, next_bias);
   const auto scale = row_parameter(scale_in, x, "scale"), w2 = row_parameter(post_weight, x, "post_weight"),
              b2 = row_parameter(post_bias, x, "post_bias"), w1 = row_parameter(next_weight, x, "next_weight"),
              b1 = row_parameter(next_bias, x, "next_bias");

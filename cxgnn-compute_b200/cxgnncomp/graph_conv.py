@@ -144,7 +144,8 @@ class MySageConv(torch.nn.Module):
             out = linear(sage_mean_forward(x, ptr, idx, num_node), self.lin_l.weight, self.lin_l.bias)
         if not self.root_weight:
             return out
-        return linear(x[:out.shape[0]], self.lin_r.weight, add=out, kept=kept)
+        root = x if out.shape[0] == x.shape[0] else x[:out.shape[0]]  # (the gradient of a slice is a copy into zeros)
+        return linear(root, self.lin_r.weight, add=out, kept=kept)
 
 
 class MyGINConv(torch.nn.Module):

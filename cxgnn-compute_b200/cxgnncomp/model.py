@@ -137,11 +137,13 @@ class ResidualGNN(torch.nn.Module):
             e = int(batch.num_edge_in_layer[L - 1 - i]) if batch.num_edge_in_layer is not None else batch.idx.shape[0]
             ptr, idx, kept = batch.ptr[:n + 1], batch.idx[:e], {"kept": rows[0]} if rows else {}
             f = F.dropout(F.relu(conv(h, ptr, idx, n, **kept)), p=self.dropout, training=self.training)
+            if n != x.shape[0]:  # (the gradient of a slice is a copy into zeros)
+                x, h = x[:n], h[:n]
             gate = None
             if self.gate is not None:
                 lin = self.gates[i]
-                gate = cxgnncomp_backend.linear_kept8(h[:n], lin.weight, lin.bias, **kept) if rows else lin(h[:n])
-            x, h, *rows = step(i + 1, x[:n], f, gate)
+                gate = cxgnncomp_backend.linear_kept8(h, lin.weight, lin.bias, **kept) if rows else lin(h)
+            x, h, *rows = step(i + 1, x, f, gate)
         return self.lin_out(h).log_softmax(dim=-1)
 
 

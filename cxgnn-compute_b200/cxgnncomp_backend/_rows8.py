@@ -91,8 +91,9 @@ def dequantize_rows(rows, index=None, dtype=torch.float32, num_rows=None):
 
 def rows8_aggregate(rows, ptr, idx, num_node, reduce="sum", edge_value=None, dtype=torch.float32):
     """out[d] = sum (or mean) over row d of the graph of [edge_value[e] *] rows[idx[e]], [num_node, width] in `dtype`: the
-    aggregations of this module over rows in 8 bits, summed in float32 in edge order. num_node = 0 means all rows of ptr, rows
-    without edges give 0, an id outside the rows counts as a row of zeros. Rows and edge values are constants: no gradient."""
+    aggregations of this module over rows in 8 bits, summed in float32 in edge order. ptr ascends from 0; num_node = 0 means all
+    rows of ptr, rows without edges give 0, an id outside the rows counts as a row of zeros. Rows and edge values are constants:
+    no gradient. Rows of up to 2048 values."""
     from . import SPLIT_EDGES
     _rows8(rows, "rows8_aggregate")
     if reduce not in ("sum", "mean"):

@@ -96,3 +96,34 @@ def test_residual_norm(cuda):
     leaf = x.clone().requires_grad_(True)
     y, h = res(leaf, f)
     _raises("no derivative", lambda: torch.autograd.grad(h.sum(), [leaf], create_graph=True))
+
+
+def test_captured_while_an_eager_graph_of_the_same_leaves_lives(cuda):
+    """torch's engine ends the process in the backward pass of such a capture; the forward call refuses it."""
+    import cxgnncomp_backend as be
+    x, w = randn((10, 32), 1).cuda(), randn((8, 32), 2).cuda().requires_grad_(True)
+    v = torch.ones(32, device="cuda", requires_grad=True)
+    calls = [lambda: be.linear_kept8(x, w), lambda: be.residual_norm(x, x, next_weight=v)[1]]
+    for call, leaf in zip(calls, (w, v)):
+        kept = call()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(graph):
+                call()
+        del graph
+        want = torch.autograd.grad(kept.sum(), [leaf])[0]
+        del kept
+        graph = torch.cuda.CUDAGraph()  # the same without it
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(call().sum(), [leaf])[0]
+        graph.replay()
+        assert torch.equal(got, want)
+
+
+def test_no_rows(cuda):
+    import cxgnncomp_backend as be
+    x, w = torch.empty(0, 32, device="cuda", requires_grad=True), randn((8, 32), 2).cuda().requires_grad_(True)
+    b = randn((8,), 3).cuda().requires_grad_(True)
+    y = be.linear_kept8(x, w, b)
+    y.sum().backward()
+    assert y.shape == (0, 8) and x.grad.shape == (0, 32) and not bool(w.grad.any()) and not bool(b.grad.any())
