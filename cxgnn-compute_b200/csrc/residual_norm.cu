@@ -47,60 +47,69 @@ struct alignas(16) Ones {
 };
 __device__ const Ones residual_ones{};
 
-// Where a lane's values lie: Q vectors of N values, the lanes' first vectors side by side, then their second ones. Rows that are
-// not whole 16-byte vectors are read value by value, as many per lane.
-template <typename T, bool VEC, int LANES>
+// Where a lane's values lie: Q vectors of N values (VB bytes: the widest that rows are whole in), the lanes' first vectors side by
+// side, then their second ones, and so on.
+template <typename T, int VB, int LANES>
 struct Place {
-  static constexpr int N = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  static constexpr int N = VB / static_cast<int>(sizeof(T));
   static constexpr int Q = kValues / N;
+  static constexpr int kBytes = VB;
   static constexpr int kLanes = LANES;
   using Element = T;
-  static constexpr bool kVec = VEC;
+  static constexpr bool kStaged = VB >= 4;  // there are asynchronous copies of that many bytes
   __device__ __forceinline__ static int column(int p, int i) { return (i / N * LANES + p) * N + i % N; }
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ Pair widened(uint32_t two) { return pair(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u)); }
 
-// Rows on their way: per thread `tensors` x Q slots of 16 bytes for each of two rows.
+// Rows on their way: per thread `tensors` x Q slots of VB bytes for each of two rows.
 template <typename P>
 struct Stage {
   uint32_t base, step;  // this thread's first slot; from a slot to the next
   int tensors;
-  __device__ Stage(const void *smem, int n) : base(shared_address(smem) + threadIdx.x * 16), step(blockDim.x * 16), tensors(n) {}
+  __device__ Stage(const void *smem, int n) : base(shared_address(smem) + threadIdx.x * P::kBytes), step(blockDim.x * P::kBytes), tensors(n) {}
   __device__ __forceinline__ uint32_t slot(int turn, int tensor, int q) const {
     return base + ((turn * tensors + tensor) * P::Q + q) * step;
   }
   // a row's offset in bytes, the lane's part included
   __device__ __forceinline__ void request(int turn, int tensor, const void *matrix, int64_t offset, int p, int width) const {
-    using T = typename P::Element;
 #pragma unroll
     for (int q = 0; q < P::Q; ++q) {
       const bool on = P::column(p, q * P::N) < width;
-      const uint8_t *src = static_cast<const uint8_t *>(matrix) + offset + q * (P::kLanes * 16);
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot(turn, tensor, q)), "l"(on ? src : matrix), "r"(on ? 16 : 0)
-                   : "memory");
+      const uint8_t *src = on ? static_cast<const uint8_t *>(matrix) + offset + q * (P::kLanes * P::kBytes) : static_cast<const uint8_t *>(matrix);
+      if constexpr (P::kBytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot(turn, tensor, q)), "l"(src), "r"(on ? 16 : 0) : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(slot(turn, tensor, q)), "l"(src), "r"(on ? P::kBytes : 0),
+                     "n"(P::kBytes)
+                     : "memory");
     }
   }
   __device__ __forceinline__ void take(int turn, int tensor, Pair (&v)[kPairs]) const {
-    using T = typename P::Element;
+    constexpr int kWords = P::kBytes / 4;
+    uint32_t w[P::Q * kWords];
 #pragma unroll
     for (int q = 0; q < P::Q; ++q) {
-      if constexpr (sizeof(T) == 4) {
-        asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[2 * q]), "=l"(v[2 * q + 1]) : "r"(slot(turn, tensor, q)) : "memory");
-      } else {
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "r"(slot(turn, tensor, q))
-                     : "memory");
+      uint32_t *d = w + q * kWords;
+      if constexpr (kWords == 4)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(slot(turn, tensor, q)) : "memory");
+      else if constexpr (kWords == 2)
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "r"(slot(turn, tensor, q)) : "memory");
+      else
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(d[0]) : "r"(slot(turn, tensor, q)) : "memory");
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-      }
+    for (int i = 0; i < kPairs; ++i) {
+      if constexpr (sizeof(typename P::Element) == 4)
+        v[i] = pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+      else
+        v[i] = widened(w[i]);
     }
   }
 };
 
-// Rows that are not whole vectors, straight from memory.
+// Rows of an odd number of bf16 values, straight from memory.
 template <typename P>
 __device__ __forceinline__ void read_row(Pair (&v)[kPairs], const void *matrix, int64_t row, int p, int width) {
   using T = typename P::Element;
@@ -125,11 +134,25 @@ __device__ __forceinline__ void store_row(void *matrix, int64_t row, int p, int 
 #pragma unroll
   for (int q = 0; q < P::Q; ++q) {
     const int c = P::column(p, q * P::N);
-    if (c < width) {
-      if constexpr (P::kVec)
-        Vec<T>::store_stream(dst + c, Vec<T>::from_float(f + q * P::N));
+    if (c >= width) continue;
+    const float *g = f + q * P::N;
+    if constexpr (P::kBytes == 16) {
+      Vec<T>::store_stream(dst + c, Vec<T>::from_float(g));
+    } else if constexpr (P::N == 1) {
+      dst[c] = from_f32<T>(g[0]);
+    } else if constexpr (sizeof(T) == 4) {
+      __stcs(reinterpret_cast<float2 *>(dst + c), make_float2(g[0], g[1]));
+    } else {
+      uint32_t w[P::N / 2];
+#pragma unroll
+      for (int i = 0; i < P::N / 2; ++i) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(g[2 * i], g[2 * i + 1]);
+        __builtin_memcpy(&w[i], &t, 4);
+      }
+      if constexpr (P::N == 4)
+        __stcs(reinterpret_cast<uint2 *>(dst + c), make_uint2(w[0], w[1]));
       else
-        dst[c] = from_f32<T>(f[q]);
+        __stcs(reinterpret_cast<unsigned *>(dst + c), w[0]);
     }
   }
 }
@@ -138,11 +161,13 @@ __device__ __forceinline__ void store_row(void *matrix, int64_t row, int p, int 
 template <typename P>
 __device__ __forceinline__ void load_param(Pair (&v)[kPairs], const float *w, int p, int width) {
 #pragma unroll
-  for (int i = 0; i < kPairs; i += P::kVec ? 2 : 1) {
+  for (int i = 0; i < kPairs; i += P::N >= 4 ? 2 : 1) {
     const int c = P::column(p, 2 * i);
-    if constexpr (P::kVec) {
+    if constexpr (P::N >= 4) {
       const ulonglong2 t = __ldg(reinterpret_cast<const ulonglong2 *>(w + (c < width ? c : 0)));
       v[i] = t.x, v[i + 1] = t.y;
+    } else if constexpr (P::N == 2) {
+      v[i] = __ldg(reinterpret_cast<const unsigned long long *>(w + (c < width ? c : 0)));
     } else {
       const int e = P::column(p, 2 * i + 1);
       v[i] = pair(__ldg(w + (c < width ? c : 0)), __ldg(w + (e < width ? e : 0)));
@@ -156,7 +181,7 @@ __device__ __forceinline__ void clear_behind(Pair (&v)[kPairs], int p, int width
   if (width == P::kLanes * kValues) return;
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
-    if (P::kVec) {
+    if (P::N > 1) {
       if (P::column(p, 2 * i) >= width) v[i] = 0;
     } else {
       const float2 t = halves(v[i]);
@@ -305,15 +330,15 @@ constexpr int kForwardWarps = 24, kBackwardWarps = 16;
 constexpr int blocks_of(int warps, int threads) { return warps * 32 / threads > 0 ? warps * 32 / threads : 1; }
 // Shared memory of a block for two rows of so many matrices.
 template <typename P>
-constexpr int stage_bytes(int tensors, int threads) { return P::kVec ? 2 * tensors * P::Q * 16 * threads : 0; }
+constexpr int stage_bytes(int tensors, int threads) { return P::kStaged ? 2 * tensors * P::Q * P::kBytes * threads : 0; }
 constexpr int kForwardTensors = 3, kBackwardTensors = 5;
 
 // GATED: a gate per value.
-template <typename T, int LANES, int WARPS, bool VEC, bool GATED>
+template <typename T, int LANES, int WARPS, int VB, bool GATED>
 __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kForwardWarps, WARPS > 1 ? 32 * WARPS : kBlock))
     residual_forward(const __grid_constant__ ResArgs a) {
   constexpr int kLanes = LANES * WARPS;
-  using P = Place<T, VEC, kLanes>;
+  using P = Place<T, VB, kLanes>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float2 place[2][WARPS];
   RowSum<LANES, WARPS> sum(place);
@@ -326,8 +351,8 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kFo
   T rr = from_f32<T>(0.f);
   auto request = [&](int turn, int64_t row) {
     const int64_t at = row < d.n ? row : d.n - 1;
-    if constexpr (VEC) {
-      const int64_t offset = at * width * static_cast<int64_t>(sizeof(T)) + p * 16;
+    if constexpr (P::kStaged) {
+      const int64_t offset = at * width * static_cast<int64_t>(sizeof(T)) + p * VB;
       stage.request(turn, 0, d.x, offset, p, width);
       if (with_f) stage.request(turn, 1, d.f, offset, p, width);
       if (GATED) stage.request(turn, 2, d.gate, offset, p, width);
@@ -343,10 +368,10 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kFo
     const bool in = row < d.n;
     const float g_row = to_f32(rr);
     Pair y[kPairs], n[kPairs], s[kPairs];
-    if constexpr (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if constexpr (P::kStaged) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (row0 + rows.step < n_end) request(turn ^ 1, row + rows.step);
     auto take = [&](Pair(&v)[kPairs], int tensor, const void *matrix) {
-      if constexpr (VEC)
+      if constexpr (P::kStaged)
         stage.take(turn, tensor, v);
       else
         read_row<P>(v, matrix, at, p, width);
@@ -397,7 +422,7 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kFo
         for (int i = 0; i < kPairs; ++i) y[i] = mul2(y[i], w[i]);
       }
       if (in) store_row<P>(d.h, row, p, width, y);
-      if constexpr (VEC) {
+      if constexpr (VB == 16 && P::kLanes * P::N >= rows8::kGroup) {  // the lanes' first vectors hold whole groups
         if (a.keep) keep_row<P>(a, row, in, y, p);
       }
     }
@@ -426,11 +451,11 @@ __device__ __forceinline__ void back_through_norm(Pair (&g)[kPairs], const Pair 
 }
 
 // BIASES: sums for them too.
-template <typename T, int LANES, int WARPS, bool VEC, bool GATED, bool BIASES>
+template <typename T, int LANES, int WARPS, int VB, bool GATED, bool BIASES>
 __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBackwardWarps, WARPS > 1 ? 32 * WARPS : kBlock))
     residual_backward(const __grid_constant__ ResArgs a) {
   constexpr int kLanes = LANES * WARPS;
-  using P = Place<T, VEC, kLanes>;
+  using P = Place<T, VB, kLanes>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float2 place[2][WARPS];
   RowSum<LANES, WARPS> sum(place);
@@ -448,8 +473,8 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
   T rr = from_f32<T>(0.f);
   auto request = [&](int turn, int64_t row) {
     const int64_t at = row < d.n ? row : d.n - 1;
-    if constexpr (VEC) {
-      const int64_t offset = at * width * static_cast<int64_t>(sizeof(T)) + p * 16;
+    if constexpr (P::kStaged) {
+      const int64_t offset = at * width * static_cast<int64_t>(sizeof(T)) + p * VB;
       stage.request(turn, 0, d.x, offset, p, width);
       if (with_f) stage.request(turn, 1, d.f, offset, p, width);
       if (GATED) stage.request(turn, 2, d.gate, offset, p, width);
@@ -465,10 +490,10 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
     const int64_t row = row0 + rows.sub, at = row < d.n ? row : d.n - 1;
     const bool in = row < d.n;  // lanes without a row go through it with gradients of zero
     const float g_row = to_f32(rr);
-    if constexpr (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if constexpr (P::kStaged) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (row0 + rows.step < d.n) request(turn ^ 1, row + rows.step);
     auto take = [&](Pair(&v)[kPairs], int tensor, const void *matrix) {
-      if constexpr (VEC)
+      if constexpr (P::kStaged)
         stage.take(turn, tensor, v);
       else
         read_row<P>(v, matrix, at, p, width);
@@ -612,9 +637,10 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
   }
 }
 
-// Lanes of a row: the smallest power of two, from 8 on, that holds it.
+// Lanes of a row: the smallest power of two, from 2 on, that holds it. (At 8 and more alone, 937500 rows of 16 bf16 values took
+// 393 us instead of 119, forward and backward, and 20 of them 409 instead of 216.)
 int lanes_of(int width) {
-  int lanes = 8;
+  int lanes = 2;
   while (lanes * kValues < width) lanes *= 2;
   return lanes;
 }
@@ -625,27 +651,33 @@ int blocks_for(int64_t n, int lanes, int warps) {
   return static_cast<int>(want < 1 ? 1 : want < most ? want : most);
 }
 
-template <typename T, bool VEC, bool GATED, typename Go>
+template <typename T, int VB, bool GATED, typename Go>
 cudaError_t by_width(int width, Go go) {
   switch (lanes_of(width)) {
-    case 8: return go.template run<T, 8, 1, VEC, GATED>();
-    case 16: return go.template run<T, 16, 1, VEC, GATED>();
-    case 32: return go.template run<T, 32, 1, VEC, GATED>();
-    case 64: return go.template run<T, 32, 2, VEC, GATED>();
-    case 128: return go.template run<T, 32, 4, VEC, GATED>();
-    case 256: return go.template run<T, 32, 8, VEC, GATED>();
-    default: return go.template run<T, 32, 16, VEC, GATED>();
+    case 2: return go.template run<T, 2, 1, VB, GATED>();
+    case 4: return go.template run<T, 4, 1, VB, GATED>();
+    case 8: return go.template run<T, 8, 1, VB, GATED>();
+    case 16: return go.template run<T, 16, 1, VB, GATED>();
+    case 32: return go.template run<T, 32, 1, VB, GATED>();
+    case 64: return go.template run<T, 32, 2, VB, GATED>();
+    case 128: return go.template run<T, 32, 4, VB, GATED>();
+    case 256: return go.template run<T, 32, 8, VB, GATED>();
+    default: return go.template run<T, 32, 16, VB, GATED>();
   }
 }
-template <typename T, typename Go>
-cudaError_t by_kind(const cxg_residual_desc &d, bool vec, Go go) {
-  const bool gated = d.gate_mode == CXG_GATE_VALUE;
-  if (vec) return gated ? by_width<T, true, true>(d.width, go) : by_width<T, true, false>(d.width, go);
-  return gated ? by_width<T, false, true>(d.width, go) : by_width<T, false, false>(d.width, go);
+template <typename T, int VB, typename Go>
+cudaError_t by_gate(const cxg_residual_desc &d, Go go) {
+  return d.gate_mode == CXG_GATE_VALUE ? by_width<T, VB, true>(d.width, go) : by_width<T, VB, false>(d.width, go);
 }
 template <typename Go>
-cudaError_t by_type(const cxg_residual_desc &d, bool vec, Go go) {
-  return d.dtype == CXG_F32 ? by_kind<float>(d, vec, go) : by_kind<__nv_bfloat16>(d, vec, go);
+cudaError_t by_type(const cxg_residual_desc &d, int vb, Go go) {
+  using bf16 = __nv_bfloat16;
+  if (d.dtype == CXG_F32)
+    return vb == 16 ? by_gate<float, 16>(d, go) : vb == 8 ? by_gate<float, 8>(d, go) : by_gate<float, 4>(d, go);
+  return vb == 16  ? by_gate<bf16, 16>(d, go)
+         : vb == 8 ? by_gate<bf16, 8>(d, go)
+         : vb == 4 ? by_gate<bf16, 4>(d, go)
+                   : by_gate<bf16, 2>(d, go);
 }
 
 template <typename P, typename Kernel>
@@ -661,9 +693,9 @@ cudaError_t launch(Kernel kernel, int tensors, int threads, int blocks, const Re
 struct Forward {
   const ResArgs &a;
   cudaStream_t st;
-  template <typename T, int LANES, int WARPS, bool VEC, bool GATED>
+  template <typename T, int LANES, int WARPS, int VB, bool GATED>
   cudaError_t run() const {
-    return launch<Place<T, VEC, LANES * WARPS>>(residual_forward<T, LANES, WARPS, VEC, GATED>, kForwardTensors,
+    return launch<Place<T, VB, LANES * WARPS>>(residual_forward<T, LANES, WARPS, VB, GATED>, kForwardTensors,
                                                 WARPS > 1 ? 32 * WARPS : kBlock,
                                                 blocks_for(a.d.n + a.keep, LANES * WARPS, kForwardWarps), a, st);
   }
@@ -672,15 +704,17 @@ struct Backward {
   const ResArgs &a;
   cudaStream_t st;
   int blocks;
-  template <typename T, int LANES, int WARPS, bool VEC, bool GATED, bool BIASES>
+  template <typename T, int LANES, int WARPS, int VB, bool GATED, bool BIASES>
   cudaError_t go() const {
-    return launch<Place<T, VEC, LANES * WARPS>>(residual_backward<T, LANES, WARPS, VEC, GATED, BIASES>, kBackwardTensors,
+    return launch<Place<T, VB, LANES * WARPS>>(residual_backward<T, LANES, WARPS, VB, GATED, BIASES>, kBackwardTensors,
                                                 WARPS > 1 ? 32 * WARPS : kBlock, blocks, a, st);
   }
-  template <typename T, int LANES, int WARPS, bool VEC, bool GATED>
+  template <typename T, int LANES, int WARPS, int VB, bool GATED>
   cudaError_t run() const {
-    return a.d.post_bias != nullptr || a.d.next_bias != nullptr ? go<T, LANES, WARPS, VEC, GATED, true>()
-                                                                : go<T, LANES, WARPS, VEC, GATED, false>();
+    if constexpr (VB == 16) {
+      if (a.d.post_bias == nullptr && a.d.next_bias == nullptr) return go<T, LANES, WARPS, VB, GATED, false>();
+    }
+    return go<T, LANES, WARPS, VB, GATED, true>();
   }
 };
 
@@ -698,13 +732,19 @@ cudaError_t arguments(const cxg_residual_desc &d, ResArgs *a) {
   return e;
 }
 
-// Rows of whole 16-byte vectors: all matrices, and the parameters, which are fp32.
-bool whole_vectors(const cxg_residual_desc &d) {
-  uint64_t bits = static_cast<uint64_t>(d.width) * (d.dtype == CXG_F32 ? 4 : 2);
-  const void *rows[] = {d.x, d.f, d.y, d.h, d.dy, d.dh, d.dx, d.df, d.scale, d.post_weight, d.post_bias, d.next_weight, d.next_bias};
-  for (const void *p : rows) bits |= reinterpret_cast<uintptr_t>(p);
+// Bytes of the widest vectors that all matrices' rows are whole in; a lane reads as many values of the fp32 parameters, up to
+// four, at once.
+int vector_bytes(const cxg_residual_desc &d) {
+  const int elem = d.dtype == CXG_F32 ? 4 : 2;
+  uint64_t bits = static_cast<uint64_t>(d.width) * elem, params = 0;
+  for (const void *p : {d.x, d.f, static_cast<const void *>(d.y), static_cast<const void *>(d.h), d.dy, d.dh, static_cast<const void *>(d.dx),
+                        static_cast<const void *>(d.df)})
+    bits |= reinterpret_cast<uintptr_t>(p);
   if (d.gate_mode == CXG_GATE_VALUE) bits |= reinterpret_cast<uintptr_t>(d.gate) | reinterpret_cast<uintptr_t>(d.dgate);
-  return bits % 16 == 0;
+  for (const float *p : {d.scale, d.post_weight, d.post_bias, d.next_weight, d.next_bias}) params |= reinterpret_cast<uintptr_t>(p);
+  int vb = 16;
+  while (vb > elem && (bits % vb != 0 || params % (vb / elem < 4 ? vb / elem * 4 : 16) != 0)) vb /= 2;
+  return vb;
 }
 
 int check_desc(const cxg_residual_desc *d, const char *who) {
@@ -727,21 +767,23 @@ using namespace cxg;
 
 extern "C" int cxg_residual_norm_max_width(void) { return kMostWidth; }
 
-extern "C" int cxg_residual_norm_keeps(const cxg_residual_desc *d) { return d != nullptr && whole_vectors(*d) ? 1 : 0; }
+extern "C" int cxg_residual_norm_keeps(const cxg_residual_desc *d) {
+  return d != nullptr && vector_bytes(*d) == 16 && lanes_of(d->width) * (d->dtype == CXG_F32 ? 4 : 8) >= rows8::kGroup ? 1 : 0;
+}
 
 extern "C" int cxg_residual_norm_forward(const cxg_residual_desc *d, void *stream) {
   const int rc = check_desc(d, "cxg_residual_norm_forward");
   if (rc != CXG_OK) return rc;
   const bool keep = d->codes != nullptr;
   CXG_REQUIRE(d->n == 0 || !d->next || d->h != nullptr, CXG_ENULL, "cxg_residual_norm_forward: h is NULL");
-  CXG_REQUIRE(!keep || (d->next && d->scales != nullptr && whole_vectors(*d) && reinterpret_cast<uintptr_t>(d->codes) % 16 == 0),
-              CXG_EINVAL, "cxg_residual_norm_forward: rows in 8 bits are kept of h, in whole 16-byte vectors");
+  CXG_REQUIRE(!keep || (d->next && d->scales != nullptr && cxg_residual_norm_keeps(d) == 1 && reinterpret_cast<uintptr_t>(d->codes) % 16 == 0),
+              CXG_EINVAL, "cxg_residual_norm_forward: rows in 8 bits are kept of h where cxg_residual_norm_keeps says 1");
   if (d->n == 0 && !keep) return CXG_OK;
   CXG_REQUIRE(d->n > 0, CXG_EINVAL, "cxg_residual_norm_forward: no rows to keep");
   ResArgs a;
   cudaError_t e = arguments(*d, &a);
   a.keep = keep ? 1 : 0;
-  if (e == cudaSuccess) e = by_type(*d, whole_vectors(*d), Forward{a, as_stream(stream)});
+  if (e == cudaSuccess) e = by_type(*d, vector_bytes(*d), Forward{a, as_stream(stream)});
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_residual_norm_forward: %s", cudaGetErrorString(e));
   count_launches(1);
   return check_launch("cxg_residual_norm_forward");
@@ -773,7 +815,7 @@ extern "C" int cxg_residual_norm_backward(const cxg_residual_desc *d, float *sum
   cudaError_t e = arguments(*d, &a);
   a.part = static_cast<float *>(workspace);
   const int blocks = blocks_for(d->n, lanes_of(d->width), kBackwardWarps);
-  if (e == cudaSuccess) e = by_type(*d, whole_vectors(*d), Backward{a, st, blocks});
+  if (e == cudaSuccess) e = by_type(*d, vector_bytes(*d), Backward{a, st, blocks});
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_residual_norm_backward: %s", cudaGetErrorString(e));
   column_sum_join(a.part, sums, blocks, kSums * d->width, st);
   count_launches(2);

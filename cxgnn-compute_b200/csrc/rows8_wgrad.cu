@@ -105,8 +105,7 @@ __device__ __forceinline__ void three_parts(const Pair (&v)[4], uint32_t (&hi)[4
   }
 }
 
-// SPANS: 64-column spans of a block of dy. VECTOR: bytes of the vectors that rows of dy are read in, all of them whole (0: value
-// by value). 32-byte vectors of fp32 take half the passes through L1 that pairs of 16-byte ones do.
+// SPANS: 64-column spans of a block of dy. VECTOR: bytes of the vectors that rows of dy are read in, all of them whole. 32-byte vectors of fp32 take half the passes through L1 that pairs of 16-byte ones do.
 template <typename T, int VECTOR, int SPANS>
 __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant__ R8Args a) {
   constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
@@ -192,12 +191,20 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
           asm("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4 % W]), "=r"(v[5 % W]), "=r"(v[6 % W]), "=r"(v[7 % W])
               : "l"(p));
-      } else if constexpr (VECTOR == 16) {
+      } else if constexpr (VECTOR > static_cast<int>(sizeof(T))) {
+        constexpr int kWords = VECTOR / 4, kStep = VECTOR / static_cast<int>(sizeof(T));  // words and values of a vector
 #pragma unroll
-        for (int i = 0; i < W; i += 4)
-          if (gcol + i < a.n) {
-            const uint4 t = __ldg(reinterpret_cast<const uint4 *>(p + i));
-            v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
+        for (int i = 0; i < W / kWords; ++i)
+          if (gcol + i * kStep < a.n) {
+            if constexpr (VECTOR == 16) {
+              const uint4 t = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+              v[4 * i] = t.x, v[4 * i + 1] = t.y, v[4 * i + 2] = t.z, v[4 * i + 3] = t.w;
+            } else if constexpr (VECTOR == 8) {
+              const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p) + i);
+              v[2 * i] = t.x, v[2 * i + 1] = t.y;
+            } else {
+              v[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+            }
           }
       } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -511,13 +518,17 @@ extern "C" int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m,
     if (e == cudaSuccess) e = launch_dependent(kernel, grid, kThreads, smem, st, a);
   };
   auto by_spans = [&](auto one, auto two) { spans == 1 ? go(one) : go(two); };
+  using bf16 = __nv_bfloat16;
   if (dtype == CXG_F32)
     bits % 32 == 0   ? by_spans(rows8_wgrad<float, 32, 1>, rows8_wgrad<float, 32, 2>)
     : bits % 16 == 0 ? by_spans(rows8_wgrad<float, 16, 1>, rows8_wgrad<float, 16, 2>)
-                     : by_spans(rows8_wgrad<float, 0, 1>, rows8_wgrad<float, 0, 2>);
+    : bits % 8 == 0  ? by_spans(rows8_wgrad<float, 8, 1>, rows8_wgrad<float, 8, 2>)
+                     : by_spans(rows8_wgrad<float, 4, 1>, rows8_wgrad<float, 4, 2>);
   else
-    bits % 16 == 0 ? by_spans(rows8_wgrad<__nv_bfloat16, 16, 1>, rows8_wgrad<__nv_bfloat16, 16, 2>)
-                   : by_spans(rows8_wgrad<__nv_bfloat16, 0, 1>, rows8_wgrad<__nv_bfloat16, 0, 2>);
+    bits % 16 == 0  ? by_spans(rows8_wgrad<bf16, 16, 1>, rows8_wgrad<bf16, 16, 2>)
+    : bits % 8 == 0 ? by_spans(rows8_wgrad<bf16, 8, 1>, rows8_wgrad<bf16, 8, 2>)
+    : bits % 4 == 0 ? by_spans(rows8_wgrad<bf16, 4, 1>, rows8_wgrad<bf16, 4, 2>)
+                    : by_spans(rows8_wgrad<bf16, 2, 1>, rows8_wgrad<bf16, 2, 2>);
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_wgrad: %s", cudaGetErrorString(e));
   const int64_t outs = static_cast<int64_t>(k) * n + (db != nullptr ? n : 0);
   const unsigned join_blocks = static_cast<unsigned>((outs + 31) / 32);

@@ -732,7 +732,7 @@ int cxg_residual_norm_max_width(void);
 int cxg_residual_norm_keeps(const cxg_residual_desc *desc);
 int cxg_residual_norm_forward(const cxg_residual_desc *desc, void *stream);
 /* sums: fp32 [5][width], the gradients of scale, post_weight, post_bias, next_weight, next_bias, added in a fixed order (those of
-   biases are zeros where neither is given). */
+   biases that are not given are not to be used). */
 int cxg_residual_norm_backward_workspace_size(int64_t n, int width, size_t *bytes);
 int cxg_residual_norm_backward(const cxg_residual_desc *desc, float *sums, void *workspace, size_t workspace_bytes, void *stream);
 

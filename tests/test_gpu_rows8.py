@@ -26,7 +26,7 @@ def _spread(n, width, seed, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,width", [(1, 1), (3, 4), (5, 31), (1, 32), (17, 33), (40, 47), (33, 64), (21, 100), (9, 257), (300, 128),
-                                     (2, 2000)])
+                                     (2, 2000), (1000, 5), (700, 50), (333, 99), (100, 130)])
 def test_write_and_read(cuda, n, width, dtype):
     import cxgnncomp_backend as be
     x = _spread(n, width, n + width, dtype)

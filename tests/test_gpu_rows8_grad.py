@@ -25,7 +25,8 @@ def _inputs(m, k, n, dtype, seed=0):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (5, 32, 8), (63, 47, 47), (64, 64, 64), (65, 100, 65), (200, 128, 128), (1000, 33, 200),
-                                   (3000, 257, 130), (20000, 100, 47), (40000, 16, 300)])
+                                   (3000, 257, 130), (20000, 100, 47), (40000, 16, 300), (500, 40, 50), (500, 40, 100),
+                                   (300, 64, 180)])
 def test_weight_grad(cuda, m, k, n, dtype):
     import cxgnncomp_backend as be
     x, dy = _inputs(m, k, n, dtype, m)
