@@ -740,8 +740,12 @@ void all_recorded_in_capture(const char *who, const T &...t) {
   (recorded_in_capture(who, t), ...);
 }
 
+// A copy of views that stand for the negative of what is stored.
+Tensor as_stored(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // A matrix of rows that lie any distance apart, each in one piece; a copy of any other.
-Tensor row_matrix(const Tensor &t, const char *name) {
+Tensor row_matrix(const Tensor &t_in, const char *name) {
+  const Tensor t = as_stored(t_in);
   if (!t.is_cuda()) fail(std::string(name) + " must be a CUDA tensor (this backend has no CPU path)");
   if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16)
     fail(std::string(name) + " has dtype " + c10::toString(t.scalar_type()) + ", which this operator does not take");
@@ -816,9 +820,9 @@ void quantize_into(const Tensor &x_in, const Tensor &codes, const Tensor &scales
                                  codes.data_ptr(), scales.data_ptr(), rows, owner->data_ptr<int32_t>(), ws.data(), ws.bytes(), st),
           "cxg_rows8_write_at");
   }
-  // a backward pass that was to read these rows hears of it
-  codes.unsafeGetTensorImpl()->bump_version();
-  scales.unsafeGetTensorImpl()->bump_version();
+  // a backward pass that was to read these rows hears of it (inference tensors cannot be kept for one and count no versions)
+  for (const Tensor *t : {&codes, &scales})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
 at::ScalarType row_type(const std::string &who, at::ScalarType t) {
@@ -861,6 +865,7 @@ Tensor rows8_aggregate(const Tensor &codes, const Tensor &scales, int64_t width,
     f32(*edge_value, "edge_value");
     same_device(codes, *edge_value, "edge_value");
     if (edge_value->numel() != idx.size(0)) fail("rows8_aggregate: one edge value per edge");
+    if (edge_value->is_neg()) fail("rows8_aggregate: edge_value is a view that stands for its negative: resolve_neg() it first");
   }
   c10::cuda::CUDAGuard guard(codes.device());
   Tensor y = at::empty({n, width}, codes.options().dtype(type));
@@ -926,7 +931,7 @@ class LinearKept8Function : public torch::autograd::Function<LinearKept8Function
     if (at::GradMode::is_enabled()) fail("linear_kept8: the rows it keeps in 8 bits have no second derivative");
     const auto saved = ctx->get_saved_variables();
     const Tensor &w = saved[0];
-    const Tensor g = grads[0].contiguous();
+    const Tensor g = as_stored(grads[0]).contiguous();
     c10::cuda::CUDAGuard guard(g.device());
     Tensor dx, dw, db;
     const bool bias = ctx->saved_data["bias"].toBool(), need_db = bias && ctx->needs_input_grad(2);
@@ -975,6 +980,9 @@ Tensor linear_kept8(Tensor x, Tensor w, optional<Tensor> bias, optional<Tensor> 
       fail("linear_kept8: kept must hold the rows of x");
   }
   c10::cuda::CUDAGuard guard(x.device());
+  x = as_stored(x), w = as_stored(w);
+  if (bias) bias = as_stored(*bias);
+  if (add) add = as_stored(*add);
   all_recorded_in_capture("linear_kept8", x, w, bias, add);
   c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);
   if (recorded(x, w, bias, add))
@@ -1074,8 +1082,8 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
     cxg_residual_desc d = describe_residual(x, f, given(2), given(3), given(4), given(5), given(6), given(7), o);
     const int h_at = f ? 1 : 0;
     Tensor dy, dh;
-    if (f && grads[0].defined()) dy = grads[0].contiguous();
-    if (o.next && grads[h_at].defined()) dh = grads[h_at].contiguous();
+    if (f && grads[0].defined()) dy = as_stored(grads[0]).contiguous();
+    if (o.next && grads[h_at].defined()) dh = as_stored(grads[h_at]).contiguous();
     variable_list out(13);
     if (!dy.defined() && !dh.defined()) return out;
     d.dy = dy.defined() ? dy.data_ptr() : nullptr;
@@ -1111,7 +1119,7 @@ optional<Tensor> row_parameter(const optional<Tensor> &t, const Tensor &x, const
   Tensor v = t->to(at::kFloat);
   if (std::string(name) == "scale" && v.numel() == 1) v = v.reshape({1}).expand({x.size(1)});
   if (v.dim() != 1 || v.size(0) != x.size(1)) fail(std::string("residual_norm: ") + name + " must be [" + std::to_string(x.size(1)) + "]");
-  return v.contiguous();
+  return as_stored(v).contiguous();
 }
 
 std::vector<optional<Tensor>> residual_norm(const Tensor &x_in, const optional<Tensor> &f_in, const optional<Tensor> &gate_in,
@@ -1120,11 +1128,13 @@ std::vector<optional<Tensor>> residual_norm(const Tensor &x_in, const optional<T
                                             const optional<Tensor> &next_bias, bool layer, double eps, bool keep) {
   if (for_torch(x_in, f_in, gate_in, scale_in, post_weight, post_bias, next_weight, next_bias))
     fail(std::string("residual_norm") + kTransform);
-  auto rows = [&](const Tensor &t, const char *name) {
+  const bool autocast = at::autocast::is_autocast_enabled(at::kCUDA);
+  auto rows = [&](Tensor t, const char *name) {
     if (!t.is_cuda()) fail(std::string(name) + " must be a CUDA tensor (this backend has no CPU path)");
+    if (autocast && t.is_floating_point()) t = t.to(x_in.scalar_type());  // what a block returns may be of another type than x
     if (t.scalar_type() != x_in.scalar_type()) fail(std::string("residual_norm: ") + name + " must be of x's type");
     same_device(x_in, t, name);
-    return t.contiguous();
+    return as_stored(t).contiguous();
   };
   row_type("residual_norm", x_in.scalar_type());
   if (x_in.dim() != 2 || x_in.size(1) == 0) fail("residual_norm: x must be a matrix with at least one column");

@@ -16,6 +16,8 @@ import os
 import numpy as np
 import torch
 
+import cxgnncomp_backend
+
 
 class Batch:
 
@@ -45,10 +47,12 @@ class Batch:
     def tofile(self, directory):
         """Writes the set fields as raw arrays, byte for byte what the reference writes: the tensor's own dtype
         and layout (`tensor.cpu().numpy().tofile`), so float32 features and int64 indices give the documented
-        format. The directory is created when missing."""
+        format (a cxgnncomp_backend.Rows8 as the float32 values it holds). The directory is created when missing."""
         os.makedirs(directory, exist_ok=True)
         for name in ("x", "ptr", "idx", "target"):
             t = getattr(self, name)
+            if isinstance(t, cxgnncomp_backend.Rows8):
+                t = cxgnncomp_backend.dequantize_rows(t)
             if t is not None:
                 t.detach().cpu().contiguous().numpy().tofile(os.path.join(directory, name + ".dat"))
 

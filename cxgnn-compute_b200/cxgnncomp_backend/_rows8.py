@@ -132,8 +132,9 @@ def residual_norm(x, f=None, gate=None, scale=None, post=True, post_weight=None,
 
     x, f: float32 or bfloat16 [n, width], width up to 4096. gate: [n, width], or [n] or [n, 1], or None (a factor of 1). scale:
     [width] or one value. norm: "rms" (v / sqrt(mean v^2 + eps)) or "layer" (the mean taken off first). Parameters may be of
-    any floating type and count as float32; missing ones are 1 or 0. Without f: (x, norm of x). With keep8=True the result is
-    (y, h, quantize_rows(h)), in the same pass. Differentiable once in everything but the rows in 8 bits."""
+    any floating type and count as float32; missing ones are 1 or 0. Under autocast f and gate are taken in x's type. Without
+    f: (x, norm of x). With keep8=True the result is (y, h, quantize_rows(h)), in the same pass. Differentiable once in
+    everything but the rows in 8 bits."""
     if norm not in ("rms", "layer"):
         raise RuntimeError(f"residual_norm: norm must be 'rms' or 'layer', not {norm!r}")
     y, h, codes, scales = _native.residual_norm(x, f, gate, scale, bool(post), post_weight, post_bias, bool(next), next_weight,

@@ -182,3 +182,28 @@ def test_other_blocks(cuda, conv):
     out = model(_batch(randn((N, 20), 5).cuda(), 2))
     out.sum().backward()
     assert out.shape == (N, 7) and all(bool(torch.isfinite(p.grad).all()) for p in model.parameters() if p.grad is not None)
+
+
+@pytest.mark.parametrize("conv,gate,kept8", [("sage", "row", True), ("sage", "value", False), ("gcn", "row", False), ("gcn", None, False),
+                                             ("gin", "value", False)])
+def test_under_autocast(cuda, conv, gate, kept8):
+    import cxgnncomp
+    torch.manual_seed(1)
+    model = cxgnncomp.ResidualGNN(conv, 20, 32, 7, 2, gate=gate, kept8=kept8).cuda()
+    batch = _batch(randn((N, 20), 5).cuda(), 2)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = F.nll_loss(model(batch).float(), torch.zeros(N, dtype=torch.int64, device="cuda"))
+    loss.backward()
+    grads = [p.grad for p in model.parameters() if p.grad is not None]
+    assert len(grads) > 5 and all(g.dtype == torch.float32 and bool(torch.isfinite(g).all()) for g in grads)
+
+
+def test_features_in_8_bits_on_disk(cuda, tmp_path):
+    """The wire format has float32 features: those that the rows hold."""
+    import cxgnncomp
+    import cxgnncomp_backend as be
+    x = randn((N, 20), 5)
+    batch = _batch(be.quantize_rows(x.cuda()), 2)
+    batch.tofile(str(tmp_path))
+    back = cxgnncomp.Batch(None, None, None).fromfile(str(tmp_path), feat_len=20)
+    assert back.x.dtype == torch.float32 and torch.equal(back.x.double(), held_values(x)) and torch.equal(back.idx, batch.idx.cpu())

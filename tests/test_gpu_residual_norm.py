@@ -97,8 +97,7 @@ def test_parts(cuda, post, following, scale, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,width", [(700, 16), (300, 8), (500, 20), (33, 32), (40, 200), (300, 256), (30, 257), (20, 512), (9, 1000),
-                                     (7, 1500), (5, 2048), (3, 4096),
-                                     (3, 4001)])
+                                     (7, 1500), (5, 2048), (3, 4096), (3, 4001)])
 def test_widths(cuda, n, width, dtype):
     _check(n, width, dtype, "value", True, True, True)
 
@@ -226,3 +225,17 @@ def test_bf16_parameters_no_rows_and_views(cuda):
     a = be.residual_norm(wide[:, 1:65], wide[:, 65:129])
     b = be.residual_norm(wide[:, 1:65].contiguous(), wide[:, 65:129].contiguous())
     assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_under_autocast(cuda):
+    """f and gate are taken in x's type; without autocast they have to be of it."""
+    import cxgnncomp_backend as be
+    x, f, gate = randn((50, 48), 1).cuda().bfloat16(), randn((50, 48), 2).cuda().requires_grad_(True), randn((50,), 3).cuda()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y, h = be.residual_norm(x, f, gate=gate)
+    want = be.residual_norm(x, f.detach().bfloat16(), gate=gate.bfloat16())
+    assert torch.equal(y, want[0]) and torch.equal(h, want[1])
+    h.sum().backward()
+    assert f.grad.dtype == torch.float32
+    with pytest.raises(RuntimeError, match="f must be of x's type"):
+        be.residual_norm(x, f)

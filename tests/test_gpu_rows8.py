@@ -185,3 +185,36 @@ def test_another_stream_and_a_captured_write(cuda):
     ids.copy_(at[2])
     graph.replay()
     assert _same(read, expect([0, 1, 2]))
+
+
+def test_a_cache_made_in_inference_mode(cuda):
+    """Written and read like any other, in inference mode and outside."""
+    import cxgnncomp_backend as be
+    x = _spread(30, 40, 3, torch.float32)
+    with torch.inference_mode():
+        cache = be.Rows8(50, 40)
+        be.quantize_rows(x[:9].cuda(), out=cache)
+    at = torch.arange(20, 50)
+    be.quantize_rows(x.cuda(), out=cache, index=at.cuda())
+    assert _same(be.dequantize_rows(cache, index=at.cuda()), held_values(x))
+    assert _same(be.dequantize_rows(cache, num_rows=9), held_values(x[:9]))
+
+
+def test_views_that_stand_for_their_negative(cuda):
+    import cxgnncomp_backend as be
+    x = randn((40, 33), 7).cuda()
+    v = torch._neg_view(x)
+    assert _same(be.dequantize_rows(be.quantize_rows(v)), held_values(-x.cpu()))
+    rows = be.quantize_rows(x)
+    dy = randn((40, 17), 8).cuda()
+    assert torch.equal(be.rows8_weight_grad(rows, torch._neg_view(dy)), be.rows8_weight_grad(rows, -dy))
+    w = randn((17, 33), 9).cuda()
+    assert torch.equal(be.linear_kept8(v, torch._neg_view(w)), be.linear_kept8(-x, -w))
+    f = randn((40, 33), 10).cuda()
+    scale = randn((33,), 11).cuda()
+    a = be.residual_norm(v, torch._neg_view(f), gate=torch._neg_view(f), scale=torch._neg_view(scale))
+    b = be.residual_norm(-x, -f, gate=-f, scale=-scale)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    ptr, idx = torch.tensor([0, 2, 3]).cuda(), torch.tensor([1, 2, 3]).cuda()
+    with pytest.raises(RuntimeError, match="resolve_neg"):
+        be.rows8_aggregate(rows, ptr, idx, 2, edge_value=torch._neg_view(torch.ones(3, device="cuda")))
