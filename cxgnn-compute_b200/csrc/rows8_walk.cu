@@ -26,7 +26,27 @@ struct Rows8Args {
   int64_t n_src;  // rows; ids outside stand for the row of zeros behind the last
   int groups;
   int whole;  // 2: rows of y are whole 16-byte vectors, 1: 8-byte ones
+  uint2 *marks;  // SPARSE: per edge that is the first of its row, that row and its end
 };
+
+// For graphs of mostly empty rows: y is zeroed here, and the walk goes from a row to the next one that has edges.
+template <typename T>
+__global__ void __launch_bounds__(256) rows8_mark(const __grid_constant__ Rows8Args r) {
+  const WalkArgs &a = r.w;
+  dependency_wait();
+  const int64_t i0 = blockIdx.x * 256ll + threadIdx.x, step = gridDim.x * 256ll;
+  const uint32_t e_total = static_cast<uint32_t>(edge_total(a));
+  for (int64_t i = i0; i < a.n_dst; i += step) {
+    const uint32_t b = walk::load_ptr_low(a.ptr, static_cast<int>(i), a.ptr_bytes), e = walk::load_ptr_low(a.ptr, static_cast<int>(i) + 1, a.ptr_bytes);
+    if (b < e && b < e_total) r.marks[b] = make_uint2(static_cast<uint32_t>(i), e);
+  }
+  const int64_t values = a.n_dst * a.width;
+  constexpr int N = Vec<T>::kElems;
+  T *y = static_cast<T *>(a.y);
+  const int64_t vectors = reinterpret_cast<uintptr_t>(y) % 16 == 0 ? values / N : 0;
+  for (int64_t i = i0; i < vectors; i += step) *reinterpret_cast<uint4 *>(y + i * N) = make_uint4(0, 0, 0, 0);
+  for (int64_t i = vectors * N + i0; i < values; i += step) y[i] = from_f32<T>(0.f);
+}
 
 template <int VB>
 struct Codes {
@@ -67,7 +87,7 @@ __device__ __forceinline__ void add_codes(unsigned long long *acc, const Codes<V
 
 // VALMODE: 0 sum, 1 a value per edge, 3 mean. WORDS: the (up to four) scales of an edge's row as one word, fetched with the ids by
 // one lane per edge; otherwise every lane fetches its own with the codes.
-template <typename T, int VB, int G, int NV, int U, int VALMODE, int MINB, bool WORDS>
+template <typename T, int VB, int G, int NV, int U, int VALMODE, int MINB, bool WORDS, bool SPARSE>
 __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_constant__ Rows8Args r) {
   const WalkArgs &a = r.w;
   constexpr int NG = 32 / G;
@@ -120,6 +140,7 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
   };
   const int t_first = static_cast<int>((blockIdx.x * static_cast<unsigned>(kThreads) + threadIdx.x) / G);
   if (e_total == 0) {  // no edge at all: every row is empty
+    if constexpr (SPARSE) return;
     for (int row = t_first; row < n_dst; row += step) zero_row(row);
     return;
   }
@@ -184,17 +205,19 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
     };
     int rend = kFar, rstart = 0, stop = kFar;
     uint32_t next_raw = 0;
+    [[maybe_unused]] uint2 next_mark = make_uint2(0, 0);
+    auto fetch_mark = [&]() {
+      if (rend < len) next_mark = __ldg(r.marks + begin + rend);
+    };
     if (len > 0) {
-      if (t == 0)
+      if (t == 0 && !SPARSE)
         for (int i = 0; i < row; ++i) zero_row(i);  // leading rows without edges
       rstart = row_begin < begin ? -1 : 0;
-      next_raw = end_raw(row + 1);
       rend = end_rel(row, row_end);
-      while (rend == 0) {  // empty rows that the previous tile's walk wrote
-        ++row;
-        rend = end_rel(row, next_raw);
+      if constexpr (SPARSE)
+        fetch_mark();
+      else
         next_raw = end_raw(row + 1);
-      }
       stop = min(rend, len);
     }
     unsigned long long acc[NV][VB / 2];
@@ -236,12 +259,18 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
       }
       if (row_done) {
         rstart = pos;
-        for (;;) {
-          ++row;
-          rend = end_rel(row, next_raw);
-          next_raw = end_raw(row + 1);
-          if (rend != pos) break;
-          zero_row(row);  // a row without edges
+        if constexpr (SPARSE) {
+          row = static_cast<int>(min(next_mark.x, static_cast<uint32_t>(n_dst)));
+          rend = pos < len ? end_rel(row, next_mark.y) : kFar;
+          fetch_mark();
+        } else {
+          for (;;) {
+            ++row;
+            rend = end_rel(row, next_raw);
+            next_raw = end_raw(row + 1);
+            if (rend != pos) break;
+            zero_row(row);  // a row without edges
+          }
         }
       }
       stop = pos == len ? kFar : min(rend, len);
@@ -322,9 +351,10 @@ bool launch_pitch(const Rows8Args &r, cudaStream_t st, int *resident) {
     if (grid > most) grid = most;
     return launch_dependent(kernel, static_cast<unsigned>(grid < 1 ? 1 : grid), kThreads, 0, st, r) == cudaSuccess;
   };
-#define CXG_ROWS8_WALK(VB, G, NV, U, CTAS, WORDS) \
-  if (r.w.row_bytes <= VB * G * NV)               \
-  return go(rows8_walk<T, VB, G, NV, U, VALMODE, CTAS, WORDS>, G, CTAS)
+#define CXG_ROWS8_WALK(VB, G, NV, U, CTAS, WORDS)                                           \
+  if (r.w.row_bytes <= VB * G * NV)                                                         \
+  return r.marks != nullptr ? go(rows8_walk<T, VB, G, NV, U, VALMODE, CTAS, false, true>, G, CTAS) \
+                            : go(rows8_walk<T, VB, G, NV, U, VALMODE, CTAS, WORDS, false>, G, CTAS)
   // Scales as words: 10.7 M edges, 32 columns bf16 214 -> 205 us, 100 fp32 with values 429 -> 405; 128 columns bf16 without values
   // 364 -> 374.
   CXG_ROWS8_WALK(4, 8, 1, 8, 8, true);
@@ -351,14 +381,25 @@ bool dispatch(const Rows8Args &r, int out_dtype, cudaStream_t st, int *resident)
 
 constexpr int kMostWidth = 2048;
 // Graphs for one launch of clusters: one / three launches (us), mean, fp32: 13,264 edges, 33 columns 18.4 / 31.6, 256 20.4 / 31.7;
-// 40,000 edges, 128 24.6 / 37.9, 256 30.7 / 37.9; 60,000, 128 28.6 / 37.9, 256 36.8 / 35.9; 84,000, 64 34.8 / 33.9.
-constexpr int64_t kSmallEdges = 65536, kSmallBytes = 12 << 20;
+// 40,000 edges, 128 24.6 / 37.9, 256 30.7 / 37.9; 60,000, 128 28.6 / 37.9, 256 36.8 / 35.9; 84,000, 64 34.8 / 33.9. Against the
+// launches for sparse graphs below: 100 columns bf16, 8192 rows and 2000 edges 22.6 / 23.3, 300 edges 67.6 / 21.6.
+constexpr int64_t kSmallEdges = 65536, kSmallBytes = 12 << 20, kSmallRowsPerEdge = 4;
 
 int tile_edges(const Rows8Args &r, int64_t nnz, int split_edges) {
   if (split_edges > 0) return split_edges;
   int resident = kNumSM * 32;
   dispatch(r, CXG_F32, nullptr, &resident);
   return walk_tile_of_waves(nnz, resident);
+}
+
+// Graphs with more rows than edges: most rows are empty, and a walk that looks at each of a tile's rows takes 0.2 us for each. (All
+// rows / those with edges, us: 1.9 M rows and 1000 edges, 100 columns bf16 33,100 / 99; 300,000 and 100,000 122 / 47; 300,000
+// and 300,000 77 / 63, 128 columns fp32 83 / 88; 500,000 edges 79 / 105.) With more edges than kMostMarked the tiles of one
+// wave have few rows each. In small tiles, as a row's end is what takes time (64 edges: 59 us where 16 take 32).
+constexpr int64_t kMostMarked = 1 << 19;
+bool is_sparse(int64_t n_dst, int64_t nnz) { return nnz <= kMostMarked && n_dst > nnz; }
+int sparse_tile(int64_t nnz, int width, int split_edges) {
+  return split_edges > 0 ? split_edges : width > 512 ? 64 : nnz <= (1 << 18) ? 16 : 32;
 }
 
 }  // namespace
@@ -373,9 +414,14 @@ extern "C" int cxg_rows8_aggregate_workspace_size(int64_t nnz, int width, int sp
   Rows8Args r = {};
   r.w.row_bytes = rows8::groups_of(width) * rows8::kGroup;
   WalkLayout L;
-  const int rc = walk_layout(nnz, walk_part_stride(width), tile_edges(r, nnz, split_edges), &L);
+  int rc = walk_layout(nnz, walk_part_stride(width), tile_edges(r, nnz, split_edges), &L);
   if (rc != CXG_OK) return set_error(rc, "cxg_rows8_aggregate: graph too large for 32-bit tile ids");
   *bytes = L.total;
+  if (nnz <= kMostMarked) {  // how many rows there are is not known here
+    rc = walk_layout(nnz, walk_part_stride(width), sparse_tile(nnz, width, split_edges), &L);
+    const size_t need = L.total + static_cast<size_t>(nnz) * sizeof(uint2);
+    if (rc == CXG_OK && need > *bytes) *bytes = need;
+  }
   return CXG_OK;
 }
 
@@ -406,13 +452,15 @@ extern "C" int cxg_rows8_aggregate(const void *codes, const void *scales, int64_
   r.n_src = n_src, r.groups = rows8::groups_of(width);
   const uint64_t bits = static_cast<uint64_t>(width) * (y_dtype == CXG_F32 ? 4 : 2) | reinterpret_cast<uintptr_t>(y);
   r.whole = bits % 16 == 0 ? 2 : bits % 8 == 0 ? 1 : 0;
-  a.tile = tile_edges(r, nnz, split_edges);
+  const bool marked = is_sparse(n_dst, nnz);
+  a.tile = marked ? sparse_tile(nnz, width, split_edges) : tile_edges(r, nnz, split_edges);
   a.part_stride = static_cast<int>(walk_part_stride(width));
   WalkLayout L;
   const int rc = walk_layout(nnz, a.part_stride, a.tile, &L);
   if (rc != CXG_OK) return set_error(rc, "cxg_rows8_aggregate: graph too large for 32-bit tile ids");
-  CXG_REQUIRE(workspace != nullptr && workspace_bytes >= L.total && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, CXG_EWORKSPACE,
-              "cxg_rows8_aggregate: workspace %zu bytes, need %zu", workspace_bytes, L.total);
+  const size_t need = L.total + (marked ? static_cast<size_t>(nnz) * sizeof(uint2) : 0);
+  CXG_REQUIRE(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, CXG_EWORKSPACE,
+              "cxg_rows8_aggregate: workspace %zu bytes, need %zu", workspace_bytes, need);
   char *ws = static_cast<char *>(workspace);
   a.hdr = reinterpret_cast<int32_t *>(ws + L.hdr);
   a.tiles = ws + L.tiles;
@@ -421,13 +469,24 @@ extern "C" int cxg_rows8_aggregate(const void *codes, const void *scales, int64_
   a.max_tiles = L.max_tiles;
   cudaStream_t st = as_stream(stream);
   // small graphs, as those of cxg_spmm_csr, in one launch of clusters
-  if (nnz <= kSmallEdges && nnz * a.x_pitch <= kSmallBytes && n_dst <= small_most_rows() && width <= 256 && a.tile == 64) {
+  if (nnz <= kSmallEdges && nnz * a.x_pitch <= kSmallBytes && n_dst <= small_most_rows() && n_dst <= kSmallRowsPerEdge * nnz + 64 &&
+      width <= 256 && (split_edges == 0 || split_edges == 64)) {
     WalkArgs small = a;
+    small.tile = 64;
     small.x = codes, small.x_rows = scales, small.rel_stride = n_src;
     if (small_launch_rows8(small, y_dtype, st)) {
       count_launches(1);
       return check_launch("cxg_rows8_aggregate (small)");
     }
+  }
+  if (marked) {
+    r.marks = reinterpret_cast<uint2 *>(ws + L.total);
+    const int64_t blocks = (n_dst + 255) / 256;
+    const unsigned grid = static_cast<unsigned>(blocks < kNumSM * 8 ? blocks : kNumSM * 8);
+    const cudaError_t e = y_dtype == CXG_F32 ? launch_dependent(rows8_mark<float>, grid, 256, 0, st, r)
+                                             : launch_dependent(rows8_mark<__nv_bfloat16>, grid, 256, 0, st, r);
+    if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_aggregate: %s", cudaGetErrorString(e));
+    count_launches(1);
   }
   walk_plan_run(a, st);
   if (!dispatch(r, y_dtype, st, nullptr)) return set_error(CXG_ECUDA, "cxg_rows8_aggregate: %s", cudaGetErrorString(cudaGetLastError()));

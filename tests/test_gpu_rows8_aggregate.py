@@ -64,6 +64,31 @@ def test_rows_without_edges_and_first_rows(cuda):
     assert be.rows8_aggregate(rows, ptr[:1].cuda(), idx.cuda(), 0).shape == (0, 40)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduce", ["sum", "mean", "value"])
+@pytest.mark.parametrize("n,edges,width", [(1000, 1, 33), (3000, 200, 4), (3000, 700, 100), (30000, 5000, 47), (30000, 29000, 128),
+                                           (9000, 2000, 300), (2000, 400, 900), (100000, 70000, 16)])
+def test_graphs_of_mostly_empty_rows(cuda, n, edges, width, reduce, dtype):
+    """More rows than edges: whole tiles of one row, rows that tiles cut, empty rows in front, between and behind."""
+    import cxgnncomp_backend as be
+    gen = torch.Generator().manual_seed(edges)
+    dst = torch.randint(n // 10, n - n // 10, (edges,), generator=gen)
+    dst[: edges // 4] = n // 2
+    ptr = torch.zeros(n + 1, dtype=torch.int64)
+    ptr[1:] = torch.bincount(dst, minlength=n).cumsum(0)
+    idx = torch.randint(0, 500, (edges,), generator=gen)
+    if width % 2:
+        ptr, idx = ptr.int(), idx.int()
+    x = randn((500, width), width)
+    ev = torch.rand(edges, generator=gen) - 0.3 if reduce == "value" else None
+    kind = "mean" if reduce == "mean" else "sum"
+    rows = be.quantize_rows(x.cuda())
+    got = be.rows8_aggregate(rows, ptr.cuda(), idx.cuda(), 0, reduce=kind, edge_value=None if ev is None else ev.cuda(), dtype=dtype)
+    assert _close(got, *aggregate(held_values(x), ptr, idx, kind, ev))
+    again = be.rows8_aggregate(rows, ptr.cuda(), idx.cuda(), 0, reduce=kind, edge_value=None if ev is None else ev.cuda(), dtype=dtype)
+    assert torch.equal(got, again)
+
+
 def test_ids_outside_and_groups_that_are_not_finite(cuda):
     import cxgnncomp_backend as be
     x = randn((20, 96), 1)
