@@ -105,4 +105,21 @@ __device__ __forceinline__ void code_values(float *f, uint32_t word) {
 }
 
 }  // namespace rows8
+
+// The weight gradient for a dy of few columns, one row behind the other (rows8_wgrad_narrow.cu); scales and dy 16-byte aligned. Its
+// sums: [parts][columns][128] and [parts][n].
+struct Rows8Narrow {
+  const uint8_t *codes, *scales;
+  const void *dy;
+  int64_t m;
+  int k, n, pitch, groups;
+  uint32_t inverse;  // floor(2^32 / n)
+  float *partial, *partial_db;
+};
+struct Rows8NarrowPlan {
+  int columns, parts;  // columns 0: not for these sizes
+};
+Rows8NarrowPlan rows8_narrow_plan(int64_t m, int k, int n);
+cudaError_t rows8_narrow_run(const Rows8Narrow &a, const Rows8NarrowPlan &plan, int dtype, cudaStream_t st);
+
 }  // namespace cxg

@@ -7,8 +7,7 @@
 //
 // The contraction runs over rows, so both operands are "MN-major": a stage holds 64 rows of the input (A: 128 columns, two
 // spans of 128 bytes per row in a 128-byte swizzle) and of dy (B: hi, then mid, then lo spans). Both are made in registers:
-// producer warps load 16 bytes at a time a whole stage ahead, convert, and write the operands where the tensor core reads
-// them. One instruction multiplies A by [hi | mid], another adds A by lo to mid's accumulator. An accumulator takes
+// producer warps load 16 bytes at a time two stages ahead, convert, and write the operands where the tensor core reads them. One instruction multiplies A by [hi | mid], another adds A by lo to mid's accumulator. An accumulator takes
 // `chunk` stages, as the tensor core's additions cut off what an fp32 addition rounds (its error grows with the number of
 // additions); the epilogue warps, each lane a column of the input, add the chunks up in shared memory.
 //
@@ -408,12 +407,12 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
   }
 }
 
-// dw[o][i] and db[o]: warp q of a block adds the partials q, q + 8, ... of 32 outputs, the eight sums are added in order. (A thread
+// dw[o][i] and db[o] from [pair of column blocks][parts][per columns of dy][128 columns of the input]: warp q of a block adds the partials q, q + 8, ... of 32 outputs, the eight sums are added in order. (A thread
 // per output and all its partials took 11 us for 148 partials of 128 x 100, a chain of loads.)
 constexpr int kJoinWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps) rows8_wgrad_join(const float *partial, const float *partial_db, T *dw, T *db, int k,
-                                                                    int n, int k_blocks, int parts) {
+                                                                    int n, int k_blocks, int parts, int per) {
   dependency_wait();
   __shared__ float side[kJoinWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -423,8 +422,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) rows8_wgrad_join(const float 
   if (i < kn) {
     const int o = static_cast<int>(i / k), c = static_cast<int>(i % k);
     const int64_t pair = c / 128 + static_cast<int64_t>(k_blocks) * (o / 128);
-    p = partial + (pair * parts * 128 + o % 128) * 128 + c % 128;
-    step = 128 * 128;
+    p = partial + (pair * parts * per + o % 128) * 128 + c % 128;
+    step = per * 128;
   } else if (db != nullptr && i < kn + n) {
     p = partial_db + (i - kn);
     step = n;
@@ -459,6 +458,18 @@ int parts_of(int k, int n, int64_t m) {
   return static_cast<int>(parts < tiles ? parts : tiles);
 }
 
+template <typename... P>
+void launch_join(int out_dtype, cudaStream_t st, const float *partial, const float *partial_db, void *dw, void *db, int k, int n, P... p) {
+  const int64_t outs = static_cast<int64_t>(k) * n + (db != nullptr ? n : 0);
+  const unsigned blocks = static_cast<unsigned>((outs + 31) / 32);
+  if (out_dtype == CXG_F32)
+    launch_dependent(rows8_wgrad_join<float>, blocks, 32 * kJoinWarps, 0, st, partial, partial_db, static_cast<float *>(dw),
+                     static_cast<float *>(db), k, n, p...);
+  else
+    launch_dependent(rows8_wgrad_join<__nv_bfloat16>, blocks, 32 * kJoinWarps, 0, st, partial, partial_db,
+                     static_cast<__nv_bfloat16 *>(dw), static_cast<__nv_bfloat16 *>(db), k, n, p...);
+}
+
 }  // namespace
 }  // namespace cxg
 
@@ -467,8 +478,10 @@ using namespace cxg;
 extern "C" int cxg_rows8_wgrad_workspace_size(int64_t m, int k, int n, size_t *bytes) {
   CXG_REQUIRE(bytes != nullptr, CXG_ENULL, "cxg_rows8_wgrad_workspace_size: bytes is NULL");
   CXG_REQUIRE(m >= 0 && k > 0 && n > 0, CXG_EINVAL, "cxg_rows8_wgrad_workspace_size: bad sizes");
+  const Rows8NarrowPlan narrow = rows8_narrow_plan(m, k, n);
   const size_t pairs = static_cast<size_t>((k + 127) / 128) * ((n + 127) / 128), parts = static_cast<size_t>(parts_of(k, n, m));
-  *bytes = parts * (pairs * 128 * 128 + n) * sizeof(float);
+  const size_t need = parts * (pairs * 128 * 128 + n), few = static_cast<size_t>(narrow.parts) * (narrow.columns * 128 + n);
+  *bytes = (need > few ? need : few) * sizeof(float);
   return CXG_OK;
 }
 
@@ -494,6 +507,19 @@ extern "C" int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m,
   cxg_rows8_wgrad_workspace_size(m, k, n, &need);
   CXG_REQUIRE(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, CXG_EWORKSPACE,
               "cxg_rows8_wgrad: workspace %zu bytes, need %zu", workspace_bytes, need);
+  const Rows8NarrowPlan narrow = rows8_narrow_plan(m, k, n);
+  if (narrow.columns > 0 && ld == n && (reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(scales)) % 16 == 0) {
+    Rows8Narrow a = {};
+    a.codes = static_cast<const uint8_t *>(codes), a.scales = static_cast<const uint8_t *>(scales), a.dy = dy;
+    a.m = m, a.k = k, a.n = n, a.groups = rows8::groups_of(k), a.pitch = a.groups * kGroup;
+    a.partial = static_cast<float *>(workspace);
+    a.partial_db = db != nullptr ? a.partial + static_cast<size_t>(narrow.parts) * narrow.columns * 128 : nullptr;
+    const cudaError_t e = rows8_narrow_run(a, narrow, dtype, st);
+    if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_wgrad: %s", cudaGetErrorString(e));
+    launch_join(out_dtype, st, a.partial, a.partial_db, dw, db, k, n, 1, narrow.parts, narrow.columns);
+    count_launches(2);
+    return check_launch("cxg_rows8_wgrad (narrow)");
+  }
   const int parts = parts_of(k, n, m), elem = dtype == CXG_F32 ? 4 : 2;
   R8Args a = {};
   a.codes = static_cast<const uint8_t *>(codes), a.scales = static_cast<const uint8_t *>(scales), a.dy = dy;
@@ -530,14 +556,7 @@ extern "C" int cxg_rows8_wgrad(const void *codes, const void *scales, int64_t m,
     : bits % 4 == 0 ? by_spans(rows8_wgrad<bf16, 4, 1>, rows8_wgrad<bf16, 4, 2>)
                     : by_spans(rows8_wgrad<bf16, 2, 1>, rows8_wgrad<bf16, 2, 2>);
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_wgrad: %s", cudaGetErrorString(e));
-  const int64_t outs = static_cast<int64_t>(k) * n + (db != nullptr ? n : 0);
-  const unsigned join_blocks = static_cast<unsigned>((outs + 31) / 32);
-  if (out_dtype == CXG_F32)
-    launch_dependent(rows8_wgrad_join<float>, join_blocks, 32 * kJoinWarps, 0, st, a.partial, a.partial_db, static_cast<float *>(dw),
-                     static_cast<float *>(db), k, n, k_blocks, parts);
-  else
-    launch_dependent(rows8_wgrad_join<__nv_bfloat16>, join_blocks, 32 * kJoinWarps, 0, st, a.partial, a.partial_db,
-                     static_cast<__nv_bfloat16 *>(dw), static_cast<__nv_bfloat16 *>(db), k, n, k_blocks, parts);
+  launch_join(out_dtype, st, a.partial, a.partial_db, dw, db, k, n, k_blocks, parts, 128);
   count_launches(2);
   return check_launch("cxg_rows8_wgrad");
 }
