@@ -42,10 +42,10 @@ def _rows_close(got, want, mag):
     return bool(((got.double().cpu() - want).abs() <= half * want.abs() + 64 * 2.0 ** -24 * mag).all())
 
 
-def _check(n, width, dtype, gate, post, following, layer, scale="vector"):
+def _check(n, width, dtype, gate, post, following, layer, scale="vector", place=lambda v: v.cuda()):
     import cxgnncomp_backend as be
     t = _inputs(n, width, dtype, gate, post, following, layer, scale, seed=n + width)
-    dev = {k: None if v is None else v.cuda().requires_grad_(True) for k, v in t.items()}
+    dev = {k: None if v is None else place(v).requires_grad_(True) for k, v in t.items()}
     ref = {k: None if v is None else v.double().requires_grad_(True) for k, v in t.items()}
     outs = [o for o in _run(be, dev, post, following, layer) if o is not None]
     want = [o for o in residual(ref["x"], ref["f"], ref["gate"], ref["scale"], post, ref["w2"], ref["b2"], following, ref["w1"],
@@ -100,6 +100,22 @@ def test_parts(cuda, post, following, scale, dtype):
                                      (7, 1500), (5, 2048), (3, 4096), (3, 4001)])
 def test_widths(cuda, n, width, dtype):
     _check(n, width, dtype, "value", True, True, True)
+
+
+@pytest.mark.parametrize("width", [1, 5, 7, 9, 15, 17, 31, 33, 63, 65, 127, 129, 255])
+def test_odd_rows_of_bf16(cuda, width):
+    _check(61, width, torch.bfloat16, "value", True, True, width % 4 == 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,width", [(1, 1), (5, 2), (30, 16), (33, 47), (40, 64), (9, 128), (21, 256), (5, 257), (3, 512), (2, 4096)])
+def test_matrices_that_start_anywhere(cuda, n, width, dtype):
+    def place(v):
+        flat = torch.empty(v.numel() + 1, dtype=v.dtype, device="cuda")
+        flat[1:] = v.flatten().cuda()
+        return flat[1:].view(v.shape)
+
+    _check(n, width, dtype, "value", True, True, False, place=place)
 
 
 def test_many_rows(cuda):
