@@ -26,6 +26,7 @@ struct Rows8Args {
   int64_t n_src;  // rows; ids outside stand for the row of zeros behind the last
   int groups;
   int whole;  // 2: rows of y are whole 16-byte vectors, 1: 8-byte ones
+  bool staged;   // STAGED
   uint2 *marks;  // SPARSE: per edge that is the first of its row, that row and its end
 };
 
@@ -87,7 +88,11 @@ __device__ __forceinline__ void add_codes(unsigned long long *acc, const Codes<V
 
 // VALMODE: 0 sum, 1 a value per edge, 3 mean. WORDS: the (up to four) scales of an edge's row as one word, fetched with the ids by
 // one lane per edge; otherwise every lane fetches its own with the codes.
-template <typename T, int VB, int G, int NV, int U, int VALMODE, int MINB, bool WORDS, bool SPARSE>
+// SPARSE: rows without edges have been written, the next one with edges is in r.marks. STAGED: bf16 rows that are no whole vectors
+// go through shared memory, so that lanes write words side by side. (Value by value / staged, us: 278,000 rows with 1.6 M edges,
+// width 99 190 / 146, 149 273 / 187, 301 550 / 269; 663,000 rows with 9.9 M edges 99 399 / 478, 149 607 / 677, 301 1130 / 1076: for
+// graphs of few edges per row. Rows of up to 64, in vectors of 4 or 8 codes, have nothing to gain.)
+template <typename T, int VB, int G, int NV, int U, int VALMODE, int MINB, bool WORDS, bool SPARSE, bool STAGED>
 __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_constant__ Rows8Args r) {
   const WalkArgs &a = r.w;
   constexpr int NG = 32 / G;
@@ -108,8 +113,33 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
   }
   auto col = [&](int q) { return (lg + q * G) * VB; };
 
+  [[maybe_unused]] __shared__ __align__(16) T out_stage[STAGED ? kThreads * VB : 1];
+  [[maybe_unused]] T *const my_out = out_stage + (STAGED ? threadIdx.x / G * (G * VB) : 0);
+  const unsigned members = G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1) << (lane / G * G);
+  // the group's row of bf16, column c from value(c), in whole words
+  [[maybe_unused]] auto write_words = [&](T *y, auto value) {
+    const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(y) >> 1) & 1;
+    for (int c = 2 * lg - odd; c < a.width; c += 2 * G) {
+      const bool lower = c >= 0, upper = c + 1 < a.width;
+      const T first = value(lower ? c : 0), second = value(upper ? c + 1 : 0);
+      if (lower && upper)
+        *reinterpret_cast<uint32_t *>(y + c) = static_cast<uint32_t>(__bfloat16_as_ushort(first)) | static_cast<uint32_t>(__bfloat16_as_ushort(second)) << 16;
+      else if (lower)
+        y[c] = first;
+      else if (upper)
+        y[c + 1] = second;
+    }
+  };
   auto store = [&](int row, float (&f)[NV][VB]) {
     T *y = static_cast<T *>(a.y) + static_cast<int64_t>(row) * a.width;
+    if constexpr (STAGED) {
+      __syncwarp(members);  // the row before has been read
+#pragma unroll
+      for (int i = 0; i < VB; i += 2) *reinterpret_cast<__nv_bfloat162 *>(my_out + lg * VB + i) = __floats2bfloat162_rn(f[0][i], f[0][i + 1]);
+      __syncwarp(members);
+      write_words(y, [&](int c) { return my_out[c]; });
+      return;
+    }
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       auto vectors = [&](auto bytes) {  // VB values in vectors of so many bytes, or the whole of them where they are fewer
@@ -131,6 +161,10 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
     }
   };
   auto zero_row = [&](int row) {
+    if constexpr (STAGED) {
+      write_words(static_cast<T *>(a.y) + static_cast<int64_t>(row) * a.width, [](int) { return from_f32<T>(0.f); });
+      return;
+    }
     float z[NV][VB];
 #pragma unroll
     for (int q = 0; q < NV; ++q)
@@ -351,10 +385,12 @@ bool launch_pitch(const Rows8Args &r, cudaStream_t st, int *resident) {
     if (grid > most) grid = most;
     return launch_dependent(kernel, static_cast<unsigned>(grid < 1 ? 1 : grid), kThreads, 0, st, r) == cudaSuccess;
   };
-#define CXG_ROWS8_WALK(VB, G, NV, U, CTAS, WORDS)                                           \
-  if (r.w.row_bytes <= VB * G * NV)                                                         \
-  return r.marks != nullptr ? go(rows8_walk<T, VB, G, NV, U, VALMODE, CTAS, false, true>, G, CTAS) \
-                            : go(rows8_walk<T, VB, G, NV, U, VALMODE, CTAS, WORDS, false>, G, CTAS)
+  constexpr bool kHalf = sizeof(T) == 2;
+#define CXG_ROWS8_WALK(VB, G, NV, U, CTAS, WORDS)                                                                               \
+  if (r.w.row_bytes <= VB * G * NV)                                                                                             \
+  return r.marks != nullptr ? go(rows8_walk<T, VB, G, NV, U, VALMODE, CTAS, false, true, false>, G, CTAS)                       \
+         : r.staged         ? go(rows8_walk<T, VB, G, NV, U, VALMODE, CTAS, WORDS, false, kHalf && VB == 16 && NV == 1>, G, CTAS) \
+                            : go(rows8_walk<T, VB, G, NV, U, VALMODE, CTAS, WORDS, false, false>, G, CTAS)
   // Scales as words: 10.7 M edges, 32 columns bf16 214 -> 205 us, 100 fp32 with values 429 -> 405; 128 columns bf16 without values
   // 364 -> 374.
   CXG_ROWS8_WALK(4, 8, 1, 8, 8, true);
@@ -452,6 +488,7 @@ extern "C" int cxg_rows8_aggregate(const void *codes, const void *scales, int64_
   r.n_src = n_src, r.groups = rows8::groups_of(width);
   const uint64_t bits = static_cast<uint64_t>(width) * (y_dtype == CXG_F32 ? 4 : 2) | reinterpret_cast<uintptr_t>(y);
   r.whole = bits % 16 == 0 ? 2 : bits % 8 == 0 ? 1 : 0;
+  r.staged = r.whole == 0 && nnz < 10 * n_dst;
   const bool marked = is_sparse(n_dst, nnz);
   a.tile = marked ? sparse_tile(nnz, width, split_edges) : tile_edges(r, nnz, split_edges);
   a.part_stride = static_cast<int>(walk_part_stride(width));

@@ -35,6 +35,21 @@ def test_aggregate(cuda, width, reduce, dtype):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduce", ["mean", "value"])
+@pytest.mark.parametrize("width", [67, 99, 149, 255, 301, 511])
+def test_odd_rows_of_few_edges(cuda, width, reduce, dtype):
+    """A graph that is too large for one launch of clusters, with fewer than ten edges per row."""
+    import cxgnncomp_backend as be
+    ptr, idx = random_csr(30000, 2000, 4, seed=width, hub=5000)
+    x = randn((2000, width), width + 1)
+    ev = torch.rand(idx.shape[0], generator=torch.Generator().manual_seed(2)) - 0.3 if reduce == "value" else None
+    kind = "mean" if reduce == "mean" else "sum"
+    got = be.rows8_aggregate(be.quantize_rows(x.cuda()), ptr.cuda(), idx.cuda(), 0, reduce=kind, edge_value=None if ev is None else ev.cuda(),
+                             dtype=dtype)
+    assert _close(got, *aggregate(held_values(x), ptr, idx, kind, ev))
+
+
 @pytest.mark.parametrize("edges", [1, 7, 64, 1000])
 def test_tiles_that_cut_rows(cuda, edges):
     """Tiles of a few edges: chains of partials, empty rows at every border."""
