@@ -431,9 +431,12 @@ int tile_edges(const Rows8Args &r, int64_t nnz, int split_edges) {
 // Graphs with more rows than edges: most rows are empty, and a walk that looks at each of a tile's rows takes 0.2 us for each. (All
 // rows / those with edges, us: 1.9 M rows and 1000 edges, 100 columns bf16 33,100 / 99; 300,000 and 100,000 122 / 47; 300,000
 // and 300,000 77 / 63, 128 columns fp32 83 / 88; 500,000 edges 79 / 105.) With more edges than kMostMarked the tiles of one
-// wave have few rows each. In small tiles, as a row's end is what takes time (64 edges: 59 us where 16 take 32).
+// wave have few rows each. In small tiles, as a row's end is what takes time (64 edges: 59 us where 16 take 32); small graphs gain
+// from them up to four edges per row (40,000 rows and 72,000 edges, 128 columns bf16 50 / 32; 243 columns fp32 63 / 81).
 constexpr int64_t kMostMarked = 1 << 19;
-bool is_sparse(int64_t n_dst, int64_t nnz) { return nnz <= kMostMarked && n_dst > nnz; }
+bool is_sparse(int64_t n_dst, int64_t nnz, int width) {
+  return (nnz <= kMostMarked && n_dst > nnz) || (nnz <= (1 << 17) && n_dst > nnz / 4 && width <= 128);
+}
 int sparse_tile(int64_t nnz, int width, int split_edges) {
   return split_edges > 0 ? split_edges : width > 512 ? 64 : nnz <= (1 << 18) ? 16 : 32;
 }
@@ -489,7 +492,7 @@ extern "C" int cxg_rows8_aggregate(const void *codes, const void *scales, int64_
   const uint64_t bits = static_cast<uint64_t>(width) * (y_dtype == CXG_F32 ? 4 : 2) | reinterpret_cast<uintptr_t>(y);
   r.whole = bits % 16 == 0 ? 2 : bits % 8 == 0 ? 1 : 0;
   r.staged = r.whole == 0 && nnz < 10 * n_dst;
-  const bool marked = is_sparse(n_dst, nnz);
+  const bool marked = is_sparse(n_dst, nnz, width);
   a.tile = marked ? sparse_tile(nnz, width, split_edges) : tile_edges(r, nnz, split_edges);
   a.part_stride = static_cast<int>(walk_part_stride(width));
   WalkLayout L;
