@@ -49,7 +49,8 @@ __device__ const Ones residual_ones{};
 
 // Where a lane's values lie: Q vectors of N values (VB bytes: the widest that rows are whole in), the lanes' first vectors side by
 // side, then their second ones, and so on.
-template <typename T, int VB, int LANES>
+// FULL: rows that fill their lanes, so that nothing asks where they end.
+template <typename T, int VB, int LANES, bool FULL = false>
 struct Place {
   static constexpr int N = VB / static_cast<int>(sizeof(T));
   static constexpr int Q = kValues / N;
@@ -58,6 +59,8 @@ struct Place {
   using Element = T;
   static constexpr bool kStaged = VB >= 4;  // there are asynchronous copies of that many bytes
   __device__ __forceinline__ static int column(int p, int i) { return (i / N * LANES + p) * N + i % N; }
+  __device__ __forceinline__ static bool has(int column, int width) { return FULL || column < width; }
+  __device__ __forceinline__ static int width_of(int width) { return FULL ? LANES * kValues : width; }
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -76,7 +79,7 @@ struct Stage {
   __device__ __forceinline__ void request(int turn, int tensor, const void *matrix, int64_t offset, int p, int width) const {
 #pragma unroll
     for (int q = 0; q < P::Q; ++q) {
-      const bool on = P::column(p, q * P::N) < width;
+      const bool on = P::has(P::column(p, q * P::N), width);
       const uint8_t *src = on ? static_cast<const uint8_t *>(matrix) + offset + q * (P::kLanes * P::kBytes) : static_cast<const uint8_t *>(matrix);
       if constexpr (P::kBytes == 16)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot(turn, tensor, q)), "l"(src), "r"(on ? 16 : 0) : "memory");
@@ -116,7 +119,7 @@ __device__ __forceinline__ void read_row(Pair (&v)[kPairs], const void *matrix, 
   const T *src = static_cast<const T *>(matrix) + row * width;
   float f[kValues];
 #pragma unroll
-  for (int i = 0; i < kValues; ++i) f[i] = P::column(p, i) < width ? to_f32(__ldg(src + P::column(p, i))) : 0.f;
+  for (int i = 0; i < kValues; ++i) f[i] = P::has(P::column(p, i), width) ? to_f32(__ldg(src + P::column(p, i))) : 0.f;
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
 }
@@ -134,7 +137,7 @@ __device__ __forceinline__ void store_row(void *matrix, int64_t row, int p, int 
 #pragma unroll
   for (int q = 0; q < P::Q; ++q) {
     const int c = P::column(p, q * P::N);
-    if (c >= width) continue;
+    if (!P::has(c, width)) continue;
     const float *g = f + q * P::N;
     if constexpr (P::kBytes == 16) {
       Vec<T>::store_stream(dst + c, Vec<T>::from_float(g));
@@ -164,13 +167,13 @@ __device__ __forceinline__ void load_param(Pair (&v)[kPairs], const float *w, in
   for (int i = 0; i < kPairs; i += P::N >= 4 ? 2 : 1) {
     const int c = P::column(p, 2 * i);
     if constexpr (P::N >= 4) {
-      const ulonglong2 t = __ldg(reinterpret_cast<const ulonglong2 *>(w + (c < width ? c : 0)));
+      const ulonglong2 t = __ldg(reinterpret_cast<const ulonglong2 *>(w + (P::has(c, width) ? c : 0)));
       v[i] = t.x, v[i + 1] = t.y;
     } else if constexpr (P::N == 2) {
-      v[i] = __ldg(reinterpret_cast<const unsigned long long *>(w + (c < width ? c : 0)));
+      v[i] = __ldg(reinterpret_cast<const unsigned long long *>(w + (P::has(c, width) ? c : 0)));
     } else {
       const int e = P::column(p, 2 * i + 1);
-      v[i] = pair(__ldg(w + (c < width ? c : 0)), __ldg(w + (e < width ? e : 0)));
+      v[i] = pair(__ldg(w + (P::has(c, width) ? c : 0)), __ldg(w + (P::has(e, width) ? e : 0)));
     }
   }
 }
@@ -178,7 +181,7 @@ __device__ __forceinline__ void load_param(Pair (&v)[kPairs], const float *w, in
 // Zeros behind the row.
 template <typename P>
 __device__ __forceinline__ void clear_behind(Pair (&v)[kPairs], int p, int width) {
-  if (width == P::kLanes * kValues) return;
+  if (P::has(P::kLanes * kValues - 1, width)) return;
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
     if (P::N > 1) {
@@ -305,7 +308,7 @@ __device__ __forceinline__ void keep_row(const ResArgs &a, int64_t row, bool in,
 #pragma unroll
     for (int i = 0; i < P::N; ++i) {
       const float2 t = halves(h[(q * P::N + i) / 2]);
-      v[i] = in && c < a.d.width ? to_f32(from_f32<T>(i & 1 ? t.y : t.x)) : 0.f;
+      v[i] = in && P::has(c, a.d.width) ? to_f32(from_f32<T>(i & 1 ? t.y : t.x)) : 0.f;
       top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
     }
 #pragma unroll
@@ -334,16 +337,16 @@ constexpr int stage_bytes(int tensors, int threads) { return P::kStaged ? 2 * te
 constexpr int kForwardTensors = 3, kBackwardTensors = 5;
 
 // GATED: a gate per value.
-template <typename T, int LANES, int WARPS, int VB, bool GATED>
+template <typename T, int LANES, int WARPS, int VB, bool GATED, bool FULL>
 __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kForwardWarps, WARPS > 1 ? 32 * WARPS : kBlock))
     residual_forward(const __grid_constant__ ResArgs a) {
   constexpr int kLanes = LANES * WARPS;
-  using P = Place<T, VB, kLanes>;
+  using P = Place<T, VB, kLanes, FULL>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float2 place[2][WARPS];
   RowSum<LANES, WARPS> sum(place);
   const cxg_residual_desc &d = a.d;
-  const int p = threadIdx.x & (kLanes - 1), width = d.width;
+  const int p = threadIdx.x & (kLanes - 1), width = P::width_of(d.width);
   const bool with_f = d.f != nullptr, row_gate = d.gate_mode == CXG_GATE_ROW;
   dependency_wait();
   const Rows<LANES, WARPS> rows;
@@ -451,16 +454,16 @@ __device__ __forceinline__ void back_through_norm(Pair (&g)[kPairs], const Pair 
 }
 
 // BIASES: sums for them too.
-template <typename T, int LANES, int WARPS, int VB, bool GATED, bool BIASES>
+template <typename T, int LANES, int WARPS, int VB, bool GATED, bool BIASES, bool FULL>
 __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBackwardWarps, WARPS > 1 ? 32 * WARPS : kBlock))
     residual_backward(const __grid_constant__ ResArgs a) {
   constexpr int kLanes = LANES * WARPS;
-  using P = Place<T, VB, kLanes>;
+  using P = Place<T, VB, kLanes, FULL>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float2 place[2][WARPS];
   RowSum<LANES, WARPS> sum(place);
   const cxg_residual_desc &d = a.d;
-  const int p = threadIdx.x & (kLanes - 1), width = d.width;
+  const int p = threadIdx.x & (kLanes - 1), width = P::width_of(d.width);
   const bool with_f = d.f != nullptr, row_gate = d.gate_mode == CXG_GATE_ROW, next = d.next && d.dh != nullptr;
   dependency_wait();
   Pair acc[kSums][kPairs];
@@ -693,28 +696,38 @@ cudaError_t launch(Kernel kernel, int tensors, int threads, int blocks, const Re
 struct Forward {
   const ResArgs &a;
   cudaStream_t st;
-  template <typename T, int LANES, int WARPS, int VB, bool GATED>
-  cudaError_t run() const {
-    return launch<Place<T, VB, LANES * WARPS>>(residual_forward<T, LANES, WARPS, VB, GATED>, kForwardTensors,
+  template <typename T, int LANES, int WARPS, int VB, bool GATED, bool FULL>
+  cudaError_t go() const {
+    return launch<Place<T, VB, LANES * WARPS>>(residual_forward<T, LANES, WARPS, VB, GATED, FULL>, kForwardTensors,
                                                 WARPS > 1 ? 32 * WARPS : kBlock,
                                                 blocks_for(a.d.n + a.keep, LANES * WARPS, kForwardWarps), a, st);
+  }
+  template <typename T, int LANES, int WARPS, int VB, bool GATED>
+  cudaError_t run() const {
+    if constexpr (VB == 16) {
+      if (a.d.width == LANES * WARPS * kValues) return go<T, LANES, WARPS, VB, GATED, true>();
+    }
+    return go<T, LANES, WARPS, VB, GATED, false>();
   }
 };
 struct Backward {
   const ResArgs &a;
   cudaStream_t st;
   int blocks;
-  template <typename T, int LANES, int WARPS, int VB, bool GATED, bool BIASES>
+  template <typename T, int LANES, int WARPS, int VB, bool GATED, bool BIASES, bool FULL>
   cudaError_t go() const {
-    return launch<Place<T, VB, LANES * WARPS>>(residual_backward<T, LANES, WARPS, VB, GATED, BIASES>, kBackwardTensors,
+    return launch<Place<T, VB, LANES * WARPS>>(residual_backward<T, LANES, WARPS, VB, GATED, BIASES, FULL>, kBackwardTensors,
                                                 WARPS > 1 ? 32 * WARPS : kBlock, blocks, a, st);
   }
   template <typename T, int LANES, int WARPS, int VB, bool GATED>
   cudaError_t run() const {
     if constexpr (VB == 16) {
-      if (a.d.post_bias == nullptr && a.d.next_bias == nullptr) return go<T, LANES, WARPS, VB, GATED, false>();
+      const bool biases = a.d.post_bias != nullptr || a.d.next_bias != nullptr;
+      if (a.d.width == LANES * WARPS * kValues)
+        return biases ? go<T, LANES, WARPS, VB, GATED, true, true>() : go<T, LANES, WARPS, VB, GATED, false, true>();
+      if (!biases) return go<T, LANES, WARPS, VB, GATED, false, false>();
     }
-    return go<T, LANES, WARPS, VB, GATED, true>();
+    return go<T, LANES, WARPS, VB, GATED, true, false>();
   }
 };
 
