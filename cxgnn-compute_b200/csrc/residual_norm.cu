@@ -252,20 +252,24 @@ __device__ __forceinline__ float normalise(Pair (&v)[kPairs], const ResArgs &a, 
   return r;
 }
 
-// sigmoid and its derivative without cancellation: t = exp(-|g|), s = 1 / (1 + t) or t / (1 + t), s' = t / (1 + t)^2. The
-// reciprocal of 1 .. 2 is the hardware's, off by an ulp. For bf16 rows the exponential is the hardware's 2^x of the product
-// rounded once (1e-6 of it at |g| = 16, where 2^-9 is what the result is rounded to).
+// sigmoid and its derivative. For fp32 rows without cancellation: t = exp(-|g|), s = 1 / (1 + t) or t / (1 + t), s' = t / (1 + t)^2;
+// the reciprocal of 1 .. 2 is the hardware's, off by an ulp. For bf16 rows, which round to 2^-9, s = 1 / (1 + exp(-g)) and
+// s' = s (1 - s), with the hardware's 2^x of the product rounded once (1e-6 of it at |g| = 16): three instructions less.
 template <typename T>
 __device__ __forceinline__ void sigmoid(float g, float *s, float *ds) {
   float t, q;
-  if constexpr (sizeof(T) == 2)
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fabsf(g) * -1.44269504f));
-  else
+  if constexpr (sizeof(T) == 2) {
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(g * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + t));
+    *s = q;
+    *ds = fmaf(-q, q, q);
+  } else {
     t = expf(-fabsf(g));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + t));
-  const float tq = t * q;
-  *s = g >= 0.f ? q : tq;
-  *ds = tq * q;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + t));
+    const float tq = t * q;
+    *s = g >= 0.f ? q : tq;
+    *ds = tq * q;
+  }
 }
 // The gate's values become sigmoids, and their derivatives where there is room for them.
 template <typename T>
@@ -490,8 +494,9 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
   int turn = 0;
   if (rows.first < d.n) request(0, rows.first + rows.sub);
   for (int64_t row0 = rows.first; row0 < d.n; row0 += rows.step, turn ^= 1) {
-    const int64_t row = row0 + rows.sub, at = row < d.n ? row : d.n - 1;
-    const bool in = row < d.n;  // lanes without a row go through it with gradients of zero
+    const int64_t row = row0 + rows.sub;
+    const bool in = kLanes >= 32 || row < d.n;  // lanes without a row go through it with gradients of zero
+    const int64_t at = in ? row : d.n - 1;
     const float g_row = to_f32(rr);
     if constexpr (P::kStaged) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (row0 + rows.step < d.n) request(turn ^ 1, row + rows.step);
@@ -541,8 +546,7 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) g[i] = 0;
     if (next) {
-      const float r1 = normalise<P>(y, a, sum, p);  // y is u1 from here on
-      Pair dh[kPairs];
+      Pair dh[kPairs], t[kPairs];
       if (in)
         take(dh, 4, d.dh);
       else
@@ -550,14 +554,34 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
         for (int i = 0; i < kPairs; ++i) dh[i] = 0;
       load_param<P>(w, d.next_weight, p, width);
 #pragma unroll
+      for (int i = 0; i < kPairs; ++i) t[i] = mul2(dh[i], w[i]);
+      // the norm's factor and what goes back through it in one round of sums: <t u1> = r1 <t y>
+      float mean_t = 0.f;
+      if (d.layer) {
+        const float2 m = sum.both(sum2(add2(add2(y[0], y[1]), add2(y[2], y[3]))), sum2(add2(add2(t[0], t[1]), add2(t[2], t[3]))));
+        const Pair off = pair(-m.x * a.inv_width, -m.x * a.inv_width);
+        mean_t = m.y * a.inv_width;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) y[i] = add2(y[i], off);
+        clear_behind<P>(y, p, width);
+      }
+      const Pair yy = add2(fma2(y[0], y[0], mul2(y[1], y[1])), fma2(y[2], y[2], mul2(y[3], y[3])));
+      const Pair ty = add2(fma2(t[0], y[0], mul2(t[1], y[1])), fma2(t[2], y[2], mul2(t[3], y[3])));
+      const float2 q = sum.both(sum2(yy), sum2(ty));
+      const float r1 = __frsqrt_rn(fmaf(q.x, a.inv_width, d.eps)), dot = q.y * r1 * a.inv_width;
+      const Pair rr1 = pair(r1, r1), dots = pair(-dot, -dot), means = pair(-mean_t, -mean_t);
+#pragma unroll
       for (int i = 0; i < kPairs; ++i) {
+        y[i] = mul2(y[i], rr1);  // u1
         acc[3][i] = fma2(dh[i], y[i], acc[3][i]);
         if (BIASES) acc[4][i] = add2(acc[4][i], dh[i]);
-        dh[i] = mul2(dh[i], w[i]);
+        Pair v = fma2(y[i], dots, t[i]);
+        if (d.layer) v = add2(v, means);
+        t[i] = mul2(v, rr1);
       }
-      back_through_norm<P>(dh, y, r1, a, sum, p);
+      if (d.layer) clear_behind<P>(t, p, width);
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) g[i] = add2(g[i], dh[i]);
+      for (int i = 0; i < kPairs; ++i) g[i] = add2(g[i], t[i]);
     }
     if (in && d.dx != nullptr) store_row<P>(d.dx, row, p, width, g);
     if (with_f) {
