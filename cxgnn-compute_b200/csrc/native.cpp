@@ -65,7 +65,6 @@ struct Lib {
   CXG_FN(cxg_relation_pairs_fill);
   CXG_FN(cxg_rows8_pitch);
   CXG_FN(cxg_rows8_write);
-  CXG_FN(cxg_rows8_write_at_workspace_size);
   CXG_FN(cxg_rows8_write_at);
   CXG_FN(cxg_rows8_read);
   CXG_FN(cxg_rows8_aggregate_workspace_size);
@@ -118,7 +117,6 @@ void init(const std::string &path) {
   CXG_FN(cxg_relation_pairs_fill);
   CXG_FN(cxg_rows8_pitch);
   CXG_FN(cxg_rows8_write);
-  CXG_FN(cxg_rows8_write_at_workspace_size);
   CXG_FN(cxg_rows8_write_at);
   CXG_FN(cxg_rows8_read);
   CXG_FN(cxg_rows8_aggregate_workspace_size);
@@ -794,9 +792,9 @@ Held held_zeros(int64_t rows, int64_t width, at::Device device) {
   return h;
 }
 
-// Rows of x over rows [0, n) of what is held, or over the rows that index names (owner: the words of cxg_rows8_write_at).
+// Rows of x over rows [0, n) of what is held, or over the rows that index names (claims: the words of cxg_rows8_write_at).
 void quantize_into(const Tensor &x_in, const Tensor &codes, const Tensor &scales, int64_t width, const optional<Tensor> &index,
-                   const optional<Tensor> &owner) {
+                   const optional<Tensor> &claims) {
   if (for_torch(x_in)) fail(std::string("quantize_rows") + kTransform);
   const Tensor x = row_matrix(x_in, "x");
   const int64_t rows = codes.size(0) - 1, n = x.size(0);
@@ -813,11 +811,8 @@ void quantize_into(const Tensor &x_in, const Tensor &codes, const Tensor &scales
     of_type(*index, "index", {at::kLong});
     same_device(codes, *index, "index");
     if (index->dim() != 1 || index->size(0) != n) fail("quantize_rows: index must name a row for every row of x");
-    size_t need = 0;
-    check(lib.cxg_rows8_write_at_workspace_size(n, &need), "cxg_rows8_write_at_workspace_size");
-    const Workspace ws = workspace_on(x.device().index(), st, static_cast<int64_t>(need), "");
     check(lib.cxg_rows8_write_at(x.data_ptr(), code_of(x), row_step(x), n, static_cast<int>(width), index->data_ptr<int64_t>(),
-                                 codes.data_ptr(), scales.data_ptr(), rows, owner->data_ptr<int32_t>(), ws.data(), ws.bytes(), st),
+                                 codes.data_ptr(), scales.data_ptr(), rows, reinterpret_cast<uint64_t *>(claims->data_ptr<int64_t>()), st),
           "cxg_rows8_write_at");
   }
   // a backward pass that was to read these rows hears of it (inference tensors cannot be kept for one and count no versions)

@@ -136,27 +136,58 @@ struct Loaded {
   }
 };
 
-// Rows [0, n) of x to the rows `to` names (itself without it; negative: nowhere); rows from n on are written as zeros.
-// owner: the row's entry is given back (write_at).
+// The positions of a call that name rows: the last one of a row counts. Each enters itself in the row's word, behind the number of the
+// call, which the word behind the last row counts; who is still there when all have done so writes. Nothing is put back.
+struct Claims {
+  const int64_t *index;  // null: row i is row i
+  unsigned long long *words;
+  int64_t rows;
+};
+constexpr int kClaims = 4;  // per thread
+__global__ void __launch_bounds__(kThreads) rows8_claim(const Claims c, int64_t n) {
+  dependency_wait();
+  const int64_t first = blockIdx.x * static_cast<int64_t>(kThreads * kClaims) + threadIdx.x;
+  int64_t r[kClaims];
+#pragma unroll
+  for (int k = 0; k < kClaims; ++k) r[k] = first + k * kThreads < n ? __ldg(c.index + first + k * kThreads) : -1;
+  const unsigned long long call = static_cast<unsigned long long>(__ldcg(reinterpret_cast<const uint32_t *>(c.words + c.rows))) << 32;
+#pragma unroll
+  for (int k = 0; k < kClaims; ++k)
+    if (r[k] >= 0 && r[k] < c.rows) atomicMax(c.words + r[k], call | static_cast<uint32_t>(first + k * kThreads));
+}
+
+// Rows [0, n) of x to themselves, or to the rows that they claimed, in which they are row `before` and on; rows from n on are written as
+// zeros.
 template <typename T, Access A>
 __global__ void __launch_bounds__(kThreads) rows8_write(const T *x, int64_t ld, uint32_t n, uint32_t width, Items items, uint8_t *codes,
-                                                        uint8_t *scales, const int64_t *to, int32_t *owner) {
+                                                        uint8_t *scales, const Claims claims, uint32_t before) {
   constexpr int V = kWritten<T>, L = kSharing<T>;
   dependency_wait();
   const uint32_t groups = items.per / L, first = blockIdx.x * (kThreads * kItems) + threadIdx.x;
   const T *x_end = x + (n > 0 ? (n - 1) * ld + width : 0);
   Loaded<T, A> in[kItems];
   int64_t dst[kItems];
-  uint32_t chunk[kItems];
+  uint32_t chunk[kItems], at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const uint32_t i = first + k * kThreads;
-    uint32_t row;
-    items.place(i, &row, &chunk[k]);
-    const bool have = i < items.total, of_x = have && row < n;
-    dst[k] = have ? static_cast<int64_t>(row) : int64_t{-1};
-    if (to != nullptr && of_x) dst[k] = __ldg(to + row);
-    in[k].load(x + (of_x ? row : 0) * ld, chunk[k] * V, width, of_x, x, x_end);
+    items.place(i, &at[k], &chunk[k]);
+    const bool have = i < items.total, of_x = have && at[k] < n;
+    dst[k] = have ? static_cast<int64_t>(at[k]) : int64_t{-1};
+    if (claims.index != nullptr && of_x) dst[k] = __ldg(claims.index + at[k]);
+    in[k].load(x + (of_x ? at[k] : 0) * ld, chunk[k] * V, width, of_x, x, x_end);
+  }
+  if (claims.index != nullptr) {
+    uint32_t last[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      if (static_cast<uint64_t>(dst[k]) >= static_cast<uint64_t>(claims.rows)) dst[k] = -1;
+      last[k] = dst[k] >= 0 ? __ldcg(reinterpret_cast<const uint32_t *>(claims.words + dst[k])) : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k)
+      if (last[k] != before + at[k]) dst[k] = -1;
+    if (first == 0 && before == 0) atomicAdd(reinterpret_cast<uint32_t *>(claims.words + claims.rows), 1u);
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
@@ -178,27 +209,8 @@ __global__ void __launch_bounds__(kThreads) rows8_write(const T *x, int64_t ld, 
       else
         *reinterpret_cast<uint4 *>(out) = make_uint4(w[0], w[1], w[V / 4 - 2], w[V / 4 - 1]);
       if (chunk[k] % L == 0) scales[group] = static_cast<uint8_t>(e);
-      if (owner != nullptr && chunk[k] == 0) owner[dst[k]] = -1;
     }
   }
-}
-
-// Of the positions that name the same row the last one counts: each enters itself in the row's word, then looks whether it is
-// still there. The words are -1 between calls (rows8_write puts them back).
-__global__ void __launch_bounds__(kThreads) rows8_claim(const int64_t *index, int64_t n, int64_t rows, int32_t *owner) {
-  dependency_wait();
-  const int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x;
-  if (i >= n) return;
-  const int64_t r = index[i];
-  if (r >= 0 && r < rows) atomicMax(owner + r, static_cast<int32_t>(i));
-}
-__global__ void __launch_bounds__(kThreads) rows8_settle(const int64_t *index, int64_t n, int64_t rows, const int32_t *owner,
-                                                         int64_t *to) {
-  dependency_wait();
-  const int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x;
-  if (i >= n) return;
-  const int64_t r = index[i];
-  to[i] = r >= 0 && r < rows && owner[r] == static_cast<int32_t>(i) ? r : -1;
 }
 
 // out[i] = the values of row index[i] (of row i without an index; ids outside the rows read as zeros).
@@ -334,16 +346,18 @@ void in_pieces(int64_t n, uint32_t per, Go go) {
 }
 
 template <typename T>
-void launch_write(const void *x_, int64_t ld, int64_t n, int64_t n_end, int width, void *codes, void *scales, const int64_t *to,
-                  int32_t *owner, cudaStream_t st) {
+void launch_write(const void *x_, int64_t ld, int64_t n, int64_t n_end, int width, void *codes, void *scales, const Claims &claims,
+                  cudaStream_t st) {
   const int groups = groups_of(width);
   const T *x = static_cast<const T *>(x_);
   in_pieces(n_end, static_cast<uint32_t>(groups * kSharing<T>), [&](int64_t r, int64_t rows, const Items &items, unsigned blocks) {
-    const int64_t have = n - r < rows ? n - r : rows, at = to != nullptr ? 0 : r;
+    const int64_t have = n - r < rows ? n - r : rows, at = claims.index != nullptr ? 0 : r;
+    Claims mine = claims;
+    if (mine.index != nullptr) mine.index += r;
     auto go = [&](auto kernel) {
       launch_dependent(kernel, blocks, kThreads, 0, st, x + (have > 0 ? r * ld : 0), ld, static_cast<uint32_t>(have > 0 ? have : 0),
                        static_cast<uint32_t>(width), items, static_cast<uint8_t *>(codes) + at * groups * kGroup,
-                       static_cast<uint8_t *>(scales) + at * groups, to != nullptr ? to + r : nullptr, owner);
+                       static_cast<uint8_t *>(scales) + at * groups, mine, static_cast<uint32_t>(r));
     };
     const Access a = access_of<T>(x + (have > 0 ? r * ld : 0), ld, width);
     a == kWide ? go(rows8_write<T, kWide>) : a == kVector ? go(rows8_write<T, kVector>) : go(rows8_write<T, kShifted>);
@@ -401,39 +415,29 @@ extern "C" int cxg_rows8_write(const void *x, int dtype, int64_t ld, int64_t n, 
   CXG_REQUIRE(codes && scales && (x || n == 0), CXG_ENULL, "cxg_rows8_write: NULL argument");
   CXG_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 16 == 0, CXG_EINVAL, "cxg_rows8_write: codes must be 16-byte aligned");
   if (dtype == CXG_F32)
-    launch_write<float>(x, ld, n, n_end, width, codes, scales, nullptr, nullptr, as_stream(stream));
+    launch_write<float>(x, ld, n, n_end, width, codes, scales, Claims{}, as_stream(stream));
   else
-    launch_write<__nv_bfloat16>(x, ld, n, n_end, width, codes, scales, nullptr, nullptr, as_stream(stream));
+    launch_write<__nv_bfloat16>(x, ld, n, n_end, width, codes, scales, Claims{}, as_stream(stream));
   return check_launch("cxg_rows8_write");
 }
 
-extern "C" int cxg_rows8_write_at_workspace_size(int64_t n, size_t *bytes) {
-  CXG_REQUIRE(bytes != nullptr, CXG_ENULL, "cxg_rows8_write_at_workspace_size: bytes is NULL");
-  CXG_REQUIRE(n >= 0, CXG_EINVAL, "cxg_rows8_write_at_workspace_size: bad size");
-  *bytes = static_cast<size_t>(n) * sizeof(int64_t);
-  return CXG_OK;
-}
-
 extern "C" int cxg_rows8_write_at(const void *x, int dtype, int64_t ld, int64_t n, int width, const int64_t *index, void *codes,
-                                  void *scales, int64_t rows, int32_t *owner, void *workspace, size_t workspace_bytes,
-                                  void *stream) {
+                                  void *scales, int64_t rows, uint64_t *claims, void *stream) {
   CXG_REQUIRE(!bad_matrix(dtype, ld, n, width) && rows >= 0, CXG_EINVAL, "cxg_rows8_write_at: bad sizes or type");
   if (n == 0) return CXG_OK;
-  CXG_REQUIRE(x && index && codes && scales && owner, CXG_ENULL, "cxg_rows8_write_at: NULL argument");
+  CXG_REQUIRE(x && index && codes && scales && claims, CXG_ENULL, "cxg_rows8_write_at: NULL argument");
   CXG_REQUIRE(n <= INT32_MAX, CXG_ELIMIT, "cxg_rows8_write_at: %lld rows, at most 2^31 - 1", static_cast<long long>(n));
-  CXG_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 16 == 0, CXG_EINVAL, "cxg_rows8_write_at: codes must be 16-byte aligned");
-  CXG_REQUIRE(workspace != nullptr && workspace_bytes >= n * sizeof(int64_t) && reinterpret_cast<uintptr_t>(workspace) % 8 == 0,
-              CXG_EWORKSPACE, "cxg_rows8_write_at: workspace %zu bytes, need %zu", workspace_bytes, n * sizeof(int64_t));
+  CXG_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 16 == 0 && reinterpret_cast<uintptr_t>(claims) % 8 == 0, CXG_EINVAL,
+              "cxg_rows8_write_at: codes must be 16-byte aligned, claims 8-byte");
   cudaStream_t st = as_stream(stream);
-  int64_t *to = static_cast<int64_t *>(workspace);
-  const unsigned grid = static_cast<unsigned>((n + kThreads - 1) / kThreads);
-  launch_dependent(rows8_claim, grid, kThreads, 0, st, index, n, rows, owner);
-  launch_dependent(rows8_settle, grid, kThreads, 0, st, index, n, rows, owner, to);
+  const Claims c{index, reinterpret_cast<unsigned long long *>(claims), rows};
+  const cudaError_t e = launch_dependent(rows8_claim, static_cast<unsigned>((n + kThreads * kClaims - 1) / (kThreads * kClaims)), kThreads, 0, st, c, n);
+  if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_write_at: %s", cudaGetErrorString(e));
   if (dtype == CXG_F32)
-    launch_write<float>(x, ld, n, n, width, codes, scales, to, owner, st);
+    launch_write<float>(x, ld, n, n, width, codes, scales, c, st);
   else
-    launch_write<__nv_bfloat16>(x, ld, n, n, width, codes, scales, to, owner, st);
-  count_launches(2);
+    launch_write<__nv_bfloat16>(x, ld, n, n, width, codes, scales, c, st);
+  count_launches(1);
   return check_launch("cxg_rows8_write_at");
 }
 

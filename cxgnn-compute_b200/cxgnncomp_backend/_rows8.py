@@ -13,7 +13,7 @@ from . import _native
 class Rows8:
     """`rows` rows of `width` values in 8 bits on a CUDA device, zeros at first: pitch + pitch / 32 bytes a row, pitch being
     `width` in whole groups of 32. quantize_rows writes them, dequantize_rows, rows8_aggregate and rows8_weight_grad read them."""
-    __slots__ = ("rows", "width", "codes", "scales", "_owner")
+    __slots__ = ("rows", "width", "codes", "scales", "_claims")
 
     def __init__(self, rows, width, device="cuda"):
         device = torch.device(device)
@@ -21,13 +21,13 @@ class Rows8:
             device = torch.device("cuda", torch.cuda.current_device())
         self.rows, self.width = int(rows), int(width)
         self.codes, self.scales = _native.rows8_zeros(self.rows, self.width, device)
-        self._owner = None
+        self._claims = None
 
     @classmethod
     def _of(cls, codes, scales, width):
         """codes [rows + 1, pitch] and scales [rows + 1, pitch / 32], the last row of zeros."""
         r = cls.__new__(cls)
-        r.rows, r.width, r.codes, r.scales, r._owner = codes.shape[0] - 1, width, codes, scales, None
+        r.rows, r.width, r.codes, r.scales, r._claims = codes.shape[0] - 1, width, codes, scales, None
         return r
 
     @property
@@ -48,16 +48,16 @@ class Rows8:
     def __repr__(self):
         return f"Rows8({self.rows}, {self.width}, device='{self.device}')"
 
-    def _owners(self):
-        """A word per row, all -1 between calls, by which writes at an index find the last of equal ids."""
-        if self._owner is not None:
-            return self._owner
-        owner = torch.full((max(1, self.rows),), -1, dtype=torch.int32, device=self.device)
+    def _claimed(self):
+        """A word per row and one for the number of calls, by which writes at an index find the last of equal ids."""
+        if self._claims is not None:
+            return self._claims
+        claims = torch.zeros((self.rows + 1,), dtype=torch.int64, device=self.device)
         # not what a capture fills when its graph runs; and other streams must not come before the fill
         if not _native.capturing(self.device.index):
             torch.cuda.current_stream(self.device).synchronize()
-            self._owner = owner
-        return owner
+            self._claims = claims
+        return claims
 
 
 def _rows8(rows, who):
@@ -76,7 +76,7 @@ def quantize_rows(x, out=None, index=None):
         codes, scales = _native.rows8_quantize(x)
         return Rows8._of(codes, scales, x.shape[1])
     _rows8(out, "quantize_rows")
-    _native.rows8_quantize_into(x, out.codes, out.scales, out.width, index, None if index is None else out._owners())
+    _native.rows8_quantize_into(x, out.codes, out.scales, out.width, index, None if index is None else out._claimed())
     return out
 
 

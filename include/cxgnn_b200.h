@@ -682,11 +682,10 @@ int cxg_rows8_pitch(int width);
 int cxg_rows8_write(const void *x, int dtype, int64_t ld, int64_t n, int width, void *codes, void *scales, int zero_row,
                     void *stream);
 /* Row i of x to row index[i]; ids outside [0, rows) are left out, and of positions with the same id the last one counts.
-   owner: int32 [rows], all -1, as it is again when the call has run. Calls that write the same rows have to be ordered by the
-   caller. n < 2^31. */
-int cxg_rows8_write_at_workspace_size(int64_t n, size_t *bytes);
+   claims: uint64 [rows + 1], zeros at first, kept from call to call (a word per row, and the number of calls). Calls that write the
+   same rows have to be ordered by the caller. n < 2^31. */
 int cxg_rows8_write_at(const void *x, int dtype, int64_t ld, int64_t n, int width, const int64_t *index, void *codes, void *scales,
-                       int64_t rows, int32_t *owner, void *workspace, size_t workspace_bytes, void *stream);
+                       int64_t rows, uint64_t *claims, void *stream);
 /* out[i] ([n, width], rows ld values apart) = row index[i], or row i where index is NULL (n <= rows). */
 int cxg_rows8_read(const void *codes, const void *scales, int64_t rows, int width, const int64_t *index, int64_t n, void *out,
                    int dtype, int64_t ld, void *stream);

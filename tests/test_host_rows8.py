@@ -26,12 +26,12 @@ def test_write_and_read():
     assert write(P, 0, 0, 10, 0, P, P, 1, None) == EINVAL
     assert write(P, 0, 40, 10, 40, P + 8, P, 1, None) == EINVAL  # codes off their alignment
     assert write(None, 0, 40, 0, 40, None, None, 0, None) == 0   # nothing to do
-    at = _fn("cxg_rows8_write_at", [vp, ci, i64, i64, ci, vp, vp, vp, i64, vp, vp, sz, vp])
-    assert at(P, 0, 40, 10, 40, None, P, P, 5, P, P, 1 << 20, None) == ENULL
-    assert at(P, 0, 40, 10, 40, P, P, P, 5, None, P, 1 << 20, None) == ENULL
-    assert at(P, 0, 40, 10, 40, P, P, P, 5, P, P, 79, None) == EWORKSPACE
-    assert at(P, 0, 40, 2 ** 31, 40, P, P, P, 5, P, P, 1 << 40, None) == ELIMIT
-    assert at(P, 0, 40, 0, 40, None, None, None, 5, None, None, 0, None) == 0
+    at = _fn("cxg_rows8_write_at", [vp, ci, i64, i64, ci, vp, vp, vp, i64, vp, vp])
+    assert at(P, 0, 40, 10, 40, None, P, P, 5, P, None) == ENULL
+    assert at(P, 0, 40, 10, 40, P, P, P, 5, None, None) == ENULL
+    assert at(P, 0, 40, 10, 40, P, P, P, 5, P + 4, None) == EINVAL
+    assert at(P, 0, 40, 2 ** 31, 40, P, P, P, 5, P, None) == ELIMIT
+    assert at(P, 0, 40, 0, 40, None, None, None, 5, None, None) == 0
     read = _fn("cxg_rows8_read", [vp, vp, i64, ci, vp, i64, vp, ci, i64, vp])
     assert read(P, P, 5, 40, None, 6, P, 0, 40, None) == EINVAL  # more rows than there are
     assert read(P, P, 5, 40, None, 5, None, 0, 40, None) == ENULL
