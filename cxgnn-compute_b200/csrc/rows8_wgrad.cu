@@ -7,9 +7,14 @@
 //
 // The contraction runs over rows, so both operands are "MN-major": a stage holds 64 rows of the input (A: 128 columns, two
 // spans of 128 bytes per row in a 128-byte swizzle) and of dy (B: hi, then mid, then lo spans). Both are made in registers:
-// producer warps load 16 bytes at a time two stages ahead, convert, and write the operands where the tensor core reads them. One instruction multiplies A by [hi | mid], another adds A by lo to mid's accumulator. An accumulator takes
-// `chunk` stages, as the tensor core's additions cut off what an fp32 addition rounds (its error grows with the number of
-// additions); the epilogue warps, each lane a column of the input, add the chunks up in shared memory.
+// producer warps load 16 or 32 bytes at a time two stages ahead, convert, and write the operands where the tensor core reads
+// them. One instruction multiplies A by [hi | mid], another adds A by lo to mid's accumulator. An accumulator takes `chunk`
+// stages, as the tensor core's additions cut off what an fp32 addition rounds (its error grows with the number of additions);
+// the epilogue warps, each lane a column of the input, add the chunks up in shared memory.
+//
+// Measured: 2.4 M rows of 100 x 128 fp32 384 us (4.1 TB/s), 400,000 77. What bounds it is shared memory: per stage 64 KB of
+// operands written and 80 read by the tensor core, besides the loads. Of the 400,000 rows' time with older loads (84), without MMA 75
+// remain, without loads 58, without conversion 75, with neither of the last two 50.
 //
 // A block owns a contiguous range of rows of one pair of 128-column blocks; its sums go to a partial of its own and a second
 // kernel adds the partials in order: the same bits on every run. Every wait is bounded (see tensor_core.cuh).
@@ -104,7 +109,8 @@ __device__ __forceinline__ void three_parts(const Pair (&v)[4], uint32_t (&hi)[4
   }
 }
 
-// SPANS: 64-column spans of a block of dy. VECTOR: bytes of the vectors that rows of dy are read in, all of them whole. 32-byte vectors of fp32 take half the passes through L1 that pairs of 16-byte ones do.
+// SPANS: 64-column spans of a block of dy. VECTOR: bytes of the vectors that rows of dy are read in, all of them whole. 32-byte
+// vectors of fp32 take half the passes through L1 that pairs of 16-byte ones do.
 template <typename T, int VECTOR, int SPANS>
 __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant__ R8Args a) {
   constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
@@ -407,8 +413,9 @@ __global__ void __launch_bounds__(kThreads, 1) rows8_wgrad(const __grid_constant
   }
 }
 
-// dw[o][i] and db[o] from [pair of column blocks][parts][per columns of dy][128 columns of the input]: warp q of a block adds the partials q, q + 8, ... of 32 outputs, the eight sums are added in order. (A thread
-// per output and all its partials took 11 us for 148 partials of 128 x 100, a chain of loads.)
+// dw[o][i] and db[o] from [pair of column blocks][parts][per columns of dy][128 columns of the input]: warp q of a block adds the
+// partials q, q + 8, ... of 32 outputs, the eight sums are added in order. (A thread per output and all its
+// partials took 11 us for 148 partials of 128 x 100, a chain of loads.)
 constexpr int kJoinWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps) rows8_wgrad_join(const float *partial, const float *partial_db, T *dw, T *db, int k,

@@ -81,7 +81,8 @@ def test_rows_without_edges_and_first_rows(cuda):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("reduce", ["sum", "mean", "value"])
-@pytest.mark.parametrize("n,edges,width", [(1000, 1, 33), (3000, 200, 4), (3000, 700, 100), (30000, 5000, 47), (30000, 29000, 128), (31000, 120000, 64),
+@pytest.mark.parametrize("n,edges,width", [(1000, 1, 33), (3000, 200, 4), (3000, 700, 100), (30000, 5000, 47), (30000, 29000, 128),
+                                           (31000, 120000, 64),
                                            (9000, 2000, 300), (2000, 400, 900), (100000, 70000, 16)])
 def test_graphs_of_mostly_empty_rows(cuda, n, edges, width, reduce, dtype):
     """More rows than edges: whole tiles of one row, rows that tiles cut, empty rows in front, between and behind."""
