@@ -93,6 +93,7 @@ def test_graphs_of_mostly_empty_rows(cuda, n, edges, width, reduce, dtype):
     ptr = torch.zeros(n + 1, dtype=torch.int64)
     ptr[1:] = torch.bincount(dst, minlength=n).cumsum(0)
     idx = torch.randint(0, 500, (edges,), generator=gen)
+    idx[::7], idx[3::11] = -1, 507
     if width % 2:
         ptr, idx = ptr.int(), idx.int()
     x = randn((500, width), width)
