@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kFo
   __shared__ float2 place[2][WARPS];
   RowSum<LANES, WARPS> sum(place);
   const cxg_residual_desc &d = a.d;
-  const int p = threadIdx.x & (kLanes - 1), width = P::width_of(d.width);
+  const int p = WARPS > 1 ? threadIdx.x : threadIdx.x & (LANES - 1), width = P::width_of(d.width);
   const bool with_f = d.f != nullptr, row_gate = d.gate_mode == CXG_GATE_ROW;
   dependency_wait();
   const Rows<LANES, WARPS> rows;
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
   __shared__ float2 place[2][WARPS];
   RowSum<LANES, WARPS> sum(place);
   const cxg_residual_desc &d = a.d;
-  const int p = threadIdx.x & (kLanes - 1), width = P::width_of(d.width);
+  const int p = WARPS > 1 ? threadIdx.x : threadIdx.x & (LANES - 1), width = P::width_of(d.width);
   const bool with_f = d.f != nullptr, row_gate = d.gate_mode == CXG_GATE_ROW, next = d.next && d.dh != nullptr;
   dependency_wait();
   Pair acc[kSums][kPairs];
@@ -670,12 +670,13 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
   }
 }
 
-// Lanes of a row: the smallest power of two, from 2 on, that holds it. (At 8 and more alone, 937500 rows of 32 bf16 values took
-// 399 us instead of 189, forward and backward, and 20 of them 409 instead of 216.)
+// Lanes of a row: the smallest power of two, from 2 on, that holds it, or three warps, six or twelve. (Eight and more alone: 937500
+// rows of 32 bf16 values, forward and backward, 399 us instead of 189, 20 of them 409 instead of 216. Powers of two alone: 78,125 of
+// 768 bf16 597 us instead of 470, 46,875 of 1280 793 instead of 623.)
 int lanes_of(int width) {
   int lanes = 2;
   while (lanes * kValues < width) lanes *= 2;
-  return lanes;
+  return lanes >= 128 && lanes / 4 * 3 * kValues >= width ? lanes / 4 * 3 : lanes;
 }
 int rows_per_block(int lanes) { return lanes > 32 ? 1 : kBlock / lanes; }
 int blocks_for(int64_t n, int lanes, int warps) {
@@ -693,8 +694,11 @@ cudaError_t by_width(int width, Go go) {
     case 16: return go.template run<T, 16, 1, VB, GATED>();
     case 32: return go.template run<T, 32, 1, VB, GATED>();
     case 64: return go.template run<T, 32, 2, VB, GATED>();
+    case 96: return go.template run<T, 32, 3, VB, GATED>();
     case 128: return go.template run<T, 32, 4, VB, GATED>();
+    case 192: return go.template run<T, 32, 6, VB, GATED>();
     case 256: return go.template run<T, 32, 8, VB, GATED>();
+    case 384: return go.template run<T, 32, 12, VB, GATED>();
     default: return go.template run<T, 32, 16, VB, GATED>();
   }
 }

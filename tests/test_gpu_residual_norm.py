@@ -97,7 +97,7 @@ def test_parts(cuda, post, following, scale, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,width", [(700, 16), (300, 8), (500, 20), (33, 32), (40, 200), (300, 256), (30, 257), (20, 512), (9, 1000),
-                                     (7, 1500), (5, 2048), (3, 4096), (3, 4001)])
+                                     (7, 1500), (9, 768), (9, 520), (7, 769), (5, 1536), (4, 2500), (5, 2048), (3, 4096), (3, 4001)])
 def test_widths(cuda, n, width, dtype):
     _check(n, width, dtype, "value", True, True, True)
 
@@ -141,7 +141,7 @@ def test_many_rows(cuda):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("n,width", [(1, 32), (1, 16), (37, 24), (100, 8), (40, 47), (300, 128), (17, 1000), (5, 264), (0, 64)])
+@pytest.mark.parametrize("n,width", [(1, 32), (1, 16), (37, 24), (100, 8), (40, 47), (300, 128), (17, 1000), (9, 768), (5, 1400), (5, 264), (0, 64)])
 def test_kept_rows_are_those_of_h(cuda, n, width, dtype):
     import cxgnncomp_backend as be
     t = _inputs(n, width, dtype, "value", True, True, False)
