@@ -334,7 +334,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
     }
   };
   cluster.sync();
-  const bool long_chains = e1 - e0 > kWalkSeqPartials * kTile;
+  const bool long_chains = tiles > kWalkSeqPartials;  // (as many edges as 64 tiles hold may lie in 65)
 #pragma unroll 1
   for (int phase = long_chains ? 0 : 1; phase < 2; ++phase) {
 #pragma unroll 1
