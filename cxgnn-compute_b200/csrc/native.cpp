@@ -812,7 +812,7 @@ void quantize_into(const Tensor &x_in, const Tensor &codes, const Tensor &scales
     same_device(codes, *index, "index");
     if (index->dim() != 1 || index->size(0) != n) fail("quantize_rows: index must name a row for every row of x");
     check(lib.cxg_rows8_write_at(x.data_ptr(), code_of(x), row_step(x), n, static_cast<int>(width), index->data_ptr<int64_t>(),
-                                 codes.data_ptr(), scales.data_ptr(), rows, reinterpret_cast<uint64_t *>(claims->data_ptr<int64_t>()), st),
+                                 codes.data_ptr(), scales.data_ptr(), rows, claims->data_ptr<int32_t>(), st),
           "cxg_rows8_write_at");
   }
   // a backward pass that was to read these rows hears of it (inference tensors cannot be kept for one and count no versions)

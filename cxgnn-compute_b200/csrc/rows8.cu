@@ -7,7 +7,7 @@
 // over these. Lanes go along rows without regard to where these end, so that none is idle for a width that is no power of two;
 // items are counted in 32 bits, larger matrices go in pieces. (4 fp32 values a lane, 64-bit counts and a limit on every code were
 // 140 instructions an item and twice the time of memory.) Measured: 169,343 rows of 256 fp32 written 35 us (6.2 TB/s); 1.2 M rows
-// of 128 bf16 to random rows of 2.4 M and 2 M random rows back 265 us (4.7 TB/s: rows are single
+// of 128 bf16 to random rows of 2.4 M and 2 M random rows back 268 us (4.7 TB/s: rows are single
 // lines, their four bytes of scales sectors of their own).
 #include "rows8.cuh"
 
@@ -138,13 +138,16 @@ struct Loaded {
   }
 };
 
-// The positions of a call that name rows: the last one of a row counts. Each enters itself in the row's word, behind the number of the
-// call, which the word behind the last row counts; who is still there when all have done so writes. Nothing is put back.
+// The positions of a call that name rows: the last one of a row counts. Each enters itself in the row's word (position + 1, the
+// largest stays); who is still there when all have done so writes the row, and sets the word's top bit, which makes it negative:
+// less than what any later call enters. Positions are compared without that bit, so it does not matter who of a row's lanes sees it
+// already. A call touches the words of its own rows alone: calls that write other rows may run beside it, in any number.
 struct Claims {
   const int64_t *index;  // null: row i is row i
-  unsigned long long *words;
+  int32_t *words;
   int64_t rows;
 };
+constexpr uint32_t kDone = 0x80000000u;
 constexpr int kClaims = 4;  // per thread (1.2 M of them 11.5 us; one per thread 21)
 __global__ void __launch_bounds__(kThreads) rows8_claim(const Claims c, int64_t n) {
   dependency_wait();
@@ -152,10 +155,9 @@ __global__ void __launch_bounds__(kThreads) rows8_claim(const Claims c, int64_t 
   int64_t r[kClaims];
 #pragma unroll
   for (int k = 0; k < kClaims; ++k) r[k] = first + k * kThreads < n ? __ldg(c.index + first + k * kThreads) : -1;
-  const unsigned long long call = static_cast<unsigned long long>(__ldcg(reinterpret_cast<const uint32_t *>(c.words + c.rows))) << 32;
 #pragma unroll
   for (int k = 0; k < kClaims; ++k)
-    if (r[k] >= 0 && r[k] < c.rows) atomicMax(c.words + r[k], call | static_cast<uint32_t>(first + k * kThreads));
+    if (r[k] >= 0 && r[k] < c.rows) atomicMax(c.words + r[k], static_cast<int32_t>(first + k * kThreads + 1));
 }
 
 // Rows [0, n) of x to themselves, or to the rows that they claimed, in which they are row `before` and on; rows from n on are written as
@@ -184,12 +186,11 @@ __global__ void __launch_bounds__(kThreads) rows8_write(const T *x, int64_t ld, 
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       if (static_cast<uint64_t>(dst[k]) >= static_cast<uint64_t>(claims.rows)) dst[k] = -1;
-      last[k] = dst[k] >= 0 ? __ldcg(reinterpret_cast<const uint32_t *>(claims.words + dst[k])) : 0u;
+      last[k] = dst[k] >= 0 ? static_cast<uint32_t>(__ldcg(claims.words + dst[k])) : 0u;
     }
 #pragma unroll
     for (int k = 0; k < kItems; ++k)
-      if (last[k] != before + at[k]) dst[k] = -1;
-    if (first == 0 && before == 0) atomicAdd(reinterpret_cast<uint32_t *>(claims.words + claims.rows), 1u);
+      if ((last[k] & ~kDone) != before + at[k] + 1) dst[k] = -1;
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(kThreads) rows8_write(const T *x, int64_t ld, 
       else
         *reinterpret_cast<uint4 *>(out) = make_uint4(w[0], w[1], w[V / 4 - 2], w[V / 4 - 1]);
       if (chunk[k] % L == 0) scales[group] = static_cast<uint8_t>(e);
+      if (claims.index != nullptr && chunk[k] == 0) __stcg(claims.words + dst[k], static_cast<int32_t>(kDone | (before + at[k] + 1)));
     }
   }
 }
@@ -424,7 +426,7 @@ extern "C" int cxg_rows8_write(const void *x, int dtype, int64_t ld, int64_t n, 
 }
 
 extern "C" int cxg_rows8_write_at(const void *x, int dtype, int64_t ld, int64_t n, int width, const int64_t *index, void *codes,
-                                  void *scales, int64_t rows, uint64_t *claims, void *stream) {
+                                  void *scales, int64_t rows, void *claims, void *stream) {
   CXG_REQUIRE(!bad_matrix(dtype, ld, n, width) && rows >= 0, CXG_EINVAL, "cxg_rows8_write_at: bad sizes or type");
   if (n == 0) return CXG_OK;
   CXG_REQUIRE(x && index && codes && scales && claims, CXG_ENULL, "cxg_rows8_write_at: NULL argument");
@@ -432,7 +434,7 @@ extern "C" int cxg_rows8_write_at(const void *x, int dtype, int64_t ld, int64_t 
   CXG_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 16 == 0 && reinterpret_cast<uintptr_t>(claims) % 8 == 0, CXG_EINVAL,
               "cxg_rows8_write_at: codes must be 16-byte aligned, claims 8-byte");
   cudaStream_t st = as_stream(stream);
-  const Claims c{index, reinterpret_cast<unsigned long long *>(claims), rows};
+  const Claims c{index, static_cast<int32_t *>(claims), rows};
   const unsigned grid = static_cast<unsigned>((n + kThreads * kClaims - 1) / (kThreads * kClaims));
   const cudaError_t e = launch_dependent(rows8_claim, grid, kThreads, 0, st, c, n);
   if (e != cudaSuccess) return set_error(CXG_ECUDA, "cxg_rows8_write_at: %s", cudaGetErrorString(e));

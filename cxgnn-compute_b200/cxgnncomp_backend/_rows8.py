@@ -49,10 +49,10 @@ class Rows8:
         return f"Rows8({self.rows}, {self.width}, device='{self.device}')"
 
     def _claimed(self):
-        """A word per row and one for the number of calls, by which writes at an index find the last of equal ids."""
+        """A word per row, by which writes at an index find the last of equal ids."""
         if self._claims is not None:
             return self._claims
-        claims = torch.zeros((self.rows + 1,), dtype=torch.int64, device=self.device)
+        claims = torch.zeros((max(self.rows, 1),), dtype=torch.int32, device=self.device)
         # not what a capture fills when its graph runs; and other streams must not come before the fill
         if not _native.capturing(self.device.index):
             torch.cuda.current_stream(self.device).synchronize()

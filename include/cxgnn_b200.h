@@ -682,10 +682,10 @@ int cxg_rows8_pitch(int width);
 int cxg_rows8_write(const void *x, int dtype, int64_t ld, int64_t n, int width, void *codes, void *scales, int zero_row,
                     void *stream);
 /* Row i of x to row index[i]; ids outside [0, rows) are left out, and of positions with the same id the last one counts.
-   claims: uint64 [rows + 1], zeros at first, kept from call to call (a word per row, and the number of calls). Calls that write the
-   same rows have to be ordered by the caller. n < 2^31. */
+   claims: int32 [rows], 8-byte aligned, zeros at first, kept from call to call (a word per row). Calls that write the same rows have
+   to be ordered by the caller; calls that write different rows share the words at any time. n < 2^31. */
 int cxg_rows8_write_at(const void *x, int dtype, int64_t ld, int64_t n, int width, const int64_t *index, void *codes, void *scales,
-                       int64_t rows, uint64_t *claims, void *stream);
+                       int64_t rows, void *claims, void *stream);
 /* out[i] ([n, width], rows ld values apart) = row index[i], or row i where index is NULL (n <= rows). */
 int cxg_rows8_read(const void *codes, const void *scales, int64_t rows, int width, const int64_t *index, int64_t n, void *out,
                    int dtype, int64_t ld, void *stream);
