@@ -104,6 +104,23 @@ __device__ __forceinline__ void code_values(float *f, uint32_t word) {
   f[0] = code_value<0>(word), f[1] = code_value<1>(word), f[2] = code_value<2>(word), f[3] = code_value<3>(word);
 }
 
+// The scale times an edge's value may leave the range of fp32 where both are finite (scales reach 2^121): every term of the group that
+// is not zero overflows then, and zeros, which an infinite factor would make NaN, have to stay zeros. The codes become -127, 0 or
+// 127, and the scale (returned as its byte) is one with which the factor lies between 2^126 and 2^127. Values below kSafeValue
+// cannot get there.
+constexpr float kSafeValue = 128.f;
+template <int N>
+__device__ __forceinline__ uint32_t keep_zeros(uint32_t (&w)[N], uint32_t byte, float value) {
+  const uint32_t value_exponent = (__float_as_uint(value) >> 23) & 255;
+  if (byte == kNotFinite || value_exponent == 255 || (__float_as_uint(scale_of(byte) * value) & 0x7fffffffu) != 0x7f800000u) return byte;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t below = __vcmpltu4(w[i], kZeroCodes), above = __vcmpgtu4(w[i], kZeroCodes);
+    w[i] = above | (below & 0x01010101u) | (kZeroCodes & ~(above | below));
+  }
+  return 127 + 253 - value_exponent;
+}
+
 }  // namespace rows8
 
 // The weight gradient for a dy of few columns, one row behind the other (rows8_wgrad_narrow.cu); scales and dy 16-byte aligned. Its

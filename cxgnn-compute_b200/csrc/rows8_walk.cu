@@ -5,12 +5,13 @@
 // column, partials of rows that cross tiles added by the same fix-up. Same bits on every run.
 //
 // A lane holds VB codes of a row, which lie in one group of 32 and share a scale. A code becomes fp32 by a byte permutation
-// and an addition (rows8.cuh); code * scale is exact, and so is scale * v (a power of two) but where that leaves the range of
-// normal numbers, so each edge rounds once, in the addition. (Two codes cost 2 permutations, a packed addition and a packed
+// and an addition (rows8.cuh); code * scale is exact, and so is scale * v (a power of two) but where it falls below the normal
+// numbers, so each edge rounds once, in the addition. Tiles with an edge value that could take scale * v out of range are walked
+// once more, edge by edge (walk_carefully). (Two codes cost 2 permutations, a packed addition and a packed
 // multiplication-addition; converting with the conversion instruction would cost a quarter-rate instruction per code.)
 //
 // Measured: 169,343 rows of 128, 2.3 M edges, mean, bf16 99 us (gathered: 3.1 TB/s); 1.94 M rows of 100, 21 M edges with values, fp32
-// 764 us (3.6 TB/s). Bound by instructions and latency together: an edge of 128 columns takes 18 warp instructions, 10 of them
+// 773 us (3.6 TB/s). Bound by instructions and latency together: an edge of 128 columns takes 18 warp instructions, 10 of them
 // to unpack it, a row's end about 80; with codes taken as they are the two graphs take 83 and 676 us.
 #include <type_traits>
 
@@ -88,6 +89,73 @@ __device__ __forceinline__ void add_codes(unsigned long long *acc, const Codes<V
     asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1,%2};\n\tadd.rn.f32x2 t, t, %3;\n\tfma.rn.f32x2 %0, t, %4, %0;\n\t}"
         : "+l"(acc[2 * i + 1])
         : "r"(d), "r"(e), "l"(bias), "l"(ss));
+  }
+}
+
+__device__ __forceinline__ int end_in_tile(uint32_t raw, uint32_t begin) {
+  return raw - begin > static_cast<uint32_t>(kFar) ? kFar : static_cast<int>(raw - begin);
+}
+
+// A tile of rows8_walk with a value per edge once more: the same lanes, sums in the same order, but with keep_zeros at every edge. (A
+// function of its own, which leaves the walk its registers: the walk takes up to 3 % longer for it, with a test per step inside it
+// took 3 to 14 %, with a second walk inside the kernel 2 to 8 %.)
+template <typename T, int VB, int G, int NV, bool SPARSE>
+__device__ __noinline__ void walk_carefully(const Rows8Args &r, int t, int n_tiles) {
+  const WalkArgs &a = r.w;
+  __syncwarp();  // what this warp has stored of the tile is replaced
+  if (t >= n_tiles) return;
+  const int lg = static_cast<int>(threadIdx.x) & (G - 1), n_dst = static_cast<int>(a.n_dst);
+  const uint64_t pitch = static_cast<uint32_t>(a.row_bytes), groups = static_cast<uint32_t>(r.groups);
+  const WalkTile here = load_tile(a, t);
+  const uint32_t begin = here.begin;
+  const int len = static_cast<int>(load_tile(a, t + 1).begin - begin);
+  int row = static_cast<int>(here.row), rend = row < n_dst ? end_in_tile(here.row_end, begin) : kFar;
+  bool whole = here.row_begin >= begin;  // the row began in this tile
+  unsigned long long acc[NV][VB / 2] = {};
+  for (int pos = 0; pos < len; ++pos) {
+    const uint32_t edge = begin + pos;
+    const int64_t given = a.idx_bytes == 8 ? __ldg(static_cast<const int64_t *>(a.idx) + edge)
+                                           : static_cast<int64_t>(__ldg(static_cast<const int32_t *>(a.idx) + edge));
+    const uint64_t id = static_cast<uint64_t>(given) < static_cast<uint64_t>(r.n_src) ? given : r.n_src;
+    const float v = __ldg(a.edge_val + edge);
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      const int at = min((lg + q * G) * VB, a.row_bytes - VB);
+      Codes<VB> c;
+      c.load(r.codes + id * pitch + at);
+      const uint32_t e = keep_zeros<VB / 4>(c.w, __ldg(r.scales + id * groups + at / kGroup), v);
+      add_codes<VB>(acc[q], c, scale_of(e) * v);
+    }
+    const bool row_done = pos + 1 == rend;
+    if (!row_done && pos + 1 < len) continue;
+    T *y = static_cast<T *>(a.y) + static_cast<int64_t>(row) * a.width;
+    float *p = a.partials + (static_cast<int64_t>(t) * 2 + (whole ? 1 : 0)) * a.part_stride;
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+      for (int i = 0; i < VB / 2; ++i) {
+        const float2 f = halves(acc[q][i]);
+        acc[q][i] = 0;
+        const int col = (lg + q * G) * VB + 2 * i;
+        if (row_done && whole) {
+          if (col < a.width) y[col] = from_f32<T>(f.x);
+          if (col + 1 < a.width) y[col + 1] = from_f32<T>(f.y);
+        } else if (row < n_dst && col < a.part_stride) {
+          *reinterpret_cast<float2 *>(p + col) = f;
+        }
+      }
+    if (!row_done || pos + 1 == len) continue;
+    whole = true;
+    if constexpr (SPARSE) {
+      const uint2 mark = __ldg(r.marks + begin + rend);
+      row = static_cast<int>(min(mark.x, static_cast<uint32_t>(n_dst)));
+      rend = row < n_dst ? end_in_tile(mark.y, begin) : kFar;
+    } else {
+      do {  // rows without edges have been written
+        ++row;
+        rend = row < n_dst ? end_in_tile(walk::load_ptr_low(a.ptr, row + 1, a.ptr_bytes), begin) : kFar;
+      } while (rend == pos + 1);
+    }
   }
 }
 
@@ -319,6 +387,7 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
     const int longest = G == 32 ? len : __reduce_max_sync(0xffffffffu, len);
     load_batch(0);
     [[maybe_unused]] uint32_t words[IB];
+    [[maybe_unused]] bool large = false;  // edge values with which scale * value may be out of range
     for (int p = 0; p < longest; p += U) {
       const int in_batch = p & 31;
       if (in_batch == 0) {
@@ -326,7 +395,10 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
 #pragma unroll
         for (int j = 0; j < IB; ++j) {
           my_ids[j * G + lg] = id_nxt[j];
-          if (VALMODE == 1) my_vals[j * G + lg] = val_nxt[j];
+          if (VALMODE == 1) {
+            my_vals[j * G + lg] = val_nxt[j];
+            large = large || !(fabsf(val_nxt[j]) < kSafeValue);
+          }
         }
         __syncwarp();
         if constexpr (kWords) {
@@ -372,6 +444,9 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
           add_codes<VB>(acc[q], c[u][q], VALMODE == 1 ? __uint_as_float(s[u][q]) * vals[u % W4] : __uint_as_float(s[u][q]));
         if (p + u + 1 == stop) event(p + u + 1);
       }
+    }
+    if constexpr (VALMODE == 1) {
+      if (__any_sync(0xffffffffu, large)) walk_carefully<T, VB, G, NV, SPARSE>(r, t, n_tiles);
     }
     t_next = __shfl_sync(0xffffffffu, t_next, 0) + lane / G;
   }

@@ -46,6 +46,9 @@ struct DenseRows {
   using A = Acc<T, VB>;
   static constexpr int EL = A::EL;
   using Loaded = Words<(VB + 3) / 4>;
+  // weights with which what is loaded has to be adapted before it is added: none
+  __device__ __forceinline__ static bool large(float) { return false; }
+  __device__ __forceinline__ static void adapt(Loaded &, float) {}
   const uint8_t *x;
   uint32_t pitch;
   DenseRows() = default;
@@ -79,6 +82,12 @@ struct CodedRows {
   struct Loaded {
     uint32_t codes, scale;
   };
+  __device__ __forceinline__ static bool large(float weight) { return !(fabsf(weight) < rows8::kSafeValue); }
+  __device__ __forceinline__ static void adapt(Loaded &v, float weight) {
+    uint32_t w[1] = {v.codes};
+    v.scale = rows8::keep_zeros<1>(w, v.scale, weight);
+    v.codes = w[0];
+  }
   const uint8_t *codes, *scales;
   uint32_t pitch;
   CodedRows() = default;
@@ -227,6 +236,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
     uint32_t *ids = id_stage[warp] + lane / G * kPitch;
     float *vals = val_stage[warp] + lane / G * kPitch;
     __syncwarp();
+    bool large = false;
     {
       uint32_t id[kPitch / G];
       float val[kPitch / G];
@@ -241,8 +251,9 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
         }
       }
 #pragma unroll
-      for (int j = 0; j < kPitch / G; ++j) ids[j * G + lg] = id[j], vals[j * G + lg] = val[j];
+      for (int j = 0; j < kPitch / G; ++j) ids[j * G + lg] = id[j], vals[j * G + lg] = val[j], large = large || Source::large(val[j]);
     }
+    large = __any_sync(0xffffffffu, large);
     A acc[NV];
 #pragma unroll
     for (int q = 0; q < NV; ++q) acc[q].zero();
@@ -266,6 +277,12 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
       float weights[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) weights[u] = vals[p + u];
+      if (large) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int q = 0; q < NV; ++q) Source::adapt(v[u][q], weights[u]);
+      }
       // the edges of one row after another
       int q0 = 0;
 #pragma unroll 1
