@@ -258,24 +258,21 @@ __device__ __forceinline__ float normalise(Pair (&v)[kPairs], const ResArgs &a, 
   return r;
 }
 
-// sigmoid and its derivative. For fp32 rows without cancellation: t = exp(-|g|), s = 1 / (1 + t) or t / (1 + t), s' = t / (1 + t)^2;
-// the reciprocal of 1 .. 2 is the hardware's, off by an ulp. For bf16 rows, which round to 2^-9, s = 1 / (1 + exp(-g)) and
-// s' = s (1 - s), with the hardware's 2^x of the product rounded once (1e-6 of it at |g| = 16): three instructions less.
+// sigmoid and its derivative without cancellation: t = exp(-|g|), s = 1 / (1 + t) or t / (1 + t), s' = t / (1 + t)^2; the
+// reciprocal of 1 .. 2 is the hardware's, off by an ulp. (s (1 - s) for s' loses half its bits at g = 10 and all from 17 on.) For
+// bf16 rows t is the hardware's 2^x of a product rounded once, off by 2^-22 + |g| 2^-24 of it (1.2e-6 at |g| = 16), where the rows
+// round by 2^-9.
 template <typename T>
 __device__ __forceinline__ void sigmoid(float g, float *s, float *ds) {
   float t, q;
-  if constexpr (sizeof(T) == 2) {
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(g * -1.44269504f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + t));
-    *s = q;
-    *ds = fmaf(-q, q, q);
-  } else {
+  if constexpr (sizeof(T) == 2)
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fabsf(g) * -1.44269504f));
+  else
     t = expf(-fabsf(g));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + t));
-    const float tq = t * q;
-    *s = g >= 0.f ? q : tq;
-    *ds = tq * q;
-  }
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + t));
+  const float tq = t * q;
+  *s = g >= 0.f ? q : tq;
+  *ds = tq * q;
 }
 // The gate's values become sigmoids, and their derivatives where there is room for them.
 template <typename T>

@@ -56,3 +56,14 @@ def test_gradients_of_one_output(cuda, n, width, dtype):
     t, dy, dh = inputs(n, width, dtype, "row", True, True, True, "vector", seed=n)
     _check(t, True, True, True, dy, None)
     _check(t, True, True, True, None, dh)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gate", ["value", "row"])
+@pytest.mark.parametrize("n,width", [(40, 64), (37, 47), (11, 300)])
+def test_gates_far_from_zero(cuda, n, width, gate, dtype):
+    """The sigmoid's derivative is as exact on its flat sides as between them."""
+    t, dy, dh = inputs(n, width, dtype, gate, True, True, False, "vector", seed=n)
+    g = torch.linspace(10, 20, t["gate"].numel()).view(t["gate"].shape)
+    t["gate"] = torch.where(t["gate"] > 0, g, -g).to(dtype)
+    _check(t, True, True, False, dy, dh)
