@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
   if (rows.first < d.n) request(0, rows.first + rows.sub);
   for (int64_t row0 = rows.first; row0 < d.n; row0 += rows.step, turn ^= 1) {
     const int64_t row = row0 + rows.sub;
-    const bool in = kLanes >= 32 || row < d.n;  // lanes without a row go through it with gradients of zero
+    const bool in = kLanes >= 32 || row < d.n;  // lanes without a row go through the last one and add nothing
     const int64_t at = in ? row : d.n - 1;
     const float g_row = to_f32(rr);
     if constexpr (P::kStaged) asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -576,8 +576,8 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
         y[i] = mul2(y[i], rr1);  // u1
-        acc[3][i] = fma2(dh[i], y[i], acc[3][i]);
-        if (BIASES) acc[4][i] = add2(acc[4][i], dh[i]);
+        if (in) acc[3][i] = fma2(dh[i], y[i], acc[3][i]);
+        if (BIASES && in) acc[4][i] = add2(acc[4][i], dh[i]);
         Pair v = fma2(y[i], dots, t[i]);
         if (d.layer) v = add2(v, means);
         t[i] = mul2(v, rr1);
@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
       load_param<P>(w, d.scale, p, width);
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
-        acc[0][i] = fma2(mul2(g[i], s[GATED ? i : 0]), t[i], acc[0][i]);
+        if (in) acc[0][i] = fma2(mul2(g[i], s[GATED ? i : 0]), t[i], acc[0][i]);
         g[i] = mul2(g[i], w[i]);
         t[i] = mul2(mul2(t[i], g[i]), ds[GATED ? i : 0]);  // dgate
         g[i] = mul2(g[i], s[GATED ? i : 0]);               // dn
@@ -620,8 +620,8 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kBa
       if (d.post) {
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
-          acc[1][i] = fma2(g[i], n[i], acc[1][i]);
-          if (BIASES) acc[2][i] = add2(acc[2][i], g[i]);
+          if (in) acc[1][i] = fma2(g[i], n[i], acc[1][i]);
+          if (BIASES && in) acc[2][i] = add2(acc[2][i], g[i]);
           g[i] = mul2(g[i], w2[i]);
         }
         back_through_norm<P>(g, n, r2, a, sum, p);

@@ -67,3 +67,23 @@ def test_gates_far_from_zero(cuda, n, width, gate, dtype):
     g = torch.linspace(10, 20, t["gate"].numel()).view(t["gate"].shape)
     t["gate"] = torch.where(t["gate"] > 0, g, -g).to(dtype)
     _check(t, True, True, False, dy, dh)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gate", ["none", "value", "row"])
+@pytest.mark.parametrize("n,width", [(1, 8), (5, 8), (17, 47), (3, 100), (1, 3)])
+def test_an_infinity_in_the_last_row(cuda, n, width, gate, dtype):
+    """Lanes that have no row of their own add nothing to the sums over rows, whatever the last row holds."""
+    import cxgnncomp_backend as be
+    t, dy, _ = inputs(n, width, dtype, gate, False, False, False, "vector", seed=n)
+    t["f"][-1, 1], t["f"][-1, 2] = float("inf"), -float("inf")
+    dev = {k: None if v is None else v.cuda().requires_grad_(True) for k, v in t.items()}
+    y, _ = _run(be, dev, False, False, False)
+    got = torch.autograd.grad(y, [dev["scale"]], dy.cuda())[0].cpu()
+    s = 1.0 if gate == "none" else torch.sigmoid(t["gate"].double())
+    terms = dy.double() * s * t["f"].double()
+    want = terms.sum(0)
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and not bool(torch.isnan(got).any())
+    assert torch.equal(got[1:3].double(), want[1:3])
+    keep = torch.isfinite(want)
+    assert bool(((got.double() - want).abs() <= 64 * 2.0 ** -24 * terms.abs().sum(0))[keep].all())
