@@ -347,12 +347,17 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
         }
       if (row_done && rstart >= 0) {
         if (VALMODE == 3) {
-          // by the correctly rounded reciprocal: two roundings for one, where a division takes five instructions a value
-          const float inv = __frcp_rn(static_cast<float>(rend - rstart));
+          // fp32: the quotient as f hi + f lo, hi + lo = 1 / count to 2^-44, which is the correctly rounded one for counts below 2^19
+          // (no quotient by d is closer than 2^-25 / d to the middle of two neighbours) and sums above 2^-100. hi is a little below
+          // the reciprocal, so that lo is positive and infinities stay what they are. (A division: 115 us in place of 99.) bf16, which
+          // rounds to 8 bits next: by the correctly rounded reciprocal, which moves one value in 2^15 to its other neighbour (hi and
+          // lo there too: 104 us).
+          const float d = static_cast<float>(rend - rstart), r1 = __frcp_rn(d);
+          const float hi = __uint_as_float(__float_as_uint(r1) - 1), lo = fmaf(-d, hi, 1.f) * r1;
 #pragma unroll
           for (int q = 0; q < NV; ++q)
 #pragma unroll
-            for (int i = 0; i < VB; ++i) f[q][i] *= inv;
+            for (int i = 0; i < VB; ++i) f[q][i] = sizeof(T) == 4 ? fmaf(f[q][i], hi, f[q][i] * lo) : f[q][i] * r1;
         }
         store(row, f);
       } else if (row < n_dst) {
