@@ -899,10 +899,11 @@ std::pair<Tensor, Tensor> rows8_weight_grad(const Tensor &codes, const Tensor &s
   return {dw, db};
 }
 
-// The result of a linear transform in the input's type: the tensor-core kernel for the fp32 matrices it takes, else torch's.
-Tensor plain_linear(const Tensor &x, const Tensor &w, const optional<Tensor> &bias, const optional<Tensor> &add) {
+// The result of a linear transform in the input's type: the tensor-core kernel for the fp32 matrices it takes, else torch's, or
+// always torch's (of_torch).
+Tensor plain_linear(const Tensor &x, const Tensor &w, const optional<Tensor> &bias, const optional<Tensor> &add, bool of_torch) {
   const bool add_fits = !add || (dense_rows(*add) && add->sizes() == at::IntArrayRef({x.size(0), w.size(0)}));
-  if (linear_fits(x, w) && add_fits && (!bias || bias->is_contiguous())) return linear_product(x, w, false, bias, add);
+  if (!of_torch && linear_fits(x, w) && add_fits && (!bias || bias->is_contiguous())) return linear_product(x, w, false, bias, add);
   const Tensor y = at::linear(x, w, bias);
   return add ? *add + y : y;
 }
@@ -911,7 +912,7 @@ Tensor plain_linear(const Tensor &x, const Tensor &w, const optional<Tensor> &bi
 class LinearKept8Function : public torch::autograd::Function<LinearKept8Function> {
  public:
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const optional<Tensor> &bias,
-                        const optional<Tensor> &add, const optional<Tensor> &codes, const optional<Tensor> &scales) {
+                        const optional<Tensor> &add, const optional<Tensor> &codes, const optional<Tensor> &scales, bool same_bits) {
     Held held;
     if (codes)
       held = {*codes, *scales};
@@ -920,7 +921,7 @@ class LinearKept8Function : public torch::autograd::Function<LinearKept8Function
     ctx->save_for_backward({w, held.codes, held.scales});
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["add"] = add.has_value();
-    return plain_linear(x, w, bias, add);
+    return plain_linear(x, w, bias, add, same_bits);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     if (at::GradMode::is_enabled()) fail("linear_kept8: the rows it keeps in 8 bits have no second derivative");
@@ -943,12 +944,12 @@ class LinearKept8Function : public torch::autograd::Function<LinearKept8Function
     } else if (need_db) {
       db = g.sum(0, false, at::kFloat).to(g.scalar_type());
     }
-    return {dx, dw, db, need_add ? grads[0] : Tensor(), Tensor(), Tensor()};
+    return {dx, dw, db, need_add ? grads[0] : Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
 Tensor linear_kept8(Tensor x, Tensor w, optional<Tensor> bias, optional<Tensor> add, const optional<Tensor> &codes,
-                    const optional<Tensor> &scales) {
+                    const optional<Tensor> &scales, bool same_bits) {
   if (for_torch(x, w, bias, add)) fail(std::string("linear_kept8") + kTransform);
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     const auto type = row_type("linear_kept8 under autocast", at::autocast::get_autocast_dtype(at::kCUDA));
@@ -981,8 +982,8 @@ Tensor linear_kept8(Tensor x, Tensor w, optional<Tensor> bias, optional<Tensor> 
   all_recorded_in_capture("linear_kept8", x, w, bias, add);
   c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);
   if (recorded(x, w, bias, add))
-    return LinearKept8Function::apply(x, w, bias, add, codes, scales);
-  return plain_linear(x, w, bias, add);
+    return LinearKept8Function::apply(x, w, bias, add, codes, scales, same_bits);
+  return plain_linear(x, w, bias, add, false);
 }
 
 // ---- the step between two blocks of a residual network -----------------------------------------------------------------

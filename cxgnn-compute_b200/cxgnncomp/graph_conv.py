@@ -1,6 +1,7 @@
 """Layer modules of the aggregation path with the names and forward signatures of the reference
 (cxgnncomp/graph_conv.py). PyG's `Linear` / `glorot` and torch_scatter, which the reference imports, are
 replaced by plain torch (same initialisation: Xavier-uniform weights, zero bias)."""
+import functools
 import math
 
 import torch
@@ -81,7 +82,7 @@ class AggrDirectedOP(torch.autograd.Function):
 class MySageConv(torch.nn.Module):
     """GraphSAGE, mean aggregator (graph_conv.py:117-159). Not in the reference: x may be a cxgnncomp_backend.Rows8 (features
     held in 8 bits, constants); with kept8 the backward pass keeps what the two transforms read in 8 bits instead of the
-    matrices (the weights' gradients are those of the rows in 8 bits, all others as without)."""
+    matrices: the weights' gradients are those of the rows in 8 bits, the result has the same bits as without."""
 
     kept8 = False  # of modules that were saved without it
 
@@ -131,13 +132,14 @@ class MySageConv(torch.nn.Module):
         mean = cxgnncomp_backend.rows8_aggregate(rows, ptr, idx, n, reduce="mean", dtype=dtype)
         root = cxgnncomp_backend.dequantize_rows(rows, num_rows=n, dtype=dtype) if self.root_weight else None
         if self.kept8 and _plain(self.lin_l) and (not self.root_weight or _plain(self.lin_r)):
-            out = cxgnncomp_backend.linear_kept8(mean, self.lin_l.weight, self.lin_l.bias)
-            return out if root is None else cxgnncomp_backend.linear_kept8(root, self.lin_r.weight, add=out, kept=rows)
+            linear = functools.partial(cxgnncomp_backend.linear_kept8, same_bits=True)
+            out = linear(mean, self.lin_l.weight, self.lin_l.bias)
+            return out if root is None else linear(root, self.lin_r.weight, add=out, kept=rows)
         out = self.lin_l(mean)
         return out if root is None else self.lin_r(root, add=out) if isinstance(self.lin_r, Linear) else out + self.lin_r(root)
 
     def _forward_kept8(self, x, ptr, idx, num_node, kept):
-        linear = cxgnncomp_backend.linear_kept8
+        linear = functools.partial(cxgnncomp_backend.linear_kept8, same_bits=True)  # as Linear
         if self.in_channels > self.hidden_channels:
             out = sage_mean_forward(linear(x, self.lin_l.weight, self.lin_l.bias, kept=kept), ptr, idx, num_node)
         else:

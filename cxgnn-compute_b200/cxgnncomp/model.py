@@ -76,8 +76,8 @@ class ResidualGNN(torch.nn.Module):
 
     norm: "rms" or "layer", between two blocks both norms, the gate and the sum in one pass (cxgnncomp_backend.residual_norm).
     gate: None, "row" (one per node) or "value" (one per node and channel), a linear function of the block's input. kept8: what
-    the SAGE blocks' and the gates' transforms read is kept in 8 bits for the backward pass. batch.x may be a
-    cxgnncomp_backend.Rows8. log_softmax at the end."""
+    the SAGE blocks' and the gates' transforms read is kept in 8 bits for the backward pass; the result has the same bits as
+    without. batch.x may be a cxgnncomp_backend.Rows8. log_softmax at the end."""
 
     def __init__(self, conv, in_channels, hidden_channels, out_channels, num_layers, norm="rms", gate=None, kept8=False, dropout=0.0):
         super().__init__()
@@ -142,7 +142,7 @@ class ResidualGNN(torch.nn.Module):
             gate = None
             if self.gate is not None:
                 lin = self.gates[i]
-                gate = cxgnncomp_backend.linear_kept8(h, lin.weight, lin.bias, **kept) if rows else lin(h)
+                gate = cxgnncomp_backend.linear_kept8(h, lin.weight, lin.bias, same_bits=True, **kept) if rows else lin(h)
             x, h, *rows = step(i + 1, x, f, gate)
         return self.lin_out(h).log_softmax(dim=-1)
 

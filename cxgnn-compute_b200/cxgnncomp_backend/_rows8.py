@@ -110,16 +110,17 @@ def rows8_weight_grad(rows, grad, bias=False):
     return (dw, db) if bias else dw
 
 
-def linear_kept8(x, weight, bias=None, add=None, kept=None):
+def linear_kept8(x, weight, bias=None, add=None, kept=None, same_bits=False):
     """x @ weight^T (+ bias) (+ add) for x [n, in] and weight [out, in], all float32 or all bfloat16, whose backward pass keeps x
-    in 8 bits instead of x itself: result and x's gradient are those of `linear`, the weight's gradient that of the rows in 8
-    bits. kept: rows in 8 bits whose first n are x, where the caller has them already (not to be written before the backward
-    pass). Once differentiable."""
+    in 8 bits instead of x itself: result and x's gradient are those of `linear` (same_bits as there; the products of bfloat16 are
+    torch's), the weight's gradient that of the rows in 8 bits. kept: rows in 8 bits whose first n are x, where the caller has them
+    already (not to be written before the backward pass). Once differentiable."""
     if kept is not None:
         _rows8(kept, "linear_kept8")
         if kept.width != x.shape[-1]:
             raise RuntimeError("linear_kept8: kept must hold the rows of x")
-    return _native.linear_kept8(x, weight, bias, add, None if kept is None else kept.codes, None if kept is None else kept.scales)
+    return _native.linear_kept8(x, weight, bias, add, None if kept is None else kept.codes, None if kept is None else kept.scales,
+                                bool(same_bits))
 
 
 def residual_norm(x, f=None, gate=None, scale=None, post=True, post_weight=None, post_bias=None, next=True, next_weight=None,
