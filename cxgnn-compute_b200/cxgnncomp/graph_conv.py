@@ -141,6 +141,10 @@ class MySageConv(torch.nn.Module):
     def _forward_kept8(self, x, ptr, idx, num_node, kept):
         linear = functools.partial(cxgnncomp_backend.linear_kept8, same_bits=True)  # as Linear
         if self.in_channels > self.hidden_channels:
+            if kept is None and self.root_weight and torch.is_grad_enabled() and self.lin_l.weight.requires_grad:
+                # both transforms read x: one copy of it in 8 bits (of what they multiply)
+                operand = x.to(torch.get_autocast_dtype("cuda")) if torch.is_autocast_enabled("cuda") else x
+                kept = cxgnncomp_backend.quantize_rows(operand.detach())
             out = sage_mean_forward(linear(x, self.lin_l.weight, self.lin_l.bias, kept=kept), ptr, idx, num_node)
         else:
             out = linear(sage_mean_forward(x, ptr, idx, num_node), self.lin_l.weight, self.lin_l.bias)

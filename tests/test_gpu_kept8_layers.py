@@ -52,3 +52,30 @@ def test_a_layer_over_features_in_8_bits_gives_the_same_bits(cuda, n_in, n_out):
     kept, plain = _pair(lambda: cxgnncomp.MySageConv(n_in, n_out, kept8=True).cuda())
     a, b = kept(rows, ptr, idx, 500), plain(rows, ptr, idx, 500)
     assert a.requires_grad and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+def test_a_narrowing_layer_keeps_one_copy_of_what_it_reads(cuda, autocast):
+    """Both transforms of a layer that narrows read the same rows."""
+    import cxgnncomp
+    n, n_in, n_out = 20000, 256, 16
+    ptr, idx = (t.cuda() for t in random_csr(n, n, 3, seed=2))
+    torch.manual_seed(1)
+    conv = cxgnncomp.MySageConv(n_in, n_out, kept8=True).cuda()
+    x = torch.randn(n, n_in, device="cuda")
+    dy = randn((n, n_out), 4).cuda()
+    with torch.autocast("cuda", torch.bfloat16, enabled=autocast):
+        y = conv(x, ptr, idx, n)  # what is kept once, per graph or library
+        del y
+        before = torch.cuda.memory_allocated()
+        y = conv(x, ptr, idx, n)
+    held = torch.cuda.memory_allocated() - before - y.numel() * y.element_size()
+    rows = (n + 1) * (n_in + n_in // 32)
+    assert rows <= held < 1.5 * rows
+    want = torch.autograd.grad(y, list(conv.parameters()), dy.to(y.dtype))
+    # the weights' gradients with rows that the caller has are the same
+    import cxgnncomp_backend as be
+    with torch.autocast("cuda", torch.bfloat16, enabled=autocast):
+        z = conv(x, ptr, idx, n, kept=be.quantize_rows(x.bfloat16() if autocast else x))
+    got = torch.autograd.grad(z, list(conv.parameters()), dy.to(z.dtype))
+    assert torch.equal(y, z) and all(torch.equal(a, b) for a, b in zip(got, want))
