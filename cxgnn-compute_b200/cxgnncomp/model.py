@@ -5,7 +5,7 @@ import torch.nn.functional as F
 
 import cxgnncomp_backend
 
-from .graph_conv import Linear, MyGATConv, MyGCNConv, MyGINConv, MyRGCNConv, MySageConv
+from .graph_conv import Linear, _plain, MyGATConv, MyGCNConv, MyGINConv, MyRGCNConv, MySageConv
 
 
 def get_conv_from_str(name, in_channels, out_channels, num_heads=1, num_rel=1, concat=False):
@@ -77,7 +77,8 @@ class ResidualGNN(torch.nn.Module):
     norm: "rms" or "layer", between two blocks both norms, the gate and the sum in one pass (cxgnncomp_backend.residual_norm).
     gate: None, "row" (one per node) or "value" (one per node and channel), a linear function of the block's input. kept8: what
     the SAGE blocks' and the gates' transforms read is kept in 8 bits for the backward pass; the result has the same bits as
-    without. batch.x may be a cxgnncomp_backend.Rows8. log_softmax at the end."""
+    without. batch.x may be a cxgnncomp_backend.Rows8, which with kept8 is not to be written before the backward pass.
+    log_softmax at the end."""
 
     def __init__(self, conv, in_channels, hidden_channels, out_channels, num_layers, norm="rms", gate=None, kept8=False, dropout=0.0):
         super().__init__()
@@ -120,9 +121,16 @@ class ResidualGNN(torch.nn.Module):
     def forward(self, batch):
         L, layer = self.num_layers, self.norm == "layer"
         x = batch.x
-        if isinstance(x, cxgnncomp_backend.Rows8):
-            x = cxgnncomp_backend.dequantize_rows(x, dtype=self.lin_in.weight.dtype)
         keep = self.kept8 and torch.is_grad_enabled()
+        if isinstance(x, cxgnncomp_backend.Rows8):
+            values = cxgnncomp_backend.dequantize_rows(x, dtype=self.lin_in.weight.dtype)
+            # the rows hold what is multiplied: the backward pass reads them (rows made in inference mode cannot be kept for one)
+            of_rows = keep and _plain(self.lin_in) and not x.codes.is_inference()
+            x = (cxgnncomp_backend.linear_kept8(values, self.lin_in.weight, self.lin_in.bias, kept=x, same_bits=True) if of_rows
+                 else self.lin_in(values))
+            del values
+        else:
+            x = self.lin_in(x)
 
         def step(i, x, f, gate):
             """The step in front of block i, or behind the last one."""
@@ -131,7 +139,7 @@ class ResidualGNN(torch.nn.Module):
                 post_bias=self.post_bias[i - 1] if i > 0 and layer else None, next_weight=self.next_weight[i],
                 next_bias=self.next_bias[i] if layer else None, norm=self.norm, keep8=keep and i < L)
 
-        x, h, *rows = step(0, self.lin_in(x), None, None)
+        x, h, *rows = step(0, x, None, None)
         for i, conv in enumerate(self.convs):
             n = int(batch.num_node_in_layer[L - 1 - i])
             e = int(batch.num_edge_in_layer[L - 1 - i]) if batch.num_edge_in_layer is not None else batch.idx.shape[0]

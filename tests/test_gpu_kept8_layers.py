@@ -79,3 +79,38 @@ def test_a_narrowing_layer_keeps_one_copy_of_what_it_reads(cuda, autocast):
         z = conv(x, ptr, idx, n, kept=be.quantize_rows(x.bfloat16() if autocast else x))
     got = torch.autograd.grad(z, list(conv.parameters()), dy.to(z.dtype))
     assert torch.equal(y, z) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_a_model_over_features_in_8_bits_keeps_no_matrix_of_them(cuda, inference):
+    import cxgnncomp
+    import cxgnncomp_backend as be
+    n, n_in = 20000, 500
+    ptr, idx = (t.cuda() for t in random_csr(n, n, 3, seed=2))
+    x = randn((n, n_in), 3).cuda()
+    with torch.inference_mode(inference):
+        rows = be.quantize_rows(x)
+    batch = cxgnncomp.Batch(rows, ptr, idx, num_node_in_layer=[n] * 2, num_edge_in_layer=[idx.shape[0]])
+    torch.manual_seed(1)
+    model = cxgnncomp.ResidualGNN("sage", n_in, 16, 4, 1, kept8=True).cuda()
+    target = torch.randint(0, 4, (n,), generator=torch.Generator().manual_seed(1)).cuda()
+
+    def grads(m, b):
+        out = m(b)
+        return out.detach(), torch.autograd.grad(torch.nn.functional.nll_loss(out, target), list(m.parameters()))
+
+    out, got = grads(model, batch)
+    before = torch.cuda.memory_allocated()
+    kept = model(batch)
+    held = torch.cuda.memory_allocated() - before
+    assert (held < n * n_in) or inference  # the matrix would be four times as much; about 20 vectors of 16 values a row are kept
+    del kept
+    # the same model over the values that the rows hold
+    batch.x = be.dequantize_rows(rows)
+    want_out, want = grads(model, batch)
+    assert torch.equal(out, want_out)
+    for k, a, b in zip(dict(model.named_parameters()), got, want):
+        # the first transform's gradients: sums of 20000 terms on either side, each rounded to 2^-24 of terms that cancel to about
+        # 1 / sqrt(20000) of their sizes
+        first = k in ("lin_in.weight", "lin_in.bias")
+        assert torch.equal(a, b) or (first and float((a - b).norm()) <= 2.0 ** -24 * 20000 ** 0.5 * float(b.norm())), k
