@@ -12,7 +12,8 @@ from . import _native
 
 class Rows8:
     """`rows` rows of `width` values in 8 bits on a CUDA device, zeros at first: pitch + pitch / 32 bytes a row, pitch being
-    `width` in whole groups of 32. quantize_rows writes them, dequantize_rows, rows8_aggregate and rows8_weight_grad read them."""
+    `width` in whole groups of 32, and four more from the first write at an index on. quantize_rows writes them, dequantize_rows,
+    rows8_aggregate and rows8_weight_grad read them."""
     __slots__ = ("rows", "width", "codes", "scales", "_claims")
 
     def __init__(self, rows, width, device="cuda"):
@@ -40,7 +41,7 @@ class Rows8:
 
     @property
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
+        return self.codes.numel() + self.scales.numel() + (0 if self._claims is None else self._claims.nbytes)
 
     def __len__(self):
         return self.rows

@@ -79,3 +79,15 @@ def test_a_cache_without_rows(cuda):
     cache = be.Rows8(0, 40)
     be.quantize_rows(torch.ones(3, 40, device="cuda"), out=cache, index=torch.tensor([0, -1, 5], device="cuda"))
     assert be.dequantize_rows(cache).shape == (0, 40)
+
+
+def test_bytes(cuda):
+    """All that a cache holds: codes and scales of its rows and of one of zeros, a word per row where rows are written by id."""
+    import cxgnncomp_backend as be
+    base = torch.cuda.memory_allocated()
+    cache = be.Rows8(10000, 47)
+    assert cache.nbytes == 10001 * 66
+    be.quantize_rows(torch.ones(3, 47, device="cuda"), out=cache, index=torch.arange(3, device="cuda"))
+    assert cache.nbytes == 10001 * 66 + 40000
+    held = torch.cuda.memory_allocated() - base
+    assert cache.nbytes <= held < cache.nbytes + 3 * 512  # (blocks of 512 bytes)
