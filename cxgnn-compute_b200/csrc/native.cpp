@@ -716,9 +716,10 @@ const char *const kTransform = " does not take tensors of a transform (vmap, for
 
 int code_of(const Tensor &t) { return t.scalar_type() == at::kFloat ? CXG_F32 : CXG_BF16; }
 
-// Whether the backward pass that a call records would lead from a graph capture into another stream's nodes: those of a leaf
-// that an eager graph still holds, or of a tensor that was computed outside the capture. torch's engine then makes the other
-// stream wait for a captured event, which ends the process.
+// Whether the backward pass that a call records would lead from a graph capture into nodes of the default stream: those of a leaf
+// that an eager graph still holds, or of a tensor that was computed outside the capture. torch's engine then makes that stream
+// wait for a captured event, which breaks the capture and can end the process. (Any other stream joins the capture by that wait,
+// and the engine joins it back: steps that were run on a side stream first may stay alive.)
 void recorded_in_capture(const char *who, const Tensor &t) {
   if (!t.defined() || !t.requires_grad() || !at::GradMode::is_enabled()) return;
   const auto stream = c10::cuda::getCurrentCUDAStream(t.device().index());
@@ -726,8 +727,8 @@ void recorded_in_capture(const char *who, const Tensor &t) {
   const auto node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
   if (!node) return;
   const auto of = node->stream();
-  if (of && *of != stream.unwrap())
-    fail(std::string(who) + ": under capture, with gradients recorded, of a tensor whose graph belongs to another stream and is still "
+  if (of && *of != stream.unwrap() && c10::cuda::CUDAStream(c10::cuda::CUDAStream::UNCHECKED, *of).stream() == nullptr)
+    fail(std::string(who) + ": under capture, with gradients recorded, of a tensor whose graph belongs to the default stream and is still "
                             "alive: drop what was computed from it before the capture");
 }
 void recorded_in_capture(const char *who, const optional<Tensor> &t) {
