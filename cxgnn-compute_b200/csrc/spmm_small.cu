@@ -46,7 +46,7 @@ struct DenseRows {
   using A = Acc<T, VB>;
   static constexpr int EL = A::EL;
   using Loaded = Words<(VB + 3) / 4>;
-  // weights with which what is loaded has to be adapted before it is added: none
+  static constexpr bool kAdapts = false;  // are there weights with which what is loaded has to be adapted before it is added
   __device__ __forceinline__ static bool large(float) { return false; }
   __device__ __forceinline__ static void adapt(Loaded &, float) {}
   const uint8_t *x;
@@ -82,6 +82,7 @@ struct CodedRows {
   struct Loaded {
     uint32_t codes, scale;
   };
+  static constexpr bool kAdapts = true;
   __device__ __forceinline__ static bool large(float weight) { return !(fabsf(weight) < rows8::kSafeValue); }
   __device__ __forceinline__ static void adapt(Loaded &v, float weight) {
     uint32_t w[1] = {v.codes};
@@ -253,7 +254,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
 #pragma unroll
       for (int j = 0; j < kPitch / G; ++j) ids[j * G + lg] = id[j], vals[j * G + lg] = val[j], large = large || Source::large(val[j]);
     }
-    large = __any_sync(0xffffffffu, large);
+    if constexpr (Source::kAdapts) large = __any_sync(0xffffffffu, large);
     A acc[NV];
 #pragma unroll
     for (int q = 0; q < NV; ++q) acc[q].zero();
@@ -277,7 +278,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kSmallThreads) w
       float weights[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) weights[u] = vals[p + u];
-      if (large) {
+      if (Source::kAdapts && large) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
