@@ -31,6 +31,14 @@ class Rows8:
         r.rows, r.width, r.codes, r.scales, r._claims = codes.shape[0] - 1, width, codes, scales, None
         return r
 
+    def __getstate__(self):
+        return {"rows": self.rows, "width": self.width, "codes": self.codes, "scales": self.scales}
+
+    def __setstate__(self, state):
+        state = state[1] if isinstance(state, tuple) else state  # (as it was saved when the words went with it)
+        self.rows, self.width, self.codes, self.scales = (state[k] for k in ("rows", "width", "codes", "scales"))
+        self._claims = None  # between two calls they hold nothing
+
     @property
     def shape(self):
         return torch.Size((self.rows, self.width))

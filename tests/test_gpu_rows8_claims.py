@@ -91,3 +91,22 @@ def test_bytes(cuda):
     assert cache.nbytes == 10001 * 66 + 40000
     held = torch.cuda.memory_allocated() - base
     assert cache.nbytes <= held < cache.nbytes + 3 * 512  # (blocks of 512 bytes)
+
+
+def test_copies_and_saved_caches(cuda):
+    """The words stay behind: those of a cache that was saved may be of another form."""
+    import copy
+    import pickle
+    import cxgnncomp_backend as be
+    x, at = torch.ones(3, 40, device="cuda"), torch.tensor([4, 1, 4], device="cuda")
+    cache = be.Rows8(6, 40)
+    be.quantize_rows(x, out=cache, index=at)
+    old = be.Rows8.__new__(be.Rows8)
+    old.__setstate__((None, {"rows": 6, "width": 40, "codes": cache.codes.clone(), "scales": cache.scales.clone(),
+                             "_claims": torch.full((7,), 2 ** 32 + 3, device="cuda")}))
+    before = be.dequantize_rows(cache)
+    # (the last one shares its rows with the cache itself)
+    for other in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache)), old, copy.copy(cache)):
+        assert other.shape == cache.shape and torch.equal(be.dequantize_rows(other), before)
+        be.quantize_rows(torch.stack([x[0] * 2, x[0] * 3, x[0] * 5]), out=other, index=at)
+        assert float(be.dequantize_rows(other)[4, 0]) == 5 and float(be.dequantize_rows(other)[1, 0]) == 3
