@@ -18,7 +18,7 @@
 // The sums over rows are kept per lane for the whole grid's pass, added up per block, and the blocks' sums are added in order
 // by a second kernel: the same bits on every run.
 //
-// Measured: 169,343 rows of 256 bf16, rms, a gate per value: forward 78 us (5.6 TB/s), backward 134 (5.2 TB/s, 470 instructions a
+// Measured: 169,343 rows of 256 bf16, rms, a gate per value: forward 78 us (5.6 TB/s), backward 137 (5.1 TB/s, 493 instructions a
 // row and warp at 2.4 per cycle: what bounds it); 250,000 rows of 128 fp32, layer norm, a gate per row, both 227 us (5.6 TB/s).
 #include <initializer_list>
 
@@ -261,10 +261,15 @@ __device__ __forceinline__ float normalise(Pair (&v)[kPairs], const ResArgs &a, 
 // sigmoid and its derivative without cancellation: t = exp(-|g|), s = 1 / (1 + t) or t / (1 + t), s' = t / (1 + t)^2; the
 // reciprocal of 1 .. 2 is the hardware's, off by an ulp. (s (1 - s) for s' loses half its bits at g = 10 and all from 17 on.) For
 // bf16 rows t is the hardware's 2^x of a product rounded once, off by 2^-22 + |g| 2^-24 of it (1.2e-6 at |g| = 16), where the rows
-// round by 2^-9.
+// round by 2^-9; where s alone is asked for it is 1 / (1 + exp(-g)), which loses nothing, two instructions less.
 template <typename T>
 __device__ __forceinline__ void sigmoid(float g, float *s, float *ds) {
   float t, q;
+  if (sizeof(T) == 2 && ds == nullptr) {
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(g * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(*s) : "f"(1.f + t));
+    return;
+  }
   if constexpr (sizeof(T) == 2)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fabsf(g) * -1.44269504f));
   else
@@ -272,7 +277,7 @@ __device__ __forceinline__ void sigmoid(float g, float *s, float *ds) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + t));
   const float tq = t * q;
   *s = g >= 0.f ? q : tq;
-  *ds = tq * q;
+  if (ds != nullptr) *ds = tq * q;
 }
 // The gate's values become sigmoids, and their derivatives where there is room for them.
 template <typename T>
@@ -281,8 +286,8 @@ __device__ __forceinline__ void sigmoids(Pair (&s)[kPairs], Pair *ds) {
   for (int i = 0; i < kPairs; ++i) {
     const float2 g = halves(s[i]);
     float a, b, da, db;
-    sigmoid<T>(g.x, &a, &da);
-    sigmoid<T>(g.y, &b, &db);
+    sigmoid<T>(g.x, &a, ds != nullptr ? &da : nullptr);
+    sigmoid<T>(g.y, &b, ds != nullptr ? &db : nullptr);
     s[i] = pair(a, b);
     if (ds != nullptr) ds[i] = pair(da, db);
   }
@@ -408,8 +413,8 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : kBlock, blocks_of(kFo
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) w[i] = mul2(w[i], s[i]);
       } else if (row_gate) {
-        float one, ds;
-        sigmoid<T>(g_row, &one, &ds);
+        float one;
+        sigmoid<T>(g_row, &one, nullptr);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) w[i] = mul2(w[i], pair(one, one));
       }
