@@ -2,7 +2,8 @@
 //   dW[o][i] = sum over the rows r of dy[r][o] * codes[r][i] * scale[r][i / 32],   db[o] = sum over the rows of dy[r][o]
 //
 // codes * scale has 7 bits and is an exact bf16 operand; fp32 dy is cut into three bf16 parts of 8 bits each, which hold all 24
-// of its bits: dy = hi + mid + lo exactly. So every product is exact and a sum of m rows takes three bf16 instructions' worth
+// of its bits: dy = hi + mid + lo exactly (from 2^-110 on; below, the last bits of lo are under bf16's smallest number, 2^-133). So
+// every product is exact and a sum of m rows takes three bf16 instructions' worth
 // of tensor core time (one for bf16 dy), where compensated TF32 would take three of half the rate and lose bits.
 //
 // The contraction runs over rows, so both operands are "MN-major": a stage holds 64 rows of the input (A: 128 columns, two

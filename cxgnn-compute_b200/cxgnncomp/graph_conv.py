@@ -81,7 +81,8 @@ class AggrDirectedOP(torch.autograd.Function):
 
 class MySageConv(torch.nn.Module):
     """GraphSAGE, mean aggregator (graph_conv.py:117-159). Not in the reference: x may be a cxgnncomp_backend.Rows8 (features
-    held in 8 bits, constants); with kept8 the backward pass keeps what the two transforms read in 8 bits instead of the
+    held in 8 bits, constants; the mean then always comes first, so that a node without neighbours gets the bias, where a matrix in
+    a layer that narrows is transformed first, as the reference does, and its nodes without neighbours do not); with kept8 the backward pass keeps what the two transforms read in 8 bits instead of the
     matrices: the weights' gradients are those of the rows in 8 bits, the result has the same bits as without."""
 
     kept8 = False  # of modules that were saved without it

@@ -113,7 +113,8 @@ def rows8_aggregate(rows, ptr, idx, num_node, reduce="sum", edge_value=None, dty
 
 def rows8_weight_grad(rows, grad, bias=False):
     """grad^T . rows (float32 [out, width]) for grad [n, out] and the first n rows: the gradient of a weight [out, width] from
-    the layer's input in 8 bits; with bias=True (that, the sum of grad's rows, float32 [out]). Summed in a fixed order."""
+    the layer's input in 8 bits; with bias=True (that, the sum of grad's rows, float32 [out]). Summed in a fixed order; no gradient
+    goes through."""
     _rows8(rows, "rows8_weight_grad")
     dw, db = _native.rows8_weight_grad(rows.codes, rows.scales, rows.width, grad, bool(bias))
     return (dw, db) if bias else dw

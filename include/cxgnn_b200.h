@@ -690,7 +690,7 @@ int cxg_rows8_write_at(const void *x, int dtype, int64_t ld, int64_t n, int widt
 int cxg_rows8_read(const void *codes, const void *scales, int64_t rows, int width, const int64_t *index, int64_t n, void *out,
                    int dtype, int64_t ld, void *stream);
 /* y[d, :] = sum or mean over row d of the CSR graph of [edge_val[e] *] row idx[e]: cxg_spmm_csr over rows in 8 bits, sums in
-   fp32 in edge order, the same bits on every run. idx outside [0, n_src): a row of zeros. y: [n_dst, width] of y_dtype.
+   fp32 in edge order, the same bits on every run; held zeros stay zeros times any finite edge value. idx outside [0, n_src): a row of zeros. y: [n_dst, width] of y_dtype.
    Widths up to 2048; split_edges as in cxg_spmm_desc. Rows and edges below 2^31 - 2^20. An edge count ptr[n_dst] above nnz is
    cut to nnz and reported by cxg_spmm_csr_status(workspace). */
 int cxg_rows8_aggregate_workspace_size(int64_t nnz, int width, int split_edges, size_t *bytes);
