@@ -7,7 +7,7 @@
 // A lane holds VB codes of a row, which lie in one group of 32 and share a scale. A code becomes fp32 by a byte permutation
 // and an addition (rows8.cuh); code * scale is exact, and so is scale * v (a power of two) but where it falls below the normal
 // numbers, so each edge rounds once, in the addition. Tiles with an edge value that could take scale * v out of range are walked
-// once more, edge by edge (walk_carefully). (Two codes cost 2 permutations, a packed addition and a packed
+// once more, edge by edge, if it does (walk_carefully). (Two codes cost 2 permutations, a packed addition and a packed
 // multiplication-addition; converting with the conversion instruction would cost a quarter-rate instruction per code.)
 //
 // Measured: 169,343 rows of 128, 2.3 M edges, mean, bf16 99 us (gathered: 3.1 TB/s); 1.94 M rows of 100, 21 M edges with values, fp32
@@ -96,28 +96,71 @@ __device__ __forceinline__ int end_in_tile(uint32_t raw, uint32_t begin) {
   return raw - begin > static_cast<uint32_t>(kFar) ? kFar : static_cast<int>(raw - begin);
 }
 
-// A tile of rows8_walk with a value per edge once more: the same lanes, sums in the same order, but with keep_zeros at every edge. (A
-// function of its own, which leaves the walk its registers: the walk takes up to 3 % longer for it, with a test per step inside it
-// took 3 to 14 %, with a second walk inside the kernel 2 to 8 %.)
-template <typename T, int VB, int G, int NV, bool SPARSE>
+// Whether a finite value takes one of the finite scales of a word out of range.
+__device__ __forceinline__ bool out_of_range(uint32_t bytes, float v) {
+  bytes &= ~__vcmpeq4(bytes, 0xffffffffu);
+  const uint32_t top = max(max(bytes & 255u, (bytes >> 8) & 255u), max((bytes >> 16) & 255u, bytes >> 24));
+  return fabsf(v) < __uint_as_float(0x7f800000u) && __float_as_uint(scale_of(top) * fabsf(v)) == 0x7f800000u;
+}
+
+// A tile of rows8_walk with edge values of kSafeValue or more: looks (unless SEEN: where the walk has) whether one of them takes a
+// scale of its row out of range, a lane per edge, and if so walks the tile once more: the same lanes, sums in the same order, but
+// with keep_zeros at every edge. (A function of its own, which leaves the walk its registers: the walk takes up to 3 % longer for
+// it, with a test per step inside it took 3 to 14 %, with a second walk inside the kernel 2 to 8 %, with a test of the sums for NaN
+// 6 %. Where all values are that large, looking takes 10 to 15 %, in the walk itself 2 %.)
+template <typename T, int VB, int G, int NV, bool SPARSE, bool SEEN>
 __device__ __noinline__ void walk_carefully(const Rows8Args &r, int t, int n_tiles) {
   const WalkArgs &a = r.w;
-  __syncwarp();  // what this warp has stored of the tile is replaced
-  if (t >= n_tiles) return;
   const int lg = static_cast<int>(threadIdx.x) & (G - 1), n_dst = static_cast<int>(a.n_dst);
   const uint64_t pitch = static_cast<uint32_t>(a.row_bytes), groups = static_cast<uint32_t>(r.groups);
-  const WalkTile here = load_tile(a, t);
+  WalkTile here = {};
+  int len = 0;
+  if (t < n_tiles) {
+    here = load_tile(a, t);
+    len = static_cast<int>(load_tile(a, t + 1).begin - here.begin);
+  }
   const uint32_t begin = here.begin;
-  const int len = static_cast<int>(load_tile(a, t + 1).begin - begin);
+  auto row_of = [&](uint32_t edge) -> uint64_t {
+    const int64_t id = a.idx_bytes == 8 ? __ldg(static_cast<const int64_t *>(a.idx) + edge)
+                                        : static_cast<int64_t>(__ldg(static_cast<const int32_t *>(a.idx) + edge));
+    return static_cast<uint64_t>(id) < static_cast<uint64_t>(r.n_src) ? id : r.n_src;
+  };
+  if constexpr (!SEEN) {
+    bool out = false;
+    constexpr int kDeep = 4;  // edges of a lane at once
+    for (int first = lg; first < len; first += kDeep * G) {
+      float v[kDeep];
+      uint64_t id[kDeep];
+      uint32_t top[kDeep] = {};  // the largest bytes of finite groups
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        const bool on = first + u * G < len;
+        v[u] = on ? __ldg(a.edge_val + begin + first + u * G) : 0.f;
+        id[u] = on ? row_of(begin + first + u * G) : static_cast<uint64_t>(r.n_src);
+        if (fabsf(v[u]) < kSafeValue) id[u] = static_cast<uint64_t>(r.n_src);
+      }
+      auto take = [&](int u, uint32_t bytes) { top[u] = __vmaxu4(top[u], bytes & ~__vcmpeq4(bytes, 0xffffffffu)); };
+      if (groups % 4 == 0) {
+        for (uint32_t g = 0; g < groups; g += 4)
+#pragma unroll
+          for (int u = 0; u < kDeep; ++u) take(u, __ldg(reinterpret_cast<const uint32_t *>(r.scales + id[u] * groups + g)));
+      } else {
+        for (uint32_t g = 0; g < groups; ++g)
+#pragma unroll
+          for (int u = 0; u < kDeep; ++u) take(u, __ldg(r.scales + id[u] * groups + g));
+      }
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) out = out || out_of_range(top[u], v[u]);
+    }
+    if (!__any_sync(0xffffffffu, out)) return;
+  }
+  __syncwarp();  // what this warp has stored of the tile is replaced
   int row = static_cast<int>(here.row), rend = row < n_dst ? end_in_tile(here.row_end, begin) : kFar;
   bool whole = here.row_begin >= begin;  // the row began in this tile
   unsigned long long acc[NV][VB / 2] = {};
   for (int pos = 0; pos < len; ++pos) {
-    const uint32_t edge = begin + pos;
-    const int64_t given = a.idx_bytes == 8 ? __ldg(static_cast<const int64_t *>(a.idx) + edge)
-                                           : static_cast<int64_t>(__ldg(static_cast<const int32_t *>(a.idx) + edge));
-    const uint64_t id = static_cast<uint64_t>(given) < static_cast<uint64_t>(r.n_src) ? given : r.n_src;
-    const float v = __ldg(a.edge_val + edge);
+    const uint64_t id = row_of(begin + pos);
+    const float v = __ldg(a.edge_val + begin + pos);
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       const int at = min((lg + q * G) * VB, a.row_bytes - VB);
@@ -392,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
     const int longest = G == 32 ? len : __reduce_max_sync(0xffffffffu, len);
     load_batch(0);
     [[maybe_unused]] uint32_t words[IB];
-    [[maybe_unused]] bool large = false;  // edge values with which scale * value may be out of range
+    [[maybe_unused]] bool large = false;  // edge values with which scale * value is (WORDS) or may be out of range
     for (int p = 0; p < longest; p += U) {
       const int in_batch = p & 31;
       if (in_batch == 0) {
@@ -402,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
           my_ids[j * G + lg] = id_nxt[j];
           if (VALMODE == 1) {
             my_vals[j * G + lg] = val_nxt[j];
-            large = large || !(fabsf(val_nxt[j]) < kSafeValue);
+            if (!kWords) large = large || !(fabsf(val_nxt[j]) < kSafeValue);
           }
         }
         __syncwarp();
@@ -431,6 +474,13 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
         if (in_batch == 0) {  // the words have been on their way together with the codes
 #pragma unroll
           for (int j = 0; j < IB; ++j) my_scales[j * G + lg] = words[j];
+          if constexpr (VALMODE == 1) {
+#pragma unroll
+            for (int j = 0; j < IB; ++j) {
+              const float v = my_vals[j * G + lg];
+              if (!(fabsf(v) < kSafeValue)) large = large || out_of_range(words[j], v);
+            }
+          }
           __syncwarp();
         }
       }
@@ -451,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, MINB) rows8_walk(const __grid_consta
       }
     }
     if constexpr (VALMODE == 1) {
-      if (__any_sync(0xffffffffu, large)) walk_carefully<T, VB, G, NV, SPARSE>(r, t, n_tiles);
+      if (__any_sync(0xffffffffu, large)) walk_carefully<T, VB, G, NV, SPARSE, kWords>(r, t, n_tiles);
     }
     t_next = __shfl_sync(0xffffffffu, t_next, 0) + lane / G;
   }
